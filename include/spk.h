@@ -488,6 +488,61 @@ int spk_attn_masked_train_bwd(const void* q, const void* k, const void* v, int d
                               int64_t T, int64_t B, int64_t H, int64_t Nq, int64_t Nk, int64_t dh, const float* g,
                               void* dq, void* dk, void* dv, float* dscale_part, void* stream);
 
+/*
+ * LayerNorm over the last dimension, forward and backward, without a LIF
+ * behind it (the nn.LayerNorm calls of SSA.py:218-249 and SpikingMLP.py:31-36
+ * on their own).  x: [rows][D] of x_dtype (F32/F16/BF16) with row stride `ld`
+ * (elements, >= D); w, b: [D] of their own types or NULL; y: [rows][D] dense
+ * of y_dtype; stats: [rows][2] fp32 (mean, 1/std) or NULL.
+ * Backward: g [rows][D] dense; gx [rows][D] dense of x_dtype, gw [D] of
+ * w_dtype, gb [D] of b_dtype, each may be NULL.  w_dtype is also gw's type
+ * when w is NULL.  Sums are fp32 in a fixed order.
+ */
+int spk_layer_norm_fwd(const void* x, int x_dtype, int64_t ld, const void* w, int w_dtype, const void* b, int b_dtype,
+                       float eps, int64_t rows, int64_t D, void* y, int y_dtype, float* stats, void* stream);
+int64_t spk_layer_norm_bwd_workspace_bytes(int64_t rows, int64_t D);
+int spk_layer_norm_bwd(const void* g, int g_dtype, const void* x, int x_dtype, int64_t ld, const float* stats,
+                       const void* w, int w_dtype, int64_t rows, int64_t D, void* gx, void* gw, void* gb, int b_dtype,
+                       void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * Scaled token embedding (TokenEmbedding, Seq2Seq.py:29-36) and the gradient
+ * of its weight.  out[i] = scale * weight[tokens[i]], [n][D] of out_dtype;
+ * weight: [V][D] of w_dtype with row stride ldw.  A token outside [0, V) reads
+ * as zeros and sets *bad_token (which the call clears first).
+ * Backward: gw [V][D] dense of w_dtype = scale * the sum of g's rows over each
+ * token's positions in ascending order (fp32), zeros for rows without a token
+ * and for row padding_idx (-1: none); tokens outside [0, V) are skipped.
+ */
+int spk_embedding_fwd(const int64_t* tokens, const void* weight, int w_dtype, int64_t ldw, float scale, int64_t n,
+                      int64_t V, int64_t D, void* out, int out_dtype, int* bad_token, void* stream);
+int64_t spk_embedding_bwd_workspace_bytes(int64_t n, int64_t V, int64_t D);
+int spk_embedding_bwd(const int64_t* tokens, const void* g, int g_dtype, float scale, int64_t padding_idx, int64_t n,
+                      int64_t V, int64_t D, void* gw, int w_dtype, void* workspace, int64_t workspace_bytes,
+                      void* stream);
+
+/*
+ * Log probabilities of given tokens under the mean over T of the logits, with
+ * entropy and the top_k (<= 32) largest alternatives (falling, ties to the
+ * lower index, NaN smallest).  logits: element (t, r, v) of dtype
+ * (F32/F16/BF16) at t*step_stride + r*row_stride + v; tokens: [rows];
+ * logp, entropy: [rows]; top_logp, top_idx: [rows][top_k] (NULL with top_k 0);
+ * stats: [rows][4] for the backward, 16-byte aligned.  Rows whose token is ignore_index give
+ * zeros and top_idx -1; so do tokens outside [0, V), which set *bad_token
+ * (cleared first).
+ * Backward: grad [T][rows][V] dense of dtype from g_logp [rows], g_entropy
+ * [rows], g_top [rows][top_k], each may be NULL.
+ */
+int64_t spk_token_logprobs_workspace_bytes(int64_t T, int64_t rows, int64_t V, int64_t top_k);
+int spk_token_logprobs_fwd(const void* logits, int dtype, int64_t T, int64_t rows, int64_t V, int64_t step_stride,
+                           int64_t row_stride, const int64_t* tokens, int64_t ignore_index, int64_t top_k, float* logp,
+                           float* entropy, float* top_logp, int64_t* top_idx, float* stats, int* bad_token,
+                           void* workspace, int64_t workspace_bytes, void* stream);
+int spk_token_logprobs_bwd(const void* logits, int dtype, int64_t T, int64_t rows, int64_t V, int64_t step_stride,
+                           int64_t row_stride, const int64_t* tokens, int64_t ignore_index, int64_t top_k,
+                           const int64_t* top_idx, const float* stats, const float* g_logp, const float* g_entropy,
+                           const float* g_top, void* grad, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -66,6 +66,16 @@ SIGNATURES = {
                                    _i64, _i64, _p, _p], _i),
     "spk_attn_masked_train_bwd": ([_p, _p, _p, _i, _p, _p, _i64, _i64, _i64, _i64, _i, _p, _i64, _i64, _i64, _i64,
                                    _i64, _i64, _p, _p, _p, _p, _p, _p], _i),
+    "spk_layer_norm_fwd": ([_p, _i, _i64, _p, _i, _p, _i, _f, _i64, _i64, _p, _i, _p, _p], _i),
+    "spk_layer_norm_bwd_workspace_bytes": ([_i64, _i64], _i64),
+    "spk_layer_norm_bwd": ([_p, _i, _p, _i, _i64, _p, _p, _i, _i64, _i64, _p, _p, _p, _i, _p, _i64, _p], _i),
+    "spk_embedding_fwd": ([_p, _p, _i, _i64, _f, _i64, _i64, _i64, _p, _i, _p, _p], _i),
+    "spk_embedding_bwd_workspace_bytes": ([_i64, _i64, _i64], _i64),
+    "spk_embedding_bwd": ([_p, _p, _i, _f, _i64, _i64, _i64, _i64, _p, _i, _p, _i64, _p], _i),
+    "spk_token_logprobs_workspace_bytes": ([_i64, _i64, _i64, _i64], _i64),
+    "spk_token_logprobs_fwd": ([_p, _i, _i64, _i64, _i64, _i64, _i64, _p, _i64, _i64, _p, _p, _p, _p, _p, _p, _p, _i64,
+                                _p], _i),
+    "spk_token_logprobs_bwd": ([_p, _i, _i64, _i64, _i64, _i64, _i64, _p, _i64, _i64, _p, _p, _p, _p, _p, _p, _p], _i),
     "spk_xnor_train_combine": ([_p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _p], _i),
     "spk_xnor_train_prep_chunks": ([_i64], _i64),
     "spk_xnor_train_grad_prep": ([_p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _p], _i),

@@ -1,0 +1,805 @@
+"""The token-side operators (embedding, LayerNorm, token log probabilities) against
+their definitions in 64 bits.
+
+Tolerances are elementwise bounds computed from the data: u = 2^-24 is half a
+step of fp32, a sum of k terms in a chain errs by at most k u of the terms'
+absolute sum, an output in a narrower type adds half a step of it
+(``torch.finfo(t).eps / 2``).  Where the data are small integers every sum is
+exact in any order, and the comparison is equality.
+"""
+
+import ctypes
+
+import pytest
+import torch
+
+from spikingtransformer_b200 import _lib
+
+DEV = "cuda"
+U = 2.0 ** -24
+FLOATS = [torch.float32, torch.float16, torch.bfloat16]
+
+
+@pytest.fixture(scope="module")
+def ops():
+    from spikingtransformer_b200 import ops as o
+    return o
+
+
+def gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def half_step(dtype):
+    return torch.finfo(dtype).eps / 2
+
+
+def tiny(dtype):
+    """Half the spacing of the type's subnormal numbers."""
+    return torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps / 2
+
+
+def assert_within(got, want, bound, what):
+    got, want, bound = got.detach().double().cpu(), want.detach().double().cpu(), bound.detach().double().cpu()
+    assert got.shape == want.shape, (what, got.shape, want.shape)
+    assert torch.isfinite(got).all(), what
+    over = (got - want).abs() - bound
+    worst = over.max().item() if over.numel() else -1.0
+    assert worst <= 0, "%s: %.3e over its bound (error %.3e)" % (what, worst, (got - want).abs().max().item())
+
+
+# ------------------------------------------------------------------ refusals without a device
+
+
+def test_c_entries_reject_bad_arguments():
+    lib = _lib.load()
+    p = ctypes.c_void_p(16)  # never dereferenced: the checks come first
+    assert lib.spk_layer_norm_fwd(None, 0, 8, None, 0, None, 0, 1e-5, 2, 8, p, 0, None, None) == 1
+    assert lib.spk_layer_norm_fwd(p, 3, 8, None, 0, None, 0, 1e-5, 2, 8, p, 0, None, None) == 1   # u8
+    assert lib.spk_layer_norm_fwd(p, 0, 7, None, 0, None, 0, 1e-5, 2, 8, p, 0, None, None) == 2   # ld < D
+    assert lib.spk_layer_norm_fwd(p, 0, 8, None, 0, None, 0, 1e-5, 0, 8, p, 0, None, None) == 2   # no rows
+    assert lib.spk_layer_norm_bwd(p, 0, p, 0, 8, None, p, 0, 2, 8, p, p, p, 0, p, 1 << 30, None) == 1
+    assert lib.spk_layer_norm_bwd(p, 0, p, 0, 8, p, p, 0, 2, 8, p, p, p, 0, p, 4, None) == 1      # workspace
+    assert lib.spk_embedding_fwd(p, p, 0, 8, 1.0, 4, 10, 8, p, 0, None, None) == 1
+    assert lib.spk_embedding_fwd(p, p, 0, 7, 1.0, 4, 10, 8, p, 0, p, None) == 2
+    assert lib.spk_embedding_fwd(p, p, 5, 8, 1.0, 4, 10, 8, p, 0, p, None) == 1
+    assert lib.spk_embedding_bwd(p, p, 0, 1.0, -1, 4, 0, 8, p, 0, p, 1 << 30, None) == 2
+    assert lib.spk_embedding_bwd(p, p, 0, 1.0, -1, 4, 10, 8, p, 0, p, 0, None) == 1               # workspace
+    args = (p, p, p, p, p, p, p, 1 << 30, None)
+    assert lib.spk_token_logprobs_fwd(None, 0, 1, 2, 8, 0, 8, p, -100, 0, *args) == 1
+    assert lib.spk_token_logprobs_fwd(p, 3, 1, 2, 8, 0, 8, p, -100, 0, *args) == 1
+    assert lib.spk_token_logprobs_fwd(p, 0, 1, 2, 8, 0, 8, p, -100, 9, *args) == 2                # top_k > V
+    assert lib.spk_token_logprobs_fwd(p, 0, 1, 2, 99, 0, 99, p, -100, 33, *args) == 2             # top_k > 32
+    assert lib.spk_token_logprobs_fwd(p, 0, 65, 2, 8, 0, 8, p, -100, 0, *args) == 2
+    assert lib.spk_token_logprobs_fwd(p, 0, 1, 2, 8, 0, -8, p, -100, 0, *args) == 2
+    assert lib.spk_token_logprobs_bwd(p, 0, 1, 2, 8, 0, 8, p, -100, 4, None, p, p, p, p, p, None) == 1  # no indices
+
+
+def test_ops_refuse_cpu_tensors(ops):
+    x, t = torch.zeros(2, 8), torch.zeros(2, dtype=torch.int64)
+    for call in (lambda: ops.layer_norm(x), lambda: ops.embedding(t, x), lambda: ops.token_logprobs(x[None], t)):
+        with pytest.raises(RuntimeError, match="CUDA"):
+            call()
+
+
+@pytest.mark.gpu
+def test_ops_refuse_what_they_do_not_take(ops):
+    x = torch.randn(4, 8, device=DEV)
+    t = torch.zeros(4, dtype=torch.int64, device=DEV)
+    for call, err in [
+            (lambda: ops.layer_norm(x.double()), TypeError),
+            (lambda: ops.layer_norm(x, torch.ones(7, device=DEV)), RuntimeError),
+            (lambda: ops.layer_norm(x, torch.ones(8)), RuntimeError),
+            (lambda: ops.layer_norm(x, out_dtype=torch.uint8), TypeError),
+            (lambda: ops.layer_norm(x[:, :0]), RuntimeError),
+            (lambda: ops.layer_norm_bwd(x[:2], x, torch.zeros(4, 2, device=DEV)), RuntimeError),
+            (lambda: ops.layer_norm_bwd(x, x, torch.zeros(3, 2, device=DEV)), RuntimeError),
+            (lambda: ops.embedding(t.float(), x), TypeError),
+            (lambda: ops.embedding(t, x[0]), RuntimeError),
+            (lambda: ops.embedding(t, x, padding_idx=4), ValueError),
+            (lambda: ops.embedding(t, x, padding_idx=-1), ValueError),
+            (lambda: ops.embedding_bwd(x[:3], t, 8), RuntimeError),
+            (lambda: ops.token_logprobs(x, t), RuntimeError),
+            (lambda: ops.token_logprobs(x[None], t[:3]), RuntimeError),
+            (lambda: ops.token_logprobs(x[None], t, top_k=9), ValueError),
+            (lambda: ops.token_logprobs(x[None], t, top_k=-1), ValueError),
+            (lambda: ops.token_logprobs(x[None].double(), t), TypeError),
+            (lambda: ops.token_logprobs(x[None], t.bool()), TypeError)]:
+        with pytest.raises(err):
+            call()
+
+
+@pytest.mark.gpu
+def test_second_derivatives_are_refused(ops):
+    x = torch.randn(4, 8, device=DEV, requires_grad=True)
+    t = torch.zeros(4, dtype=torch.int64, device=DEV)
+    for y in (ops.layer_norm(x), ops.embedding(t, x)[0], ops.token_logprobs(x[None], t)[0]):
+        (g,) = torch.autograd.grad(y.square().sum(), x, create_graph=True)
+        with pytest.raises(RuntimeError):
+            g.sum().backward()
+
+
+# ------------------------------------------------------------------ LayerNorm
+
+
+def ln_case(rows, D, dtype, seed, offset=1.0, w_dtype=torch.float32):
+    g = gen(seed)
+    x = (torch.randn(rows, D, generator=g) * 1.5 + offset * torch.randn(rows, 1, generator=g)).to(dtype)
+    w = (1 + 0.3 * torch.randn(D, generator=g)).to(w_dtype)
+    b = (0.3 * torch.randn(D, generator=g)).to(w_dtype)
+    gy = torch.randn(rows, D, generator=g).to(dtype)
+    return x, w, b, gy
+
+
+def ln_exact(x, w, b, gy, eps, out_dtype):
+    """The formulas and the error bounds of y, gx, gw, gb in 64 bits."""
+    D = x.shape[-1]
+    k = D / 32 + 16  # a thread's chain over its part of the row, and the joins
+    X, G = x.double(), gy.double()
+    W = torch.ones(D, dtype=torch.float64) if w is None else w.double()
+    Bv = torch.zeros(D, dtype=torch.float64) if b is None else b.double()
+    mean = X.mean(-1, keepdim=True)
+    var = ((X - mean) ** 2).mean(-1, keepdim=True)
+    r = 1 / torch.sqrt(var + eps)
+    h = (X - mean) * r
+    y = h * W + Bv
+    e_mean = (k + 1) * U * X.abs().mean(-1, keepdim=True)
+    e_c = e_mean + U * (X - mean).abs()                  # of x - mean
+    e_var = (2 * (X - mean).abs() * e_c + e_c ** 2).mean(-1, keepdim=True) + (k + 2) * U * var
+    e_r = r * (e_var / (2 * (var + eps)) * 1.01 + 4 * U)
+    e_h = r * e_c + (X - mean).abs() * e_r + 2 * U * h.abs()
+    step = half_step(out_dtype)
+    e_y = (e_h * W.abs() + 2 * U * (h * W).abs() + U * y.abs()) * (1 + step) + step * y.abs() + tiny(out_dtype)
+    a = G * W
+    ma, mh = a.mean(-1, keepdim=True), (a * h).mean(-1, keepdim=True)
+    gx = r * (a - ma - h * mh)
+    e_ma = (k + 2) * U * a.abs().mean(-1, keepdim=True)
+    e_mh = (k + 3) * U * (a * h).abs().mean(-1, keepdim=True) + (a.abs() * e_h).mean(-1, keepdim=True)
+    e_in = 4 * U * (a.abs() + ma.abs() + (h * mh).abs()) + e_ma + h.abs() * e_mh + e_h * mh.abs() + e_h * e_mh
+    step = half_step(x.dtype)
+    e_gx = (r + e_r) * e_in + e_r * (a - ma - h * mh).abs() + 3 * U * gx.abs()
+    e_gx = e_gx * (1 + step) + step * gx.abs() + tiny(x.dtype)
+    kr = x.shape[0] / 8 + 600  # a chain over part of the rows, and the joins of the parts
+    gw, gb = (G * h).sum(0), G.sum(0)
+    e_gw = (G.abs() * e_h).sum(0) + (kr + 2) * U * (G * h).abs().sum(0)
+    e_gb = kr * U * G.abs().sum(0)
+    return (y, gx, gw, gb), (e_y, e_gx, e_gw, e_gb)
+
+
+LN_SHAPES = [(1, 1), (3, 2), (5, 7), (2, 32), (9, 33), (64, 384), (33, 512), (7, 515), (130, 1000), (17, 1024),
+             (6, 1536), (5, 2047), (4, 4096), (3, 5001), (2, 8192), (2, 20000), (1500, 96), (777, 130), (1, 384)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,D", LN_SHAPES)
+@pytest.mark.parametrize("dtype", FLOATS)
+def test_layer_norm_values_and_gradients(ops, rows, D, dtype):
+    x, w, b, gy = ln_case(rows, D, dtype, rows * 7 + D, w_dtype=dtype if D % 2 else torch.float32)
+    want, err = ln_exact(x, w, b, gy, 1e-5, dtype)
+    xd, wd, bd = (t.to(DEV).requires_grad_(True) for t in (x, w, b))
+    y = ops.layer_norm(xd, wd, bd, 1e-5)
+    got = (y, *torch.autograd.grad(y, (xd, wd, bd), gy.to(DEV)))
+    assert [t.dtype for t in got] == [dtype, dtype, w.dtype, w.dtype]
+    for name, t, v, e in zip(("y", "gx", "gw", "gb"), got, want, err):
+        if name in ("gw", "gb"):
+            e = e + half_step(w.dtype) * (v.abs() + e) + tiny(w.dtype)
+        assert_within(t, v, e, name)
+    assert torch.equal(ops.layer_norm(xd.detach(), wd.detach(), bd.detach(), 1e-5), y)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("with_w,with_b", [(False, False), (True, False), (False, True)])
+@pytest.mark.parametrize("dtype,out_dtype", [(torch.bfloat16, torch.float32), (torch.float32, torch.bfloat16),
+                                             (torch.float16, torch.bfloat16)])
+def test_layer_norm_without_parameters_and_other_output_types(ops, with_w, with_b, dtype, out_dtype):
+    x, w, b, gy = ln_case(37, 200, dtype, 3)
+    gy = gy.to(out_dtype)
+    w, b = w if with_w else None, b if with_b else None
+    want, err = ln_exact(x, w, b, gy, 1e-5, out_dtype)
+    leaves = [t.to(DEV).requires_grad_(True) for t in (x, w, b) if t is not None]
+    it = iter(leaves)
+    args = [next(it) if t is not None else None for t in (x, w, b)]
+    y = ops.layer_norm(*args, 1e-5, out_dtype=out_dtype)
+    assert y.dtype == out_dtype
+    grads = iter(torch.autograd.grad(y, leaves, gy.to(DEV)))
+    assert_within(y, want[0], err[0], "y")
+    for i, (t, name) in enumerate(zip((x, w, b), ("gx", "gw", "gb"))):
+        if t is not None:
+            assert_within(next(grads), want[1 + i], err[1 + i], name)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("start,D,pitch", [(0, 515, 643), (8, 384, 1152), (3, 64, 200), (1, 1001, 1003), (5, 32, 40)])
+@pytest.mark.parametrize("dtype", FLOATS)
+def test_layer_norm_reads_column_slices(ops, start, D, pitch, dtype):
+    wide, w, b, _ = ln_case(21, pitch, dtype, start + D)
+    wide, w, b = wide.to(DEV), w.to(DEV)[:D], b.to(DEV)[:D]
+    gy = torch.randn(3, 7, D, generator=gen(1)).to(dtype).to(DEV)
+    xs = wide.view(3, 7, pitch)[..., start:start + D]
+    res = []
+    for x in (xs.detach(), xs.contiguous()):
+        x.requires_grad_(True)
+        y = ops.layer_norm(x, w, b)
+        res.append((y, *torch.autograd.grad(y, x, gy)))
+    # aligned and unaligned rows may split a row's sums differently: two results, each within its bound
+    want, err = ln_exact(xs.reshape(21, D).cpu(), w.cpu(), b.cpu(), gy.reshape(21, D).cpu(), 1e-5, dtype)
+    for y, gx in res:
+        assert y.is_contiguous() and gx.shape == (3, 7, D)
+        assert_within(y.reshape(21, D), want[0], err[0], "y")
+        assert_within(gx.reshape(21, D), want[1], err[1], "gx")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,D", [(1, 8), (2, 384), (147, 96), (148, 384), (149, 515), (1184, 64), (1185, 1000),
+                                    (5000, 384), (3001, 2048), (700, 8192)])
+@pytest.mark.parametrize("dtype", FLOATS)
+def test_layer_norm_parameter_gradients_are_exact_on_integers(ops, rows, D, dtype):
+    """With mean 0, 1/std 1 and small integers g_w = sum g x and g_b = sum g are
+    exact in any order: a lost or doubled row shows.  Sums stay below 2^24."""
+    g = gen(rows + D)
+    x = torch.randint(-8, 9, (rows, D), generator=g).to(dtype)
+    gy = torch.randint(-8, 9, (rows, D), generator=g).to(dtype)
+    stats = torch.tensor([0.0, 1.0]).repeat(rows, 1).to(DEV)
+    w = torch.ones(D, device=DEV)
+    _, gw, gb = ops.layer_norm_bwd(gy.to(DEV), x.to(DEV), stats, w, need_x=False)
+    assert torch.equal(gw.cpu().double(), (gy.double() * x.double()).sum(0))
+    assert torch.equal(gb.cpu().double(), gy.double().sum(0))
+    gx, gw2, gb2 = ops.layer_norm_bwd(gy.to(DEV), x.to(DEV), stats, w)
+    assert torch.equal(gw, gw2) and torch.equal(gb, gb2) and gx.shape == x.shape
+
+
+@pytest.mark.gpu
+def test_layer_norm_large_offset_keeps_its_digits(ops):
+    """x = 1000 + noise: var from squares of x itself would lose 20 of 24 bits."""
+    x, w, b, gy = ln_case(50, 384, torch.float32, 5, offset=0.0)
+    x = x + 1000.0
+    want, err = ln_exact(x, w, b, gy, 1e-5, torch.float32)
+    y = ops.layer_norm(x.to(DEV), w.to(DEV), b.to(DEV))
+    assert_within(y, want[0], err[0], "y")
+    # the bound itself: mean's error k u |x| times 1/std, about 28 * 6e-8 * 1000 / 1.5
+    assert err[0].max() < 0.02
+
+
+@pytest.mark.gpu
+def test_layer_norm_constant_rows_nan_rows_and_empty_input(ops):
+    x = torch.randn(6, 100, generator=gen(1))
+    x[1] = 2.5
+    x[3, 7] = float("nan")
+    x[4, 9] = float("inf")
+    w = torch.ones(100)
+    y = ops.layer_norm(x.to(DEV), w.to(DEV), w.to(DEV)).cpu()
+    assert torch.equal(y[1], torch.ones(100))  # x - mean is 0
+    assert y[3].isnan().all() and y[4].isnan().all()
+    for i in (0, 2, 5):
+        assert torch.isfinite(y[i]).all()
+    xe = torch.empty(0, 3, 100, device=DEV, requires_grad=True)
+    wd = w.to(DEV).requires_grad_(True)
+    ye = ops.layer_norm(xe, wd)
+    gx, gw = torch.autograd.grad(ye, (xe, wd), torch.empty_like(ye))
+    assert ye.shape == (0, 3, 100) and gx.shape == xe.shape and torch.equal(gw.cpu(), torch.zeros(100))
+
+
+@pytest.mark.gpu
+def test_layer_norm_gradient_against_differences(ops):
+    """<gx, v> + <gw, vw> + <gb, vb> against the central difference of the 64-bit
+    forward (step 1e-5: its own error is far below the bound's)."""
+    x, w, b, gy = ln_case(9, 77, torch.float32, 11)
+    vs = [torch.randn(t.shape, generator=gen(12 + i), dtype=torch.float64) for i, t in enumerate((x, w, b))]
+
+    def f(s):
+        X, W, Bv = (t.double() + s * v for t, v in zip((x, w, b), vs))
+        c = X - X.mean(-1, keepdim=True)
+        return ((c / torch.sqrt((c * c).mean(-1, keepdim=True) + 1e-5) * W + Bv) * gy.double()).sum()
+
+    diff = (f(1e-5) - f(-1e-5)) / 2e-5
+    leaves = [t.to(DEV).requires_grad_(True) for t in (x, w, b)]
+    got = torch.autograd.grad(ops.layer_norm(*leaves), leaves, gy.to(DEV))
+    _, err = ln_exact(x, w, b, gy, 1e-5, torch.float32)
+    bound = sum((e * v.abs()).sum() for e, v in zip(err[1:], vs)) + 1e-7
+    assert abs(sum((t.cpu().double() * v).sum() for t, v in zip(got, vs)) - diff) <= bound
+
+
+# ------------------------------------------------------------------ embedding
+
+
+EMB_SHAPES = [(1, 1, 1), (1, 5, 3), (64, 256, 384), (100, 7, 33), (513, 1000, 512), (4096, 256, 384), (2000, 3, 8),
+              (3000, 40000, 24), (33, 2, 1030), (5000, 70000, 5), (257, 300, 2048), (9000, 1, 40)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,V,D", EMB_SHAPES)
+@pytest.mark.parametrize("dtype", FLOATS)
+def test_embedding_forward_is_the_rounded_product(ops, n, V, D, dtype):
+    g = gen(n + V + D)
+    w = torch.randn(V, D, generator=g).to(dtype)
+    tok = torch.randint(0, V, (n,), generator=g)
+    scale = D ** 0.5
+    out, bad = ops.embedding(tok.to(DEV), w.to(DEV), scale)
+    assert int(bad) == 0 and out.dtype == dtype
+    # one fp32 product and one rounding: equality
+    assert torch.equal(out.cpu(), (w[tok].float() * torch.tensor(scale, dtype=torch.float32)).to(dtype))
+    wide, _ = ops.embedding(tok.to(DEV), w.to(DEV), 1.0, out_dtype=torch.float32)
+    assert torch.equal(wide.cpu(), w[tok].float())
+
+
+def scatter_exact(tok, g, V, scale, padding_idx=None):
+    out = torch.zeros(V, g.shape[-1], dtype=torch.float64)
+    keep = (tok >= 0) & (tok < V)
+    if padding_idx is not None:
+        keep &= tok != padding_idx
+    out.index_add_(0, tok[keep], g[keep].double())
+    return out * scale
+
+
+def token_mix(n, V, kind, g):
+    if kind == "uniform":
+        return torch.randint(0, V, (n,), generator=g)
+    if kind == "one":  # every token the same
+        return torch.full((n,), V - 1)
+    if kind == "falling":
+        return (torch.arange(n).flip(0) * V) // max(n, 1)
+    tok = (torch.rand(n, generator=g) ** 4 * V).long().clamp(max=V - 1)  # long-tailed
+    return torch.randperm(V, generator=g)[tok]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,V,D", EMB_SHAPES)
+@pytest.mark.parametrize("kind", ["uniform", "one", "falling", "tail"])
+def test_embedding_gradient_is_exact_on_integers(ops, n, V, D, kind):
+    """Integers below 2^24 in the sums: equality in every type of g, whatever the
+    order; a token's row that is lost, doubled or misplaced shows."""
+    gr = gen(n * 3 + V + D)
+    tok = token_mix(n, V, kind, gr)
+    gi = torch.randint(-100, 101, (n, D), generator=gr)
+    want = scatter_exact(tok, gi, V, 0.5)
+    for dtype in FLOATS:
+        got = ops.embedding_bwd(gi.to(dtype).to(DEV), tok.to(DEV), V, 0.5)
+        assert got.dtype == torch.float32 and torch.equal(got.cpu().double(), want), dtype
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", FLOATS)
+def test_embedding_gradient_values(ops, dtype):
+    """Real values: a row's sum over c tokens errs by at most (c + 2) u of its
+    absolute sum (any order), times the scale's product, and half a step."""
+    n, V, D = 6000, 501, 130
+    gr = gen(4)
+    tok = token_mix(n, V, "tail", gr)
+    gy = torch.randn(n, D, generator=gr).to(dtype)
+    w = torch.randn(V, D, generator=gr).to(dtype).to(DEV).requires_grad_(True)
+    scale = D ** 0.5
+    out, _ = ops.embedding(tok.to(DEV), w, scale)
+    (got,) = torch.autograd.grad(out, w, gy.to(DEV))
+    want = scatter_exact(tok, gy, V, scale)
+    c = torch.bincount(tok, minlength=V).double().unsqueeze(1)
+    e = (c + 4) * U * scatter_exact(tok, gy.abs(), V, scale)
+    assert got.dtype == dtype
+    assert_within(got, want, e * (1 + half_step(dtype)) + half_step(dtype) * want.abs() + tiny(dtype), "gw")
+    again = torch.autograd.grad(ops.embedding(tok.to(DEV), w, scale)[0], w, gy.to(DEV))[0]
+    assert torch.equal(got, again)  # fixed order of the sums
+
+
+@pytest.mark.gpu
+def test_embedding_gradient_against_differences(ops):
+    """The operator is linear in the weight: the difference quotient is exact."""
+    tok = torch.randint(0, 11, (4, 9), generator=gen(1))
+    w = torch.randint(-5, 6, (11, 6), generator=gen(2)).float()
+    gy = torch.randint(-5, 6, (4, 9, 6), generator=gen(3)).float()
+    f = lambda m: ((m[tok] * 2.0) * gy).double().sum()  # noqa: E731
+    wd = w.to(DEV).requires_grad_(True)
+    (got,) = torch.autograd.grad(ops.embedding(tok.to(DEV), wd, 2.0)[0], wd, gy.to(DEV))
+    for v, d in [(0, 0), (10, 5), (3, 2)]:
+        step = torch.zeros_like(w)
+        step[v, d] = 1.0
+        assert float(got[v, d]) == float(f(w + step) - f(w))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,V,D", [(50, 9, 24), (3000, 257, 40)])
+def test_embedding_padding_and_bad_tokens(ops, n, V, D):
+    gr = gen(n)
+    tok = torch.randint(0, V, (n,), generator=gr)
+    tok[::7] = 2
+    gi = torch.randint(-50, 51, (n, D), generator=gr).float()
+    w = torch.randn(V, D, generator=gr).to(DEV).requires_grad_(True)
+    out, bad = ops.embedding(tok.to(DEV), w, 1.0, padding_idx=2)
+    (got,) = torch.autograd.grad(out, w, gi.to(DEV))
+    assert int(bad) == 0 and torch.equal(out.cpu(), w.detach().cpu()[tok])  # the row itself is read as it is
+    assert torch.equal(got.cpu().double(), scatter_exact(tok, gi, V, 1.0, 2)) and not got[2].any()
+    for wrong in (-1, V, -(1 << 40), 1 << 40, (1 << 32) + 1):
+        t = tok.clone()
+        t[n // 2] = wrong
+        out, bad = ops.embedding(t.to(DEV), w, 1.0)
+        (got,) = torch.autograd.grad(out, w, gi.to(DEV))
+        assert int(bad) == 1 and not out[n // 2].any()
+        assert torch.equal(got.cpu().double(), scatter_exact(t, gi, V, 1.0))
+
+
+@pytest.mark.gpu
+def test_embedding_token_types_layouts_and_empty_input(ops):
+    V, D = 50, 24
+    wide = torch.randn(V, 64, generator=gen(1)).to(DEV)
+    w = wide[:, 8:8 + D]
+    tok = torch.randint(0, V, (6, 10), generator=gen(2)).to(DEV)
+    want = w[tok]
+    for t in (tok, tok.int(), tok.to(torch.int16), tok.to(torch.uint8), tok.t().contiguous().t()):
+        assert torch.equal(ops.embedding(t, w)[0], want)
+    assert torch.equal(ops.embedding(tok[:, ::2], w)[0], want[:, ::2])
+    assert torch.equal(ops.embedding(tok[0, 0], w)[0], want[0, 0])
+    # a gradient that is one value expanded, and one with transposed storage
+    wl = w.detach().requires_grad_(True)
+    (g1,) = torch.autograd.grad(ops.embedding(tok, wl)[0].sum(), wl)
+    assert torch.equal(g1, torch.bincount(tok.flatten(), minlength=V).float().unsqueeze(1).expand(V, D))
+    gt = torch.randint(-9, 10, (D, 10, 6), generator=gen(3)).float().to(DEV)
+    (g2,) = torch.autograd.grad(ops.embedding(tok, wl)[0], wl, gt.permute(2, 1, 0))
+    assert torch.equal(g2.cpu().double(), scatter_exact(tok.flatten().cpu(), gt.permute(2, 1, 0).reshape(60, D).cpu(),
+                                                        V, 1.0))
+    empty = torch.empty(0, 3, dtype=torch.int64, device=DEV)
+    out, bad = ops.embedding(empty, wl)
+    (g3,) = torch.autograd.grad(out, wl, torch.empty_like(out))
+    assert out.shape == (0, 3, D) and int(bad) == 0 and not g3.any()
+
+
+# ------------------------------------------------------------------ token log probabilities
+
+
+def lp_exact(logits, tok, K, ignore=-100):
+    """Values and bounds in 64 bits.  Terms of a bound: the T-mean rounded once and
+    the constant log2 e (relative u each, on z), the rounding of t = z log2 e - c
+    (u |t|), 2^t (2^-22 relative), sums in chains of k, and the last few steps."""
+    z = logits.double().mean(0).float().double()  # the operator's mean is rounded once to fp32
+    V = z.shape[-1]
+    k = V / 128 + 64
+    zm = torch.where(torch.isinf(z), 0.0, z).abs().amax(-1)
+    lse = torch.logsumexp(z, -1)
+    lp = z - lse.unsqueeze(-1)
+    p = lp.exp()
+    lpf = torch.where(p > 0, lp, 0.0)
+    H = -(p * lpf).sum(-1)
+    t = lpf.abs() + (z.amax(-1, keepdim=True) - lse.unsqueeze(-1)).abs() + 1  # at least |t_j| ln 2
+    mt, mt2 = (p * t).sum(-1), (p * t * t).sum(-1)
+    e_lse = 4 * U * zm + (k + 10) * U + 2.0 ** -22 + 2 * U * mt
+    e_lp = (e_lse.unsqueeze(-1) + 4 * U * zm.unsqueeze(-1) + 6 * U * t)
+    e_H = 2 * e_lse + ((k + 10) * U + 2.0 ** -22) * (1 + mt) + 2 * U * mt2 + 8 * U * (mt + H.abs() + 1) \
+        + 8 * U * zm * (1 + mt)
+    used = (tok != ignore) & (tok >= 0) & (tok < V)
+    y = tok.clamp(0, V - 1).unsqueeze(-1)
+    out = {"z": z, "p": p, "lp": lp, "lpf": lpf, "H": H, "e_lp": e_lp, "e_H": e_H, "used": used, "y": y,
+           "logp": torch.where(used, lp.gather(-1, y).squeeze(-1), 0.0), "entropy": torch.where(used, H, 0.0),
+           "e_logp": e_lp.gather(-1, y).squeeze(-1)}
+    if K:
+        idx = torch.sort(z, dim=-1, descending=True, stable=True).indices[..., :K]
+        out["top_idx"] = torch.where(used.unsqueeze(-1), idx, -1)
+        out["top_logp"] = torch.where(used.unsqueeze(-1), lp.gather(-1, idx), 0.0)
+        out["e_top"] = e_lp.gather(-1, idx)
+    return out
+
+
+def lp_grad_exact(o, gl, gh, gt, T, dtype):
+    """dlogits of one step and its bound."""
+    used = o["used"].double()
+    gl = torch.zeros_like(used) if gl is None else gl.double() * used
+    gh = torch.zeros_like(used) if gh is None else gh.double() * used
+    G = gl.clone()
+    if gt is not None:
+        G = G + (gt.double() * used.unsqueeze(-1)).sum(-1)
+    u1 = lambda v: v.unsqueeze(-1)  # noqa: E731
+    F = u1(G) + u1(gh) * (o["lpf"] + u1(o["H"]))
+    d = -o["p"] * F
+    hot = torch.zeros_like(d)
+    hot.scatter_add_(-1, o["y"], u1(gl))
+    n_top = 0
+    mag = hot.abs()
+    if gt is not None:
+        n_top = gt.shape[-1]
+        add = gt.double() * u1(used)
+        hot.scatter_add_(-1, o["top_idx"].clamp(min=0), add)
+        mag.scatter_add_(-1, o["top_idx"].clamp(min=0), add.abs())
+    Gm = u1(gl.abs() + (0 if gt is None else (gt.double() * u1(used)).abs().sum(-1)))
+    e_F = u1(gh.abs()) * (o["e_lp"] + u1(o["e_H"])) + (n_top + 6) * U * (Gm + u1(gh.abs()) * (o["lpf"].abs()
+                                                                                         + u1(o["H"]) + 2))
+    e = o["p"] * (e_F + F.abs() * (o["e_lp"] + 2.0 ** -22 + 6 * U)) + 4 * U * (mag + d.abs())
+    d, e = (d + hot) / T, e / T
+    return d, e * (1 + half_step(dtype)) + (half_step(dtype) + U) * d.abs() + tiny(dtype) + 2.0 ** -120
+
+
+LP_SHAPES = [(1, 1, 1), (1, 3, 2), (4, 5, 31), (1, 9, 32), (3, 7, 33), (4, 130, 256), (10, 33, 1000), (1, 17, 1023),
+             (2, 5, 2048), (1, 6, 2049), (1, 4, 4097), (4, 3, 8200), (1, 3, 50001), (1, 1, 131072), (1, 600, 96)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,rows,V", LP_SHAPES)
+@pytest.mark.parametrize("dtype", FLOATS)
+@pytest.mark.parametrize("K", [0, 5, 32])
+def test_token_logprobs_values_and_gradients(ops, T, rows, V, dtype, K):
+    K = min(K, V)
+    g = gen(T + rows + V)
+    x = (torch.randn(T, rows, V, generator=g) * 3).to(dtype)
+    tok = torch.randint(0, V, (rows,), generator=g)
+    if rows > 3:
+        tok[1] = -100
+    o = lp_exact(x, tok, K)
+    xd = x.to(DEV).requires_grad_(True)
+    logp, H, top, idx, bad = ops.token_logprobs(xd, tok.to(DEV), top_k=K)
+    assert int(bad) == 0 and logp.dtype == torch.float32
+    assert_within(logp, o["logp"], o["e_logp"], "logp")
+    assert_within(H, o["entropy"], o["e_H"], "entropy")
+    gs = [torch.randn(rows, generator=g), torch.randn(rows, generator=g)]
+    outs = [logp, H]
+    if K:
+        assert torch.equal(idx.cpu(), o["top_idx"])
+        assert_within(top, o["top_logp"], o["e_top"], "top_logp")
+        gs.append(torch.randn(rows, K, generator=g))
+        outs.append(top)
+    else:
+        assert top is None and idx is None
+    (gx,) = torch.autograd.grad(outs, xd, [t.to(DEV) for t in gs], retain_graph=True)
+    d, e = lp_grad_exact(o, gs[0], gs[1], gs[2] if K else None, T, dtype)
+    for t in range(T):
+        assert_within(gx[t], d, e, "grad")
+    # each output alone
+    (gx,) = torch.autograd.grad(logp, xd, gs[0].to(DEV), retain_graph=True)
+    assert_within(gx[0], *lp_grad_exact(o, gs[0], None, None, T, dtype), "grad of logp")
+    (gx,) = torch.autograd.grad(H, xd, gs[1].to(DEV), retain_graph=True)
+    assert_within(gx[T - 1], *lp_grad_exact(o, None, gs[1], None, T, dtype), "grad of entropy")
+    if K:
+        (gx,) = torch.autograd.grad(top, xd, gs[2].to(DEV))
+        assert_within(gx[0], *lp_grad_exact(o, None, None, gs[2], T, dtype), "grad of top_logp")
+    with torch.no_grad():
+        again = ops.token_logprobs(xd, tok.to(DEV), top_k=K)
+    assert all(a is b or torch.equal(a, b) for a, b in zip(again, (logp, H, top, idx, bad)))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("V", [8, 300, 5000, 40000])
+@pytest.mark.parametrize("order", ["equal", "rising", "falling", "few values", "zeros of both signs"])
+def test_top_alternatives_take_the_lower_index_on_ties(ops, V, order):
+    rows, K = 6, 8
+    if order == "equal":
+        x = torch.full((1, rows, V), 0.25)
+    elif order == "rising":
+        x = (torch.arange(V) / V).expand(1, rows, V).contiguous()
+    elif order == "falling":
+        x = (-torch.arange(V) / V).expand(1, rows, V).contiguous()
+    elif order == "few values":
+        x = torch.randint(0, 3, (1, rows, V), generator=gen(V)).float()
+    else:
+        x = torch.zeros(1, rows, V) * torch.where(torch.arange(V) % 2 == 0, -1.0, 1.0)
+    tok = torch.zeros(rows, dtype=torch.int64)
+    o = lp_exact(x, tok, K)
+    _, H, top, idx, _ = ops.token_logprobs(x.to(DEV), tok.to(DEV), top_k=K)
+    assert torch.equal(idx.cpu(), o["top_idx"])
+    assert_within(top, o["top_logp"], o["e_top"], "top_logp")
+    assert_within(H, o["entropy"], o["e_H"], "entropy")
+
+
+@pytest.mark.gpu
+def test_near_ties_of_the_step_mean_keep_the_exact_order(ops):
+    """fp32 logits of 4 steps whose means differ by a few units in the last place:
+    the order is that of the means rounded once."""
+    g = gen(3)
+    base = torch.randn(4, 50, 1, generator=g)
+    x = base + torch.randint(-3, 4, (4, 50, 256), generator=g) * 2.0 ** -23
+    tok = torch.zeros(50, dtype=torch.int64)
+    _, _, _, idx, _ = ops.token_logprobs(x.to(DEV), tok.to(DEV), top_k=16)
+    assert torch.equal(idx.cpu(), lp_exact(x, tok, 16)["top_idx"])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,V", [(1, 40), (4, 300), (1, 70000)])
+@pytest.mark.parametrize("dtype", FLOATS)
+def test_barred_symbols_and_rows_without_a_distribution(ops, T, V, dtype):
+    rows, K = 8, 6
+    g = gen(V)
+    x = (torch.randn(T, rows, V, generator=g) * 2).to(dtype)
+    x[:, :, torch.rand(V, generator=g) < 0.5] = float("-inf")
+    x[:, :, 3] = 1.0
+    x[:, 2, 4:] = float("-inf")                      # fewer symbols left than alternatives asked for
+    x[:, 2, :3] = torch.tensor([0.5, float("-inf"), 0.25]).to(dtype)
+    x[:, 3, :] = torch.finfo(dtype).min              # the type's lowest value everywhere: uniform
+    x[0, 4, :] = float("-inf")                       # nothing left
+    x[0, 5, V - 1] = float("nan")
+    x[0, 6, 1] = float("inf")
+    tok = torch.full((rows,), 3)
+    tok[7] = -100
+    gl, gh = torch.randn(rows, generator=g), torch.randn(rows, generator=g)
+    o = lp_exact(x, tok, K)
+    xd = x.to(DEV).requires_grad_(True)
+    logp, H, top, idx, bad = ops.token_logprobs(xd, tok.to(DEV), top_k=K)
+    (gx,) = torch.autograd.grad((logp, H), xd, (gl.to(DEV), gh.to(DEV)))
+    d, e = lp_grad_exact(o, gl, gh, None, T, dtype)
+    assert int(bad) == 0
+    for r in (0, 1, 2, 7):
+        assert_within(logp[r], o["logp"][r], o["e_logp"][r], "logp %d" % r)
+        assert_within(H[r], o["entropy"][r], o["e_H"][r], "entropy %d" % r)
+        assert torch.equal(idx[r].cpu(), o["top_idx"][r])
+        fin = torch.isfinite(o["top_logp"][r])
+        assert torch.equal(top[r].cpu()[~fin].double(), o["top_logp"][r][~fin])
+        assert_within(top[r].cpu()[fin], o["top_logp"][r][fin], o["e_top"][r][fin], "top %d" % r)
+        for t in range(T):
+            assert_within(gx[t, r], d[r], e[r], "grad %d" % r)
+    # all equal: logp = -log V, H = log V, whatever the common value
+    lv = torch.tensor(float(V), dtype=torch.float64).log()
+    k = (V / 128 + 80) * U + 2.0 ** -22
+    logp, H = logp.detach(), H.detach()
+    assert abs(float(logp[3]) + lv) <= k + 4 * U * lv and abs(float(H[3]) - lv) <= 2 * k + 8 * U * lv
+    assert torch.equal(idx[3].cpu(), torch.arange(K))
+    for r in (4, 5, 6):
+        assert logp[r].isnan() and H[r].isnan() and top[r].isnan().all() and gx[:, r].isnan().all()
+        assert len(set(idx[r].tolist())) == K and 0 <= int(idx[r].min()) and int(idx[r].max()) < V
+    assert not gx[:, 7].any()
+
+
+@pytest.mark.gpu
+def test_token_logprobs_near_one_keeps_its_digits(ops):
+    """p_y = 1 - 1e-7 or so: logp comes from t_y - log2 S, not from the difference
+    of two numbers near 20."""
+    x = torch.zeros(1, 4, 64)
+    x[:, :, 5] = torch.tensor([16.0, 18.0, 20.0, 24.0])
+    tok = torch.full((4,), 5)
+    logp = ops.token_logprobs(x.to(DEV), tok.to(DEV))[0].cpu().double()
+    want = x.double().log_softmax(-1)[0, :, 5]
+    # S = 1 + s with t_y exact to u |t_y|, |t_y| <= 1/2 ... and log2 S exact to a few u
+    assert ((logp - want).abs() <= 8 * U).all()
+
+
+@pytest.mark.gpu
+def test_token_logprobs_layouts_bad_tokens_and_empty_input(ops):
+    g = gen(9)
+    T, B, N, V = 4, 3, 6, 70
+    x = torch.randn(T, B, N, V, generator=g).to(DEV)
+    tok = torch.randint(0, V, (B, N), generator=g).to(DEV)
+    full = ops.token_logprobs(x, tok, top_k=3)
+    last = ops.token_logprobs(x[:, :, -1], tok[:, -1], top_k=3)          # rows of a decoding step
+    cut = ops.token_logprobs(x[:, 1:, :, :], tok[1:], top_k=3)
+    perm = ops.token_logprobs(x.transpose(1, 2), tok.t(), top_k=3)       # not collapsible: copied
+    narrow = ops.token_logprobs(torch.cat([x, x], -1)[..., 1:1 + V], tok, top_k=3)
+    odd = ops.token_logprobs(x[..., 1:], tok.clamp(max=V - 2), top_k=3)
+    same = ops.token_logprobs(x[..., 1:].contiguous(), tok.clamp(max=V - 2), top_k=3)
+    steps = ops.token_logprobs(x[:1].expand(T, B, N, V), tok, top_k=3)   # one step repeated is its own mean
+    one = ops.token_logprobs(x[:1], tok, top_k=3)
+    scalar = ops.token_logprobs(x[:, 0, 0], tok[0, 0], top_k=3)
+    tol = dict(rtol=0, atol=1e-5)  # 16 u of values below 10, where aligned and unaligned rows split sums differently
+    for i in range(4):
+        for a, b in [(last[i], full[i][:, -1]), (cut[i], full[i][1:]), (perm[i], full[i].transpose(0, 1)),
+                     (odd[i], same[i]), (steps[i], one[i]), (scalar[i], full[i][0, 0])]:
+            assert torch.equal(a, b) if i == 3 else torch.allclose(a, b, **tol)
+    assert torch.isfinite(narrow[0]).all()
+    xl = x.detach().requires_grad_(True)
+    (g1,) = torch.autograd.grad(ops.token_logprobs(xl[:, :, -1], tok[:, -1])[0].sum(), xl)
+    (g2,) = torch.autograd.grad((xl.mean(0).log_softmax(-1)[:, -1]).gather(-1, tok[:, -1:]).sum(), xl)
+    assert torch.allclose(g1, g2, rtol=0, atol=1e-6)
+    for wrong in (-1, V, 1 << 40):
+        t = tok.clone()
+        t[1, 2] = wrong
+        xl = x.detach().requires_grad_(True)
+        logp, H, top, idx, bad = ops.token_logprobs(xl, t, top_k=2)
+        (gx,) = torch.autograd.grad(logp.sum() + H.sum() + top.sum(), xl)
+        assert int(bad) == 1 and float(logp[1, 2]) == 0 and float(H[1, 2]) == 0
+        assert (idx[1, 2] == -1).all() and not gx[:, 1, 2].any() and torch.isfinite(gx).all()
+        assert torch.equal(logp[0], full[0][0])
+    e = ops.token_logprobs(x[:, :0].detach().requires_grad_(True), tok[:0], top_k=2)
+    assert e[0].shape == (0, N) and e[2].shape == (0, N, 2) and int(e[4]) == 0
+
+
+@pytest.mark.gpu
+def test_token_logprobs_gradient_against_differences(ops):
+    g = gen(5)
+    x = torch.randn(3, 7, 50, generator=g)
+    tok = torch.randint(0, 50, (7,), generator=g)
+    gl, gh, gt = (torch.randn(*s, generator=g) for s in ((7,), (7,), (7, 2)))
+    v = torch.randn(3, 7, 50, generator=g, dtype=torch.float64)
+    o = lp_exact(x, tok, 2)
+
+    def f(s):
+        lp = (x.double() + s * v).mean(0).log_softmax(-1)
+        H = -(lp.exp() * lp).sum(-1)
+        return ((lp.gather(-1, tok[:, None])[:, 0] * gl).sum() + (H * gh).sum()
+                + (lp.gather(-1, o["top_idx"]) * gt).sum())
+
+    diff = (f(1e-5) - f(-1e-5)) / 2e-5
+    xd = x.to(DEV).requires_grad_(True)
+    logp, H, top, _, _ = ops.token_logprobs(xd, tok.to(DEV), top_k=2)
+    (gx,) = torch.autograd.grad((logp, H, top), xd, (gl.to(DEV), gh.to(DEV), gt.to(DEV)))
+    d, e = lp_grad_exact(o, gl, gh, gt, 3, torch.float32)
+    # the difference is of unrounded means: u |z| more on each logit
+    bound = ((e + 4 * U * (d.abs() + o["p"])) * v.abs().sum(0)).sum() + 1e-6
+    assert abs((gx.cpu().double() * v).sum() - diff) <= bound
+
+
+# ------------------------------------------------------------------ together, streams, graphs
+
+
+def chain(ops, tok, tgt, w, gamma, beta, out_w):
+    h, _ = ops.embedding(tok, w, w.shape[1] ** 0.5)
+    y = ops.layer_norm(h, gamma, beta)
+    return ops.token_logprobs((y @ out_w.t()).unsqueeze(0), tgt, top_k=3)
+
+
+def chain_inputs(seed, V=300, D=96, B=4, N=33):
+    g = gen(seed)
+    tok = torch.randint(0, V, (B, N), generator=g).to(DEV)
+    tgt = torch.randint(0, V, (B, N), generator=g).to(DEV)
+    ps = [torch.randn(V, D, generator=g) * 0.1, 1 + 0.1 * torch.randn(D, generator=g),
+          0.1 * torch.randn(D, generator=g), torch.randn(V, D, generator=g) * 0.1]
+    return tok, tgt, [p.to(DEV).requires_grad_(True) for p in ps]
+
+
+@pytest.mark.gpu
+def test_the_operators_together_train_as_the_plain_model(ops):
+    """Embedding, LayerNorm, projection and log probabilities in a row, fp32, against
+    the same in 64 bits: errors of about 1e-6 a stage of values of order 1."""
+    tok, tgt, ps = chain_inputs(1)
+    logp, H, top, idx, _ = chain(ops, tok, tgt, *ps)
+    loss = -logp.mean() - 0.01 * H.mean() + 0.1 * top.mean()
+    grads = torch.autograd.grad(loss, ps)
+    qs = [p.detach().double().requires_grad_(True) for p in ps]
+    w, gamma, beta, out_w = qs
+    h = w[tok] * w.shape[1] ** 0.5
+    y = torch.nn.functional.layer_norm(h, (h.shape[-1],), gamma, beta)
+    lp = (y @ out_w.t()).log_softmax(-1)
+    H2 = -(lp.exp() * lp).sum(-1)
+    loss2 = -lp.gather(-1, tgt[..., None]).mean() - 0.01 * H2.mean() + 0.1 * lp.gather(-1, idx).mean()
+    assert abs(float(loss) - float(loss2)) < 1e-5
+    for a, b in zip(grads, torch.autograd.grad(loss2, qs)):
+        # K = 96 and 132-row fp32 products (at most 132 u of the terms' size) dominate
+        assert (a.double() - b).abs().max() <= 2e-5 * b.abs().max()
+
+
+@pytest.mark.gpu
+def test_operators_on_another_stream(ops):
+    tok, tgt, ps = chain_inputs(2)
+    want = chain(ops, tok, tgt, *ps)
+    gw = torch.autograd.grad(want[0].sum(), ps)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = chain(ops, tok, tgt, *ps)
+        gg = torch.autograd.grad(got[0].sum(), ps)
+    torch.cuda.current_stream().wait_stream(side)
+    for a, b in zip(list(want) + list(gw), list(got) + list(gg)):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_operators_in_two_cuda_graphs(ops):
+    """Forward and backward captured twice (each graph with buffers of its own),
+    replayed in turn on new inputs: the eager results."""
+    def static(seed):
+        tok, tgt, ps = chain_inputs(seed)
+        return tok, tgt, ps
+
+    def step(s):
+        out = chain(ops, s[0], s[1], *s[2])
+        return list(out) + list(torch.autograd.grad(out[0].sum() + out[1].sum(), s[2]))
+
+    made = []
+    for seed in (3, 4):
+        s = static(seed)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            step(s)
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs = step(s)
+        made.append((s, graph, outs))
+    for seed in (5, 6):
+        for s, graph, _ in made:
+            new = static(seed)
+            s[0].copy_(new[0])
+            s[1].copy_(new[1])
+            with torch.no_grad():
+                for p, q in zip(s[2], new[2]):
+                    p.copy_(q)
+            graph.replay()
+    torch.cuda.synchronize()
+    for s, graph, outs in made:
+        for a, b in zip(outs, step(s)):
+            assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_no_device_timeouts(ops):
+    ops.device_error_check()
