@@ -24,44 +24,49 @@ namespace embg {
 
 // ---------------------------------------------------------------- forward
 
-// A thread per vector of VEC elements, four in flight.
+// rows that a warp has in flight
+constexpr int kDeep = 8;
+
+// A warp per (kDeep tokens, tile of 32 * VEC columns): the tokens are read
+// together, then their rows, then written.
 template <int WDT, int ODT, int VEC>
 __global__ void __launch_bounds__(256) gather_kernel(const int64_t* __restrict__ tokens,
                                                      const typename Elem<WDT>::T* __restrict__ w, int64_t ldw,
-                                                     float scale, int64_t n, int64_t V, int D,
+                                                     float scale, int64_t n, int64_t V, int D, int tiles,
                                                      typename Elem<ODT>::T* __restrict__ out, int* bad) {
-  const unsigned per_row = (unsigned)(D / VEC);
-  const int64_t total = n * per_row;
-  const int64_t stride = (int64_t)gridDim.x * 256;
-  for (int64_t e0 = blockIdx.x * (int64_t)256 + threadIdx.x; e0 < total; e0 += 4 * stride) {
-    typename Vec<WDT, VEC>::W x[4];
-    int64_t tok[4];
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const int64_t e = e0 + k * stride;
-      tok[k] = -1;
-      if (e < total) {
-        const int64_t i = total < (1ll << 32) ? (int64_t)((unsigned)e / per_row) : e / per_row;
-        const unsigned d = (unsigned)(e - i * per_row);
-        tok[k] = __ldg(tokens + i);
-        if (tok[k] < 0 || tok[k] >= V) {
-          tok[k] = -1;
-          if (d == 0) atomicExch(bad, 1);
-        } else {
-          x[k] = Vec<WDT, VEC>::raw(w + tok[k] * ldw + (int64_t)d * VEC);
-        }
-      }
+  const int lane = threadIdx.x & 31;
+  const int64_t item = blockIdx.x * (int64_t)8 + (threadIdx.x >> 5);
+  const int64_t group = item / tiles;
+  const int col = (int)(item - group * tiles) * 32 * VEC + lane * VEC;
+  const int64_t i0 = group * kDeep;
+  if (i0 >= n) return;
+  int64_t tok = -1;
+  if (lane < kDeep && i0 + lane < n) {
+    tok = __ldg(tokens + i0 + lane);
+    if (tok < 0 || tok >= V) {
+      tok = -1;
+      atomicExch(bad, 1);
     }
+  }
+  typename Vec<WDT, VEC>::W x[kDeep];
+  unsigned in = 0;  // rows that are inside the vocabulary
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const int64_t e = e0 + k * stride;
-      if (e >= total) break;
-      float v[VEC];
-      if (tok[k] >= 0) Vec<WDT, VEC>::unpack(x[k], v);
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) v[j] = tok[k] >= 0 ? v[j] * scale : 0.0f;
-      Vec<ODT, VEC>::store(out + e * VEC, v);
+  for (int k = 0; k < kDeep; ++k) {
+    const int64_t t = __shfl_sync(0xffffffffu, tok, k);
+    if (t >= 0 && col < D) {
+      in |= 1u << k;
+      x[k] = Vec<WDT, VEC>::raw(w + t * ldw + col);
     }
+  }
+  if (col >= D) return;
+#pragma unroll
+  for (int k = 0; k < kDeep; ++k) {
+    if (i0 + k >= n) break;
+    float v[VEC];
+    Vec<WDT, VEC>::unpack(x[k], v);
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) v[j] = (in >> k) & 1u ? v[j] * scale : 0.0f;
+    Vec<ODT, VEC>::store(out + (i0 + k) * D + col, v);
   }
 }
 
@@ -70,6 +75,7 @@ __global__ void __launch_bounds__(256) gather_kernel(const int64_t* __restrict__
 constexpr int kSortThreads = 1024;
 constexpr int kSortWarps = kSortThreads / 32;
 constexpr int kMaxDigit = 10;
+constexpr int kBatch = 8;  // items of a lane that are loaded together
 
 __device__ __forceinline__ uint32_t ld_cluster_u32(uint32_t addr) {
   uint32_t v;
@@ -90,8 +96,8 @@ __device__ __forceinline__ uint32_t cluster_size() {
 // order.  Positions without a gradient get the key V and end up last.
 __global__ void __launch_bounds__(kSortThreads) sort_clear_kernel(const int64_t* tokens, int64_t n, int64_t V,
                                                                   int64_t padding_idx, int bits, int passes,
-                                                                  uint32_t* key0, uint32_t* pos0, uint32_t* key1,
-                                                                  uint32_t* pos1, void* gw, int64_t gw_bytes) {
+                                                                  uint2* item0, uint2* item1, void* gw,
+                                                                  int64_t gw_bytes) {
   extern __shared__ uint32_t sm[];
   const uint32_t ncta = cluster_size(), rank = cluster_ctarank(), cl = cluster_id_x();
   if (cl > 0) {
@@ -117,30 +123,39 @@ __global__ void __launch_bounds__(kSortThreads) sort_clear_kernel(const int64_t*
   const int64_t hi = lo + per_warp < n ? lo + per_warp : n;
   uint32_t* mine = count + warp * bins;
   for (int p = 0; p < passes; ++p) {
-    const uint32_t *kin = (p & 1) ? key0 : key1, *pin = (p & 1) ? pos0 : pos1;
-    uint32_t *kout = (p & 1) ? key1 : key0, *pout = (p & 1) ? pos1 : pos0;
+    const uint2* in_items = (p & 1) ? item0 : item1;
+    uint2* out_items = (p & 1) ? item1 : item0;
     const int shift = p * bits;
-    auto key_at = [&](int64_t i) -> uint32_t {
-      if (p > 0) return __ldcg(kin + i);
+    auto item_at = [&](int64_t i) -> uint2 {  // (key, position)
+      if (p > 0) return __ldcg(in_items + i);
       const int64_t t = __ldg(tokens + i);
-      return t >= 0 && t < V && t != padding_idx ? (uint32_t)t : (uint32_t)V;
+      return make_uint2(t >= 0 && t < V && t != padding_idx ? (uint32_t)t : (uint32_t)V, (uint32_t)i);
     };
     for (int i = lane; i < bins; i += 32) mine[i] = 0;
     __syncwarp();
-    for (int64_t i0 = lo; i0 < hi; i0 += 32) {
-      const int64_t i = i0 + lane;
-      const uint32_t d = i < hi ? (key_at(i) >> shift) & (bins - 1) : 0xffffffffu;
-      const uint32_t same = __match_any_sync(0xffffffffu, d);
-      if (i < hi && (same >> lane) == 1u) mine[d] += __popc(same);  // the highest lane of its digit
-      __syncwarp();
+    for (int64_t i0 = lo; i0 < hi; i0 += 32 * kBatch) {
+      uint32_t k[kBatch];
+#pragma unroll
+      for (int b = 0; b < kBatch; ++b) k[b] = i0 + b * 32 + lane < hi ? item_at(i0 + b * 32 + lane).x : 0u;
+#pragma unroll
+      for (int b = 0; b < kBatch; ++b) {
+        if (i0 + b * 32 >= hi) break;
+        const bool in = i0 + b * 32 + lane < hi;
+        const uint32_t d = in ? (k[b] >> shift) & (bins - 1) : 0xffffffffu;
+        const uint32_t same = __match_any_sync(0xffffffffu, d);
+        if (in && (same >> lane) == 1u) mine[d] += __popc(same);  // the highest lane of its digit
+        __syncwarp();
+      }
     }
     __syncthreads();
     for (int d = threadIdx.x; d < bins; d += kSortThreads) {
-      uint32_t s = 0;
+      uint32_t c[kSortWarps], s = 0;
+#pragma unroll
+      for (int w = 0; w < kSortWarps; ++w) c[w] = count[w * bins + d];
+#pragma unroll
       for (int w = 0; w < kSortWarps; ++w) {
-        const uint32_t c = count[w * bins + d];
         count[w * bins + d] = s;
-        s += c;
+        s += c[w];
       }
       total[d] = s;
     }
@@ -163,25 +178,31 @@ __global__ void __launch_bounds__(kSortThreads) sort_clear_kernel(const int64_t*
     }
     if (lane == 31) wsum[warp] = inc;
     __syncthreads();
-    uint32_t off = 0;
-    for (int w = 0; w < warp; ++w) off += wsum[w];
+    uint32_t off = lane < warp ? wsum[lane] : 0u;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) off += __shfl_xor_sync(0xffffffffu, off, o);
     if (d < bins) base[d] = off + inc - all + before;
     __syncthreads();
-    for (int64_t i0 = lo; i0 < hi; i0 += 32) {
-      const int64_t i = i0 + lane;
-      const bool in = i < hi;
-      const uint32_t k = in ? key_at(i) : 0u;
-      const uint32_t dd = in ? (k >> shift) & (bins - 1) : 0xffffffffu;
-      const uint32_t same = __match_any_sync(0xffffffffu, dd);
-      uint32_t at = 0;
-      if (in) at = base[dd] + mine[dd] + __popc(same & ((1u << lane) - 1u));
-      __syncwarp();
-      if (in) {
-        kout[at] = k;
-        pout[at] = p > 0 ? __ldcg(pin + i) : (uint32_t)i;
-        if ((same >> lane) == 1u) mine[dd] += __popc(same);
+    for (int64_t i0 = lo; i0 < hi; i0 += 32 * kBatch) {
+      uint2 k[kBatch];
+#pragma unroll
+      for (int b = 0; b < kBatch; ++b)
+        k[b] = i0 + b * 32 + lane < hi ? item_at(i0 + b * 32 + lane) : make_uint2(0u, 0u);
+#pragma unroll
+      for (int b = 0; b < kBatch; ++b) {
+        if (i0 + b * 32 >= hi) break;
+        const bool in = i0 + b * 32 + lane < hi;
+        const uint32_t dd = in ? (k[b].x >> shift) & (bins - 1) : 0xffffffffu;
+        const uint32_t same = __match_any_sync(0xffffffffu, dd);
+        uint32_t at = 0;
+        if (in) at = base[dd] + mine[dd] + __popc(same & ((1u << lane) - 1u));
+        __syncwarp();
+        if (in) {
+          out_items[at] = k[b];
+          if ((same >> lane) == 1u) mine[dd] += __popc(same);
+        }
+        __syncwarp();
       }
-      __syncwarp();
     }
     cluster_sync_all();  // the items are written and nobody reads `total` any more
   }
@@ -189,15 +210,26 @@ __global__ void __launch_bounds__(kSortThreads) sort_clear_kernel(const int64_t*
 
 // ---------------------------------------------------------------- backward: sum and join
 
-// rows of g that a warp has in flight
-constexpr int kDeep = 8;
+__device__ __forceinline__ void copy_async(uint32_t dst, const void* src, int bytes_is_16) {
+  if (bytes_is_16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+  else asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
+}
 
-// A warp per (chunk of sorted positions, tile of 32 * VEC columns).
+// A warp per (chunk of sorted positions, tile of 32 * VEC columns).  With
+// VEC > 1 a lane's vectors of the next kRing rows are on their way into a
+// ring of its own in shared memory (a lane reads back only what it copied
+// itself, so the ring needs no barrier); single elements, which asynchronous
+// copies cannot move in two bytes, go through registers.
+constexpr int kRing = 16;
+constexpr int kStep = 4;  // rows of one copy group
+
 template <int GDT, int WDT, int VEC>
-__global__ void __launch_bounds__(256) sum_kernel(const uint32_t* __restrict__ key, const uint32_t* __restrict__ pos,
+__global__ void __launch_bounds__(256) sum_kernel(const uint2* __restrict__ items,
                                                   const typename Elem<GDT>::T* __restrict__ g, float scale, int64_t n,
                                                   uint32_t V, int D, int chunk, int tiles, int64_t chunks,
                                                   typename Elem<WDT>::T* __restrict__ gw, float* __restrict__ part) {
+  using W = typename Vec<GDT, VEC>::W;
+  extern __shared__ uint4 ring_mem[];
   const int lane = threadIdx.x & 31;
   const int64_t item = blockIdx.x * (int64_t)8 + (threadIdx.x >> 5);
   if (item >= chunks * tiles) return;
@@ -205,18 +237,19 @@ __global__ void __launch_bounds__(256) sum_kernel(const uint32_t* __restrict__ k
   const int col = (int)(item - c * tiles) * 32 * VEC + lane * VEC;
   const bool on = col < D;
   const int64_t lo = c * chunk, hi = lo + chunk < n ? lo + chunk : n;
-  const uint32_t before = lo > 0 ? key[lo - 1] : 0xffffffffu;
-  const uint32_t after = hi < n ? key[hi] : 0xffffffffu;
-  uint32_t cur = key[lo];
+  const int m = (int)(hi - lo);
+  const uint32_t before = lo > 0 ? items[lo - 1].x : 0xffffffffu;
+  const uint32_t after = hi < n ? items[hi].x : 0xffffffffu;
+  uint32_t cur = items[lo].x;
   bool first = true;  // the chunk's first token is being added
   float acc[VEC];
 #pragma unroll
   for (int j = 0; j < VEC; ++j) acc[j] = 0.0f;
+  // the sum so far belongs to token `cur`: to the gradient, or to the parts
   auto flush = [&](bool last) {
-    if (cur >= V) return;
+    if (cur >= V || !on) return;
     const bool head = first && cur == before;
     const bool tail = last && cur == after;
-    if (!on) return;
     if (head || tail) {
       // [chunk][0]: the part of a token that comes from the chunk before (and may go on),
       // [chunk][1]: of one that begins here and goes on
@@ -230,120 +263,198 @@ __global__ void __launch_bounds__(256) sum_kernel(const uint32_t* __restrict__ k
       Vec<WDT, VEC>::store(gw + (int64_t)cur * D + col, v);
     }
   };
-  for (int64_t i0 = lo; i0 < hi; i0 += 32) {
-    const int m = hi - i0 < 32 ? (int)(hi - i0) : 32;
-    const uint32_t k = lane < m ? key[i0 + lane] : 0xffffffffu;
-    const uint32_t q = lane < m ? pos[i0 + lane] : 0u;
-    for (int j0 = 0; j0 < m; j0 += kDeep) {
-      typename Vec<GDT, VEC>::W x[kDeep];
+  auto take = [&](uint32_t k, const W& x) {
+    if (k != cur) {
+      flush(false);
+      cur = k;
+      first = false;
 #pragma unroll
-      for (int j = 0; j < kDeep; ++j) {
-        const uint32_t kj = __shfl_sync(0xffffffffu, k, j0 + j), qj = __shfl_sync(0xffffffffu, q, j0 + j);
-        if (on && kj < V) x[j] = Vec<GDT, VEC>::raw(g + (int64_t)qj * D + col);
+      for (int i = 0; i < VEC; ++i) acc[i] = 0.0f;
+    }
+    if (k < V) {
+      float v[VEC];
+      Vec<GDT, VEC>::unpack(x, v);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) acc[i] += v[i];
+    }
+  };
+  // the items of the group of 32 that is added, and of the next one
+  auto group_of = [&](int j) { return j + lane < m ? items[lo + j + lane] : make_uint2(0xffffffffu, 0u); };
+  uint2 a = group_of(0);
+  if constexpr (VEC > 1) {
+    uint2 b = group_of(32);
+    W* ring = reinterpret_cast<W*>(ring_mem) + (threadIdx.x >> 5) * kRing * 32 + lane;
+    const uint32_t ring_at = smem_u32(ring);
+    auto issue = [&](int j) {  // rows [j, j + kStep), at most 32 + the group of `a` away
+#pragma unroll
+      for (int i = 0; i < kStep; ++i) {
+        const int r = (j + i) & 31;
+        const bool in_b = ((j + i) >> 5) != 0;
+        const uint32_t k = __shfl_sync(0xffffffffu, in_b ? b.x : a.x, r);
+        const uint32_t q = __shfl_sync(0xffffffffu, in_b ? b.y : a.y, r);
+        if (on && k < V)
+          copy_async(ring_at + ((j + i) & (kRing - 1)) * 32 * (int)sizeof(W), g + (int64_t)q * D + col,
+                     sizeof(W) == 16);
       }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
 #pragma unroll
-      for (int j = 0; j < kDeep; ++j) {
-        if (j0 + j >= m) break;
-        const uint32_t kj = __shfl_sync(0xffffffffu, k, j0 + j);
-        if (kj != cur) {
-          flush(false);
-          cur = kj;
-          first = false;
+    for (int j = 0; j < kRing; j += kStep) issue(j);
+    for (int j0 = 0; j0 < m; j0 += 32) {
 #pragma unroll
-          for (int i = 0; i < VEC; ++i) acc[i] = 0.0f;
+      for (int j = 0; j < 32; j += kStep) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(kRing / kStep - 1) : "memory");
+#pragma unroll
+        for (int i = 0; i < kStep; ++i) {
+          const uint32_t k = __shfl_sync(0xffffffffu, a.x, j + i);
+          if (j0 + j + i < m) take(k, ring[((j + i) & (kRing - 1)) * 32]);
         }
-        if (on && kj < V) {
-          float v[VEC];
-          Vec<GDT, VEC>::unpack(x[j], v);
+        issue(j + kRing);
+      }
+      a = b;
+      b = group_of(j0 + 64);
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+  } else {
+    for (int j0 = 0; j0 < m; j0 += 32) {
+      for (int j = 0; j < 32 && j0 + j < m; j += kDeep) {
+        W x[kDeep];
 #pragma unroll
-          for (int i = 0; i < VEC; ++i) acc[i] += v[i];
+        for (int i = 0; i < kDeep; ++i) {
+          const uint32_t k = __shfl_sync(0xffffffffu, a.x, j + i), q = __shfl_sync(0xffffffffu, a.y, j + i);
+          if (on && k < V) x[i] = Vec<GDT, VEC>::raw(g + (int64_t)q * D + col);
+        }
+#pragma unroll
+        for (int i = 0; i < kDeep; ++i) {
+          const uint32_t k = __shfl_sync(0xffffffffu, a.x, j + i);
+          if (j0 + j + i < m) take(k, x[i]);
         }
       }
+      a = group_of(j0 + 32);
     }
   }
   flush(true);
 }
 
-// A block per (chunk, 32 columns): where the chunk's last token begins in it and
-// goes on, adds the token's parts.  The parts are cut into one run a warp; the
-// warps' sums are added in order.
-template <int WDT>
-__global__ void __launch_bounds__(256) join_kernel(const uint32_t* __restrict__ key, float scale, int64_t n, uint32_t V,
+// A block per chunk: where the chunk's last token begins in it and goes on, adds
+// the token's parts.  Few parts: a thread adds them, four columns each.  Many:
+// they are cut into one run a warp, and the warps' sums are added in order.
+constexpr int kFewParts = 16;
+
+template <int WDT, int VEC>
+__global__ void __launch_bounds__(256) join_kernel(const uint2* __restrict__ items, float scale, int64_t n, uint32_t V,
                                                    int D, int chunk, int64_t chunks,
                                                    typename Elem<WDT>::T* __restrict__ gw,
                                                    const float* __restrict__ part) {
-  __shared__ float red[8][32];
+  __shared__ float red[8][32 * VEC];
   const int64_t c = blockIdx.x;
   const int64_t lo = c * chunk, hi = lo + chunk;
-  if (hi >= n) return;
-  const uint32_t k = key[hi - 1];
-  if (k >= V || key[hi] != k) return;                  // nothing goes on
-  if (lo > 0 && key[lo] == k && key[lo - 1] == k) return;  // it began before
-  int64_t a = c + 1, b = chunks;                        // chunks (c, a) begin with k
-  while (a < b) {
-    const int64_t mid = (a + b) / 2;
-    if (key[mid * chunk] == k) a = mid + 1;
-    else b = mid;
+  const uint32_t k = items[hi - 1].x;
+  if (k >= V || items[hi].x != k) return;                      // nothing goes on
+  if (lo > 0 && items[lo].x == k && items[lo - 1].x == k) return;  // it began before
+  int64_t a = c + 1, step = 1;  // chunks (c, a) begin with k: doubling steps, then halving ones
+  while (a + step < chunks && items[(a + step) * chunk].x == k) {
+    a += step;
+    step *= 2;
   }
-  const int64_t m = a - c;  // parts: [c][1], [c + 1][0], ..., [a - 1][0]
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int col = blockIdx.y * 32 + lane;
-  float s = 0.0f;
-  if (col < D) {
-    const int64_t p0 = m * warp / 8, p1 = m * (warp + 1) / 8;
-#pragma unroll 8
-    for (int64_t p = p0; p < p1; ++p) s += part[((c + p) * 2 + (p == 0 ? 1 : 0)) * D + col];
-  }
-  red[warp][lane] = s;
-  __syncthreads();
-  if (warp == 0 && col < D) {
-    s = 0.0f;
+  for (; step > 0; step /= 2)
+    if (a + step < chunks && items[(a + step) * chunk].x == k) a += step;
+  const int64_t m = a + 1 - c;  // parts: [c][1], [c + 1][0], ..., [a][0]
+  const float* first = part + (c * 2 + 1) * D;
+  const float* rest = part + c * 2 * D;  // part p > 0 at rest + 2 p D
+  auto add = [&](int64_t p0, int64_t p1, int col, float (&s)[VEC]) {
 #pragma unroll
-    for (int w = 0; w < 8; ++w) s += red[w][lane];
-    gw[(int64_t)k * D + col] = Elem<WDT>::make(s * scale);
+    for (int j = 0; j < VEC; ++j) s[j] = 0.0f;
+#pragma unroll 4
+    for (int64_t p = p0; p < p1; ++p) {
+      float v[VEC];
+      Vec<SPK_F32, VEC>::load((p == 0 ? first : rest + 2 * p * D) + col, v);
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) s[j] += v[j];
+    }
+  };
+  auto put = [&](int col, float (&s)[VEC]) {
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) s[j] *= scale;
+    Vec<WDT, VEC>::store(gw + (int64_t)k * D + col, s);
+  };
+  float s[VEC];
+  if (m <= kFewParts) {
+    for (int col = (blockIdx.y * 256 + threadIdx.x) * VEC; col < D; col += gridDim.y * 256 * VEC) {
+      add(0, m, col, s);
+      put(col, s);
+    }
+    return;
+  }
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (int col0 = blockIdx.y * 32 * VEC; col0 < D; col0 += gridDim.y * 32 * VEC) {
+    const int col = col0 + lane * VEC;
+    if (col < D) {
+      add(m * warp / 8, m * (warp + 1) / 8, col, s);
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) red[warp][lane * VEC + j] = s[j];
+    }
+    __syncthreads();
+    if (warp == 0 && col < D) {
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        s[j] = 0.0f;
+        for (int w = 0; w < 8; ++w) s[j] += red[w][lane * VEC + j];
+      }
+      put(col, s);
+    }
+    __syncthreads();
   }
 }
 
-// positions of a chunk: enough chunks to fill the machine with small batches, few parts with large ones
-inline int chunk_of(int64_t n) { return n <= (1 << 14) ? 16 : n <= (1 << 20) ? 64 : 512; }
 inline int64_t align16(int64_t b) { return (b + 15) / 16 * 16; }
 
+// Chunks: one for every warp that the machine holds (24 an SM) where there are
+// positions enough, of 16 to 1024 positions.
 struct Plan {
-  int bits, passes, chunk;
-  int64_t chunks, items;  // items: bytes of one key or position array
-  Plan(int64_t n, int64_t V) {
+  int bits, passes, chunk, tiles;
+  int64_t chunks, items;  // items: bytes of one array of (key, position)
+  Plan(int64_t n, int64_t V, int64_t D, int vec) {
     int b = 1;
     while ((V >> b) != 0) ++b;  // keys 0 .. V
     passes = (b + kMaxDigit - 1) / kMaxDigit;
     bits = (b + passes - 1) / passes;
-    chunk = chunk_of(n);
+    tiles = (int)((D + 32 * vec - 1) / (32 * vec));
+    const int64_t warps = (int64_t)num_sms() * 24;
+    int64_t ch = ((n * tiles + warps - 1) / warps + 15) / 16 * 16;
+    chunk = (int)(ch < 16 ? 16 : ch > 1024 ? 1024 : ch);
     chunks = (n + chunk - 1) / chunk;
-    items = align16(4 * n);
+    items = align16(8 * n);
   }
 };
 
 template <int GDT, int WDT, int VEC>
-void launch_sum(const Plan& pl, const uint32_t* key, const uint32_t* pos, const void* g, float scale, int64_t n,
-                int64_t V, int D, void* gw, float* part, cudaStream_t st) {
-  const int tiles = (D + 32 * VEC - 1) / (32 * VEC);
-  const int64_t blocks = (pl.chunks * tiles + 7) / 8;
-  sum_kernel<GDT, WDT, VEC><<<(unsigned)blocks, 256, 0, st>>>(
-      key, pos, reinterpret_cast<const typename Elem<GDT>::T*>(g), scale, n, (uint32_t)V, D, pl.chunk, tiles,
-      pl.chunks, reinterpret_cast<typename Elem<WDT>::T*>(gw), part);
+int launch_bwd(const Plan& pl, const uint2* items, const void* g, float scale, int64_t n, int64_t V, int D, void* gw,
+               float* part, cudaStream_t st) {
+  auto* out = reinterpret_cast<typename Elem<WDT>::T*>(gw);
+  const int64_t blocks = (pl.chunks * pl.tiles + 7) / 8;
+  const int smem = VEC > 1 ? 8 * kRing * 32 * (int)sizeof(typename Vec<GDT, VEC>::W) : 0;
+  if (smem > 48 << 10) {
+    const cudaError_t e = cudaFuncSetAttribute(sum_kernel<GDT, WDT, VEC>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                               smem);
+    if (e != cudaSuccess) return fail(SPK_ERR_LAUNCH, "embedding_bwd: %s", cudaGetErrorString(e));
+  }
+  sum_kernel<GDT, WDT, VEC><<<(unsigned)blocks, 256, smem, st>>>(items, reinterpret_cast<const typename Elem<GDT>::T*>(g),
+                                                                scale, n, (uint32_t)V, D, pl.chunk, pl.tiles, pl.chunks,
+                                                                out, part);
+  if (pl.chunks > 1) {
+    // a few blocks a chunk: a token of many parts has its columns spread over them
+    const dim3 grid((unsigned)(pl.chunks - 1), D >= 512 ? 4 : 1);
+    join_kernel<WDT, VEC == 1 ? 1 : 4><<<grid, 256, 0, st>>>(items, scale, n, (uint32_t)V, D, pl.chunk, pl.chunks, out,
+                                                             part);
+  }
+  return check_launch("embedding_bwd");
 }
 
-template <int GDT, int WDT>
-void launch_bwd(const Plan& pl, const uint32_t* key, const uint32_t* pos, const void* g, float scale, int64_t n,
-                int64_t V, int D, void* gw, float* part, cudaStream_t st) {
-  constexpr int kWide = GDT == SPK_F32 || WDT == SPK_F32 ? 4 : 8;  // the wider type's access is 16 bytes
-  const int ge = dtype_size(GDT), we = dtype_size(WDT);
-  if (D % kWide == 0 && aligned(g, kWide * ge) && aligned(gw, kWide * we))
-    launch_sum<GDT, WDT, kWide>(pl, key, pos, g, scale, n, V, D, gw, part, st);
-  else
-    launch_sum<GDT, WDT, 1>(pl, key, pos, g, scale, n, V, D, gw, part, st);
-  if (pl.chunks > 1)
-    join_kernel<WDT><<<dim3((unsigned)(pl.chunks - 1), (unsigned)((D + 31) / 32)), 256, 0, st>>>(
-        key, scale, n, (uint32_t)V, D, pl.chunk, pl.chunks, reinterpret_cast<typename Elem<WDT>::T*>(gw), part);
+// elements of an access: 16 bytes of the wider type where the layout allows
+inline int bwd_vec(const void* g, int g_dtype, const void* gw, int w_dtype, int64_t D) {
+  const int v = g_dtype == SPK_F32 || w_dtype == SPK_F32 ? 4 : 8;
+  return D % v == 0 && aligned(g, v * dtype_size(g_dtype)) && aligned(gw, v * dtype_size(w_dtype)) ? v : 1;
 }
 
 template <int WDT, int ODT>
@@ -352,14 +463,13 @@ void launch_gather(const int64_t* tokens, const void* w, int64_t ldw, float scal
   constexpr int kWide = WDT == SPK_F32 || ODT == SPK_F32 ? 4 : 8;
   const bool wide = D % kWide == 0 && ldw % kWide == 0 && aligned(w, kWide * dtype_size(WDT)) &&
                     aligned(out, kWide * dtype_size(ODT));
-  int64_t grid = (n * (D / (wide ? kWide : 1)) + 1023) / 1024;
-  const int64_t cap = (int64_t)num_sms() * 8;
-  if (grid > cap) grid = cap;
-  if (grid < 1) grid = 1;
+  const int tiles = (D + 32 * (wide ? kWide : 1) - 1) / (32 * (wide ? kWide : 1));
+  const int64_t grid = ((n + kDeep - 1) / kDeep * tiles + 7) / 8;
   auto* wp = reinterpret_cast<const typename Elem<WDT>::T*>(w);
   auto* op = reinterpret_cast<typename Elem<ODT>::T*>(out);
-  if (wide) gather_kernel<WDT, ODT, kWide><<<(unsigned)grid, 256, 0, st>>>(tokens, wp, ldw, scale, n, V, D, op, bad);
-  else gather_kernel<WDT, ODT, 1><<<(unsigned)grid, 256, 0, st>>>(tokens, wp, ldw, scale, n, V, D, op, bad);
+  if (wide)
+    gather_kernel<WDT, ODT, kWide><<<(unsigned)grid, 256, 0, st>>>(tokens, wp, ldw, scale, n, V, D, tiles, op, bad);
+  else gather_kernel<WDT, ODT, 1><<<(unsigned)grid, 256, 0, st>>>(tokens, wp, ldw, scale, n, V, D, tiles, op, bad);
 }
 
 #define SPK_EMB_TYPES(A, B, CALL)                                                  \
@@ -402,8 +512,8 @@ int spk_embedding_fwd(const int64_t* tokens, const void* weight, int w_dtype, in
 int64_t spk_embedding_bwd_workspace_bytes(int64_t n, int64_t V, int64_t D) {
   using namespace spk::embg;
   if (n < 1 || V < 1 || D < 1) return 16;
-  const Plan pl(n, V);
-  return 4 * pl.items + pl.chunks * 2 * D * (int64_t)sizeof(float);
+  const Plan pl(n, V, D, 8);  // the widest tiles make the most chunks
+  return 2 * pl.items + pl.chunks * 2 * D * (int64_t)sizeof(float);
 }
 
 int spk_embedding_bwd(const int64_t* tokens, const void* g, int g_dtype, float scale, int64_t padding_idx, int64_t n,
@@ -421,16 +531,15 @@ int spk_embedding_bwd(const int64_t* tokens, const void* g, int g_dtype, float s
   int rc = check_stream_device(stream);
   if (rc != SPK_OK) return rc;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  const Plan pl(n, V);
+  const int vec = bwd_vec(g, g_dtype, gw, w_dtype, D);
+  const Plan pl(n, V, D, vec);
   char* ws = reinterpret_cast<char*>(workspace);
-  uint32_t* key0 = reinterpret_cast<uint32_t*>(ws);
-  uint32_t* pos0 = reinterpret_cast<uint32_t*>(ws + pl.items);
-  uint32_t* key1 = reinterpret_cast<uint32_t*>(ws + 2 * pl.items);
-  uint32_t* pos1 = reinterpret_cast<uint32_t*>(ws + 3 * pl.items);
-  float* part = reinterpret_cast<float*>(ws + 4 * pl.items);
+  uint2* item0 = reinterpret_cast<uint2*>(ws);
+  uint2* item1 = reinterpret_cast<uint2*>(ws + pl.items);
+  float* part = reinterpret_cast<float*>(ws + 2 * pl.items);
   const int64_t gw_bytes = V * D * dtype_size(w_dtype);
 
-  const int csize = n <= 4096 ? 1 : 8;
+  const int csize = n <= 4096 ? 1 : n <= 32768 ? 8 : 16;
   int64_t fill = (gw_bytes + (int64_t)csize * (64 << 10) - 1) / ((int64_t)csize * (64 << 10));
   const int64_t most = num_sms() / csize;
   if (fill > most) fill = most;
@@ -446,16 +555,18 @@ int spk_embedding_bwd(const int64_t* tokens, const void* g, int g_dtype, float s
   cfg.numAttrs = 1;
   cudaError_t e = cudaFuncSetAttribute(sort_clear_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                        (int)((kSortWarps + 2) << kMaxDigit) * 4);
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(sort_clear_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
   if (e == cudaSuccess)
-    e = cudaLaunchKernelEx(&cfg, sort_clear_kernel, tokens, n, V, padding_idx, pl.bits, pl.passes, key0, pos0, key1,
-                           pos1, gw, gw_bytes);
+    e = cudaLaunchKernelEx(&cfg, sort_clear_kernel, tokens, n, V, padding_idx, pl.bits, pl.passes, item0, item1, gw,
+                           gw_bytes);
   if (e != cudaSuccess) return fail(SPK_ERR_LAUNCH, "embedding_bwd: %s", cudaGetErrorString(e));
-  const uint32_t* key = pl.passes & 1 ? key0 : key1;
-  const uint32_t* pos = pl.passes & 1 ? pos0 : pos1;
-#define CALL(G, W) launch_bwd<G, W>(pl, key, pos, g, scale, n, V, (int)D, gw, part, st)
+  const uint2* items = pl.passes & 1 ? item0 : item1;
+#define CALL(G, W)                                                                                        \
+  constexpr int kWide = G == SPK_F32 || W == SPK_F32 ? 4 : 8;                                             \
+  return vec == kWide ? launch_bwd<G, W, kWide>(pl, items, g, scale, n, V, (int)D, gw, part, st)          \
+                      : launch_bwd<G, W, 1>(pl, items, g, scale, n, V, (int)D, gw, part, st)
   SPK_EMB_TYPES(g_dtype, w_dtype, CALL);
 #undef CALL
-  return check_launch("embedding_bwd");
 }
 
 }  // extern "C"
