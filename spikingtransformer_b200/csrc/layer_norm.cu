@@ -12,11 +12,16 @@
 // Bound by HBM.  A row lives in the registers of 1 to 16 warps (a group), read
 // once and written once; a lane owns the same columns of every row, so w and b
 // (and, in the backward, the column sums of g_w and g_b) stay in registers too.
-// Groups walk over the rows and have the next row's loads on their way while
-// they reduce the present one.  A group of one warp needs shuffles only; a wider
-// one meets at a named barrier.  The fewest warps are taken that hold the row
-// in kNvFwd (kNvBwd) vectors a lane: the backward keeps five values a column
-// instead of three.
+// Groups walk over the rows.  Rows that can be read in vectors of four are copied
+// asynchronously, up to four rows ahead, into a ring in shared memory: a lane
+// reads back only what it copied itself, so the ring needs no barrier.  Other
+// rows go element by element through registers, one row ahead.  A group of one
+// warp needs shuffles only; a wider one meets at a named barrier.  The fewest
+// warps are taken that hold the row in kNvFwd (kNvBwd) vectors a lane: the
+// backward keeps five values a column instead of three.  Columns past the end
+// hold zeros, and the arithmetic runs on pairs (fp32x2) without asking where
+// they are: with a branch for them a row took three times the instructions, and
+// 65536 x 1536 bf16 forward and backward 351 us instead of 193.
 #include "vec.cuh"
 
 namespace spk {
@@ -64,92 +69,259 @@ struct GroupSum {
   }
 };
 
-// where the calling thread stands: its group among all groups, and its column of vector i
+// where the calling thread stands: its group, the rows that the group walks over
+// (first, first + step, ...), and how many they are
 struct Place {
-  int lane, group, in_group;  // group of the block, warp of the group
-  int64_t first, step;        // rows of the group: first, first + step, ...
-  __device__ __forceinline__ Place(int wpr) {
+  int lane, group, in_group, count;
+  int64_t first, step;
+  __device__ __forceinline__ Place(int wpr, int64_t rows) {
     const int warp = threadIdx.x >> 5, groups = (blockDim.x >> 5) / wpr;
     lane = threadIdx.x & 31;
     group = warp / wpr;
     in_group = warp - group * wpr;
     first = (int64_t)blockIdx.x * groups + group;
     step = (int64_t)gridDim.x * groups;
+    count = first < rows ? (int)((rows - first + step - 1) / step) : 0;
   }
 };
 
+// A lane's values of a row as pairs: vector i of four is pairs 2 i and 2 i + 1,
+// single elements 2 i and 2 i + 1 are pair i.
 template <int DT, int VEC, int NV>
-__device__ __forceinline__ void load_row(const typename Elem<DT>::T* row, int col, int stride, int D,
-                                         typename Vec<DT, VEC>::W (&w)[NV]) {
+struct Pairs {
+  static constexpr int P = NV * VEC / 2;
+  using E = typename Elem<DT>::T;
+  using W = typename Vec<DT, VEC>::W;
+  static_assert(VEC == 4 || (VEC == 1 && NV % 2 == 0), "vectors of four, or an even number of elements");
+  __device__ static __forceinline__ float2 unpack2(uint32_t w) {
+    if constexpr (DT == SPK_BF16) return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+    return __half22float2(*reinterpret_cast<const __half2*>(&w));
+  }
+  __device__ static __forceinline__ uint32_t pack2(float2 v) {
+    if constexpr (DT == SPK_BF16) {
+      const __nv_bfloat162 h = __floats2bfloat162_rn(v.x, v.y);
+      return *reinterpret_cast<const uint32_t*>(&h);
+    }
+    const __half2 h = __floats2half2_rn(v.x, v.y);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+  __device__ static __forceinline__ void unpack(const W (&w)[NV], float2 (&v)[P]) {
+    if constexpr (VEC == 1) {
 #pragma unroll
-  for (int i = 0; i < NV; ++i)
-    if (col + i * stride < D) w[i] = Vec<DT, VEC>::raw(row + col + i * stride);
+      for (int i = 0; i < P; ++i) {
+        float lo[1], hi[1];
+        Vec<DT, 1>::unpack(w[2 * i], lo);
+        Vec<DT, 1>::unpack(w[2 * i + 1], hi);
+        v[i] = make_float2(lo[0], hi[0]);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        if constexpr (DT == SPK_F32) {
+          v[2 * i] = make_float2(__uint_as_float(w[i].x), __uint_as_float(w[i].y));
+          v[2 * i + 1] = make_float2(__uint_as_float(w[i].z), __uint_as_float(w[i].w));
+        } else {
+          v[2 * i] = unpack2(w[i].x);
+          v[2 * i + 1] = unpack2(w[i].y);
+        }
+      }
+    }
+  }
+  // the values to a row, from column `col` of D
+  __device__ static __forceinline__ void store(E* row, int col, int D, const float2 (&v)[P]) {
+    if constexpr (VEC == 1) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+        if (col + i * 32 < D) row[i * 32] = Elem<DT>::make(i & 1 ? v[i / 2].y : v[i / 2].x);
+    } else {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        W w;
+        if constexpr (DT == SPK_F32) {
+          w.x = __float_as_uint(v[2 * i].x);
+          w.y = __float_as_uint(v[2 * i].y);
+          w.z = __float_as_uint(v[2 * i + 1].x);
+          w.w = __float_as_uint(v[2 * i + 1].y);
+        } else {
+          w.x = pack2(v[2 * i]);
+          w.y = pack2(v[2 * i + 1]);
+        }
+        if (col + i * 128 < D) *reinterpret_cast<W*>(row + i * 128) = w;
+      }
+    }
+  }
+};
+
+// A lane's vectors of the coming rows, zeros past column D and past the last
+// row.  VEC > 1: `S` rows in a ring in shared memory; VEC = 1: the next row in
+// registers.
+template <int DT, int VEC, int NV, int S>
+struct Rows {
+  using E = typename Elem<DT>::T;
+  using W = typename Vec<DT, VEC>::W;
+  using PR = Pairs<DT, VEC, NV>;
+  static constexpr int kBytes = VEC > 1 ? S * NV * (int)sizeof(W) : 0;  // of shared memory a thread
+  W next[VEC > 1 ? 1 : NV];
+  uint32_t mine, at;  // the lane's part of the ring [S][NV][32], and the slot's offset in it
+  const E* src;       // the lane's first column of the next row to fetch
+  int64_t hop;
+  int left, col, D;   // rows to fetch
+  __device__ __forceinline__ Rows(void* ring, const E* base, int64_t ld, const Place& pl, int c, int cols)
+      : mine(0), at(0), src(base + (pl.count > 0 ? pl.first * ld : 0) + (c < cols ? c : 0)), hop(pl.step * ld), left(pl.count), col(c), D(cols) {
+    if constexpr (VEC > 1)
+      mine = smem_u32(ring) + (threadIdx.x >> 5) * 32 * kBytes + (threadIdx.x & 31) * (int)sizeof(W);
+    else
+#pragma unroll
+      for (int i = 0; i < NV; ++i) next[i] = 0;
+  }
+  __device__ __forceinline__ void fetch() {
+    const bool in = left > 0;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const bool on = in && col + i * 32 * VEC < D;
+      if constexpr (VEC > 1) {
+        // no bytes to copy: zeros are written, the address is not read
+        const uint32_t to = mine + at + i * 32 * (int)sizeof(W);
+        const int bytes = on ? (int)sizeof(W) : 0;
+        if constexpr (sizeof(W) == 16)
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(src + (on ? i * 32 * VEC : 0)),
+                       "r"(bytes)
+                       : "memory");
+        else
+          asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(to), "l"(src + (on ? i * 32 * VEC : 0)),
+                       "r"(bytes)
+                       : "memory");
+      } else if (on) {
+        next[i] = Vec<DT, VEC>::raw(src + i * 32);
+      }
+    }
+    if (--left > 0) src += hop;
+    at = at + NV * 32 * (int)sizeof(W) == (uint32_t)(kBytes * 32) ? 0 : at + NV * 32 * (int)sizeof(W);
+  }
+  // the oldest row
+  __device__ __forceinline__ void take(float2 (&v)[PR::P]) {
+    if constexpr (VEC > 1) {
+      W w[NV];
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const uint32_t from = mine + at + i * 32 * (int)sizeof(W);
+        if constexpr (sizeof(W) == 16)
+          asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                       : "=r"(w[i].x), "=r"(w[i].y), "=r"(w[i].z), "=r"(w[i].w)
+                       : "r"(from)
+                       : "memory");
+        else
+          asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(w[i].x), "=r"(w[i].y) : "r"(from) : "memory");
+      }
+      PR::unpack(w, v);
+    } else {
+      PR::unpack(next, v);
+    }
+  }
+};
+__device__ __forceinline__ void commit_copies() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void wait_copies() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
+// column of the lane's value that is half `hi` of pair p
 template <int VEC>
-__device__ __forceinline__ void store_as(void* y, int ydt, int64_t at, const float (&v)[VEC]) {
-  if (ydt == SPK_F32) Vec<SPK_F32, VEC>::store(reinterpret_cast<float*>(y) + at, v);
-  else if (ydt == SPK_F16) Vec<SPK_F16, VEC>::store(reinterpret_cast<__half*>(y) + at, v);
-  else Vec<SPK_BF16, VEC>::store(reinterpret_cast<__nv_bfloat16*>(y) + at, v);
+__device__ __forceinline__ int pair_col(int col, int p, int hi) {
+  return VEC == 4 ? col + (p >> 1) * 128 + (p & 1) * 2 + hi : col + (2 * p + hi) * 32;
 }
+
+// the lane's columns of a parameter, `other` where there is none, zeros past column D
+template <int VEC, int P>
+__device__ __forceinline__ void load_param(const void* w, int wdt, int col, int D, float other, float2 (&v)[P]) {
+  auto go = [&](auto at) {
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+      const int c0 = pair_col<VEC>(col, p, 0), c1 = pair_col<VEC>(col, p, 1);
+      v[p] = make_float2(c0 < D ? at(c0) : 0.0f, c1 < D ? at(c1) : 0.0f);
+    }
+  };
+  if (!w) go([&](int) { return other; });
+  else if (wdt == SPK_F32) go([&](int c) { return __ldg(reinterpret_cast<const float*>(w) + c); });
+  else if (wdt == SPK_F16) go([&](int c) { return __half2float(reinterpret_cast<const __half*>(w)[c]); });
+  else go([&](int c) { return __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(w)[c]); });
+}
+
+// rows ahead: as many as 48 KB (forward) or 96 KB (backward) of shared memory hold for 256 threads, at most 4
+constexpr int ahead(int bytes_a_row, int most) {
+  return most / bytes_a_row > 4 ? 4 : most / bytes_a_row < 2 ? 2 : most / bytes_a_row;
+}
+
+template <int XDT, int VEC, int NV>
+struct Fwd {
+  static constexpr int S = VEC > 1 ? ahead(NV * VEC * (int)sizeof(typename Elem<XDT>::T), 192) : 1;
+  using X = Rows<XDT, VEC, NV, S>;
+};
+template <int GDT, int XDT, int VEC, int NV>
+struct Bwd {
+  static constexpr int S =
+      VEC > 1 ? ahead(NV * VEC * (int)(sizeof(typename Elem<XDT>::T) + sizeof(typename Elem<GDT>::T)), 384) : 1;
+  using X = Rows<XDT, VEC, NV, S>;
+  using G = Rows<GDT, VEC, NV, S>;
+};
 
 template <int XDT, int VEC, int NV>
 __global__ void __launch_bounds__(32 * kMaxGroup) fwd_kernel(const typename Elem<XDT>::T* __restrict__ x, int64_t ld,
                                                              const void* w, int wdt, const void* b, int bdt, float eps,
                                                              int64_t rows, int D, int wpr, void* __restrict__ y,
                                                              int ydt, float2* __restrict__ stats) {
+  extern __shared__ uint4 ring[];
   __shared__ float2 slots[kWarps][2 * kMaxGroup];
-  const Place pl(wpr);
+  constexpr int S = Fwd<XDT, VEC, NV>::S, P = NV * VEC / 2;
+  const Place pl(wpr, rows);
   GroupSum sum{slots[pl.group], wpr, pl.in_group, pl.lane, pl.group + 1, 0};
-  const int stride = 32 * VEC * wpr, col = (pl.in_group * 32 + pl.lane) * VEC;
-  using W = typename Vec<XDT, VEC>::W;
-  W next[NV];
-  if (pl.first < rows) load_row<XDT, VEC, NV>(x + pl.first * ld, col, stride, D, next);
-  float wv[NV * VEC], bv[NV * VEC];
+  const int col = (pl.in_group * 32 * NV + pl.lane) * VEC;
+  typename Fwd<XDT, VEC, NV>::X in(ring, x, ld, pl, col, D);
 #pragma unroll
-  for (int i = 0; i < NV; ++i)
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) {
-      const int c = col + i * stride + j;
-      wv[i * VEC + j] = w && c < D ? ld_any(w, wdt, c) : 1.0f;
-      bv[i * VEC + j] = b && c < D ? ld_any(b, bdt, c) : 0.0f;
-    }
-  const float inv_d = 1.0f / (float)D;
-  for (int64_t r = pl.first; r < rows; r += pl.step) {
-    W now[NV];
-#pragma unroll
-    for (int i = 0; i < NV; ++i) now[i] = next[i];
-    if (r + pl.step < rows) load_row<XDT, VEC, NV>(x + (r + pl.step) * ld, col, stride, D, next);
-    float v[NV][VEC], s = 0.0f;
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      if (col + i * stride < D) {
-        Vec<XDT, VEC>::unpack(now[i], v[i]);
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) s += v[i][j];
-      }
-    }
-    const float mean = sum(s) * inv_d;
-    float q = 0.0f;
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
-      if (col + i * stride < D)
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          v[i][j] -= mean;
-          q = fmaf(v[i][j], v[i][j], q);
-        }
-    const float rstd = 1.0f / sqrtf(fmaf(sum(q), inv_d, eps));
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
-      if (col + i * stride < D) {
-        float o[VEC];
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) o[j] = fmaf(v[i][j] * rstd, wv[i * VEC + j], bv[i * VEC + j]);
-        store_as<VEC>(y, ydt, r * D + col + i * stride, o);
-      }
-    if (stats && pl.in_group == 0 && pl.lane == 0) stats[r] = make_float2(mean, rstd);
+  for (int k = 0; k < S; ++k) {
+    in.fetch();
+    commit_copies();
   }
+  float2 wv[P], bv[P];
+  load_param<VEC, P>(w, wdt, col, D, 1.0f, wv);
+  load_param<VEC, P>(b, bdt, col, D, 0.0f, bv);
+  const float inv_d = 1.0f / (float)D;
+  int64_t at = pl.first * D + col;  // of y
+  const int64_t hop = pl.step * D;
+  float2* st = stats ? stats + pl.first : nullptr;
+  for (int n = pl.count; n > 0; --n, at += hop) {
+    float2 v[P];
+    wait_copies<S - 1>();
+    in.take(v);
+    float2 s2 = v[0];
+#pragma unroll
+    for (int p = 1; p < P; ++p) s2 = add2(s2, v[p]);
+    const float part = s2.x + s2.y;
+    in.fetch();
+    commit_copies();
+    const float mean = sum(part) * inv_d;
+    const float2 shift = make_float2(-mean, -mean);
+    float2 q2 = make_float2(0.0f, 0.0f);
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+      v[p] = add2(v[p], shift);
+      if (pair_col<VEC>(col, p, 0) >= D) v[p].x = 0.0f;
+      if (pair_col<VEC>(col, p, 1) >= D) v[p].y = 0.0f;
+      q2 = fma2(v[p], v[p], q2);
+    }
+    const float rstd = rsqrtf(fmaf(sum(q2.x + q2.y), inv_d, eps));
+    const float2 r2 = make_float2(rstd, rstd);
+#pragma unroll
+    for (int p = 0; p < P; ++p) v[p] = fma2(mul2(v[p], r2), wv[p], bv[p]);
+    if (ydt == SPK_F32) Pairs<SPK_F32, VEC, NV>::store(reinterpret_cast<float*>(y) + at, col, D, v);
+    else if (ydt == SPK_F16) Pairs<SPK_F16, VEC, NV>::store(reinterpret_cast<__half*>(y) + at, col, D, v);
+    else Pairs<SPK_BF16, VEC, NV>::store(reinterpret_cast<__nv_bfloat16*>(y) + at, col, D, v);
+    if (stats) {
+      if (pl.in_group == 0 && pl.lane == 0) *st = make_float2(mean, rstd);
+      st += pl.step;
+    }
+  }
+  wait_copies<0>();
 }
 
 // part[block][2][D]: (sum g * h, sum g) over the block's rows
@@ -160,90 +332,86 @@ __global__ void __launch_bounds__(32 * kMaxGroup) bwd_kernel(const typename Elem
                                                              int64_t rows, int D, int wpr,
                                                              typename Elem<XDT>::T* __restrict__ gx,
                                                              float* __restrict__ part) {
-  extern __shared__ float cols[];  // [2][D] where a block has several groups
+  extern __shared__ uint4 ring[];  // the rows ahead; at the end [groups][2][D] column sums
   __shared__ float2 slots[kWarps][2 * kMaxGroup];
+  using T = Bwd<GDT, XDT, VEC, NV>;
+  constexpr int S = T::S, P = NV * VEC / 2;
   pdl_trigger();
-  const Place pl(wpr);
+  const Place pl(wpr, rows);
   GroupSum sum{slots[pl.group], wpr, pl.in_group, pl.lane, pl.group + 1, 0};
-  const int stride = 32 * VEC * wpr, col = (pl.in_group * 32 + pl.lane) * VEC;
-  typename Vec<XDT, VEC>::W nx[NV];
-  typename Vec<GDT, VEC>::W ng[NV];
-  float2 ns = make_float2(0.0f, 0.0f);
-  if (pl.first < rows) {
-    load_row<XDT, VEC, NV>(x + pl.first * ld, col, stride, D, nx);
-    load_row<GDT, VEC, NV>(g + pl.first * D, col, stride, D, ng);
-    ns = stats[pl.first];
+  const int col = (pl.in_group * 32 * NV + pl.lane) * VEC;
+  typename T::X xin(ring, x, ld, pl, col, D);
+  typename T::G gin(reinterpret_cast<char*>(ring) + T::X::kBytes * (int)blockDim.x, g, D, pl, col, D);
+#pragma unroll
+  for (int k = 0; k < S; ++k) {
+    xin.fetch();
+    gin.fetch();
+    commit_copies();
   }
-  float wv[NV][VEC], sw[NV][VEC], sb[NV][VEC];
+  // statistics of the present row and the next one
+  const float2* st = stats + pl.first;
+  float2 st0 = pl.count > 0 ? *st : make_float2(0.0f, 0.0f), st1 = st0;
+  if (pl.count > 1) st1 = *(st += pl.step);
+  float2 wv[P], sw[P], sb[P];
+  load_param<VEC, P>(w, wdt, col, D, 1.0f, wv);
 #pragma unroll
-  for (int i = 0; i < NV; ++i)
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) {
-      const int c = col + i * stride + j;
-      wv[i][j] = w && c < D ? ld_any(w, wdt, c) : 1.0f;
-      sw[i][j] = sb[i][j] = 0.0f;
-    }
+  for (int p = 0; p < P; ++p) sw[p] = sb[p] = make_float2(0.0f, 0.0f);
   const float inv_d = 1.0f / (float)D;
-  for (int64_t r = pl.first; r < rows; r += pl.step) {
-    float h[NV][VEC], a[NV][VEC];
-    const float mean = ns.x, rstd = ns.y;
-    float2 s = make_float2(0.0f, 0.0f);
+  int64_t at = pl.first * D + col;  // of gx
+  const int64_t hop = pl.step * D;
+  for (int n = pl.count; n > 0; --n, at += hop) {
+    float2 h[P], a[P];
+    const float2 shift = make_float2(-st0.x, -st0.x), r2 = make_float2(st0.y, st0.y);
+    st0 = st1;
+    if (n > 2) st1 = *(st += pl.step);
+    wait_copies<S - 1>();
+    xin.take(h);
+    gin.take(a);
+    float2 sa = make_float2(0.0f, 0.0f), sh = sa;
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
-      if (col + i * stride < D) {
-        Vec<XDT, VEC>::unpack(nx[i], h[i]);
-        Vec<GDT, VEC>::unpack(ng[i], a[i]);
-      }
-    if (r + pl.step < rows) {
-      load_row<XDT, VEC, NV>(x + (r + pl.step) * ld, col, stride, D, nx);
-      load_row<GDT, VEC, NV>(g + (r + pl.step) * D, col, stride, D, ng);
-      ns = stats[r + pl.step];
+    for (int p = 0; p < P; ++p) {  // past column D a is 0, and h counts nowhere
+      h[p] = mul2(add2(h[p], shift), r2);
+      sw[p] = fma2(a[p], h[p], sw[p]);
+      sb[p] = add2(sb[p], a[p]);
+      a[p] = mul2(a[p], wv[p]);
+      sa = add2(sa, a[p]);
+      sh = fma2(a[p], h[p], sh);
     }
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
-      if (col + i * stride < D)
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          h[i][j] = (h[i][j] - mean) * rstd;
-          sw[i][j] = fmaf(a[i][j], h[i][j], sw[i][j]);
-          sb[i][j] += a[i][j];
-          a[i][j] *= wv[i][j];
-          s.x += a[i][j];
-          s.y = fmaf(a[i][j], h[i][j], s.y);
-        }
+    const float2 both = make_float2(sa.x + sa.y, sh.x + sh.y);
+    xin.fetch();
+    gin.fetch();
+    commit_copies();
     if (gx) {
-      s = sum(s);
+      const float2 s = sum(both);
       const float ma = s.x * inv_d, mh = s.y * inv_d;
+      const float2 ma2 = make_float2(-ma, -ma), mh2 = make_float2(-mh, -mh);
 #pragma unroll
-      for (int i = 0; i < NV; ++i)
-        if (col + i * stride < D) {
-          float o[VEC];
-#pragma unroll
-          for (int j = 0; j < VEC; ++j) o[j] = rstd * (a[i][j] - ma - h[i][j] * mh);
-          Vec<XDT, VEC>::store(gx + r * D + col + i * stride, o);
-        }
+      for (int p = 0; p < P; ++p) a[p] = mul2(r2, fma2(h[p], mh2, add2(a[p], ma2)));
+      Pairs<XDT, VEC, NV>::store(gx + at, col, D, a);
     }
   }
+  wait_copies<0>();
   if (!part) return;
   float* out = part + (int64_t)blockIdx.x * 2 * D;
   const int groups = (blockDim.x >> 5) / wpr;
-  for (int k = 0; k < groups; ++k) {  // the groups in turn, the last one to global memory
-    if (pl.group == k)
+  float* cols = groups > 1 ? reinterpret_cast<float*>(ring) + (int64_t)pl.group * 2 * D : out;
+  __syncthreads();  // nobody reads rows from the ring any more
 #pragma unroll
-      for (int i = 0; i < NV; ++i)
-        if (col + i * stride < D)
+  for (int p = 0; p < P; ++p)
 #pragma unroll
-          for (int j = 0; j < VEC; ++j) {
-            const int c = col + i * stride + j;
-            if (k > 0) {
-              sw[i][j] += cols[c];
-              sb[i][j] += cols[D + c];
-            }
-            float* to = k + 1 < groups ? cols : out;
-            to[c] = sw[i][j];
-            to[D + c] = sb[i][j];
-          }
-    if (k + 1 < groups) __syncthreads();
+    for (int hi = 0; hi < 2; ++hi) {
+      const int c = pair_col<VEC>(col, p, hi);
+      if (c < D) {
+        cols[c] = hi ? sw[p].y : sw[p].x;
+        cols[D + c] = hi ? sb[p].y : sb[p].x;
+      }
+    }
+  if (groups == 1) return;
+  __syncthreads();
+  for (int c = threadIdx.x; c < 2 * D; c += blockDim.x) {
+    float s = 0.0f;
+    for (int k = 0; k < groups; ++k) s += reinterpret_cast<float*>(ring)[k * 2 * D + c];
+    out[c] = s;
   }
 }
 
@@ -350,29 +518,38 @@ __global__ void __launch_bounds__(kLong) long_bwd_w_kernel(const void* g, int gd
 
 // ---------------------------------------------------------------- which kernel, how many blocks
 
-// vectors (single elements) a lane holds at most, forward and backward
-constexpr int kNvFwd = 6, kNvBwd = 4, kNv1Fwd = 24, kNv1Bwd = 16;
+// vectors a lane holds at most, forward and backward; single elements: the second
+// number only where 16 warps of the first do not hold the row (it spills)
+constexpr int kNvFwd = 6, kNvBwd = 4, kNv1Fwd = 12, kNv1Bwd = 10, kNv1FwdLast = 24, kNv1BwdLast = 16;
 
 struct Shape {
   int vec, nv, wpr;  // nv = 0: the row does not fit the registers
-  Shape(int64_t D, bool wide, int most4, int most1) {
+  Shape(int64_t D, bool wide, int most4, int most1, int last1) {
     vec = wide ? 4 : 1;
     const int most = wide ? most4 : most1;
     const int64_t vecs = (D + vec - 1) / vec;
     for (wpr = 1; wpr < kMaxGroup && vecs > 32ll * wpr * most; wpr *= 2) {}
     const int64_t n = (vecs + 32 * wpr - 1) / (32 * wpr);
-    nv = n > most ? 0 : (int)n;
+    nv = n > (wide ? most4 : last1) ? 0 : (int)n;
   }
   int threads() const { return 32 * (wpr > kWarps ? wpr : kWarps); }
   int groups() const { return wpr > kWarps ? 1 : kWarps / wpr; }
 };
 
-inline unsigned blocks_of(int64_t rows, const Shape& s, int per_sm) {
-  const int64_t need = (rows + s.groups() - 1) / s.groups(), cap = (int64_t)num_sms() * per_sm * kWarps * 32 / s.threads();
+constexpr int kBwdPerSm = 3, kLongChunks = 64;
+
+// blocks of a kernel that walks over the rows: what the machine holds at once
+template <typename K>
+unsigned blocks_of(K kernel, int64_t rows, const Shape& s, size_t smem, int most) {
+  int per_sm = 1;
+  if (smem > (40u << 10))  // 48 KB without asking, the kernel's static arrays included
+    cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, s.threads(), smem) != cudaSuccess || per_sm < 1)
+    per_sm = 1;
+  if (per_sm > most) per_sm = most;
+  const int64_t need = (rows + s.groups() - 1) / s.groups(), cap = (int64_t)num_sms() * per_sm;
   return (unsigned)(need < cap ? need : cap);
 }
-
-constexpr int kFwdPerSm = 4, kBwdPerSm = 2, kLongChunks = 64;
 
 // parts of the backward's column sums, whatever its kernel
 inline int64_t max_parts(int64_t rows) {
@@ -383,16 +560,21 @@ inline int64_t max_parts(int64_t rows) {
 template <int XDT, int VEC, int NV>
 void launch_fwd(const void* x, int64_t ld, const void* w, int wdt, const void* b, int bdt, float eps, int64_t rows,
                 int64_t D, const Shape& s, void* y, int ydt, float* stats, cudaStream_t st) {
-  fwd_kernel<XDT, VEC, NV><<<blocks_of(rows, s, kFwdPerSm), s.threads(), 0, st>>>(
-      reinterpret_cast<const typename Elem<XDT>::T*>(x), ld, w, wdt, b, bdt, eps, rows, (int)D, s.wpr, y, ydt,
-      reinterpret_cast<float2*>(stats));
+  const size_t smem = (size_t)Fwd<XDT, VEC, NV>::X::kBytes * s.threads();
+  const unsigned blocks = blocks_of(fwd_kernel<XDT, VEC, NV>, rows, s, smem, 8);
+  fwd_kernel<XDT, VEC, NV><<<blocks, s.threads(), smem, st>>>(reinterpret_cast<const typename Elem<XDT>::T*>(x), ld, w,
+                                                             wdt, b, bdt, eps, rows, (int)D, s.wpr, y, ydt,
+                                                             reinterpret_cast<float2*>(stats));
 }
 
 template <int GDT, int XDT, int VEC, int NV>
 int launch_bwd(const void* g, const void* x, int64_t ld, const float* stats, const void* w, int wdt, int64_t rows,
                int64_t D, const Shape& s, void* gx, float* part, cudaStream_t st) {
-  const unsigned blocks = blocks_of(rows, s, kBwdPerSm);
-  const size_t smem = part && s.groups() > 1 ? (size_t)(2 * D) * sizeof(float) : 0;
+  using T = Bwd<GDT, XDT, VEC, NV>;
+  size_t smem = (size_t)(T::X::kBytes + T::G::kBytes) * s.threads();
+  const size_t sums = part && s.groups() > 1 ? (size_t)s.groups() * 2 * D * sizeof(float) : 0;
+  if (sums > smem) smem = sums;
+  const unsigned blocks = blocks_of(bwd_kernel<GDT, XDT, VEC, NV>, rows, s, smem, kBwdPerSm);
   bwd_kernel<GDT, XDT, VEC, NV><<<blocks, s.threads(), smem, st>>>(
       reinterpret_cast<const typename Elem<GDT>::T*>(g), reinterpret_cast<const typename Elem<XDT>::T*>(x), ld,
       reinterpret_cast<const float2*>(stats), w, wdt, rows, (int)D, s.wpr,
@@ -414,7 +596,7 @@ bool dispatch_fwd(const void* x, int64_t ld, const void* w, int wdt, const void*
       default: return GO(4, 6);
     }
   }
-  return s.nv <= 6 ? GO(1, 6) : s.nv <= 12 ? GO(1, 12) : GO(1, 24);
+  return s.nv <= 4 ? GO(1, 4) : s.nv <= 6 ? GO(1, 6) : s.nv <= 10 ? GO(1, 10) : s.nv <= 12 ? GO(1, 12) : GO(1, 24);
 #undef GO
 }
 
@@ -430,7 +612,7 @@ int dispatch_bwd(const void* g, const void* x, int64_t ld, const float* stats, c
       default: return GO(4, 4);
     }
   }
-  return s.nv <= 4 ? GO(1, 4) : s.nv <= 10 ? GO(1, 10) : GO(1, 16);
+  return s.nv <= 4 ? GO(1, 4) : s.nv <= 6 ? GO(1, 6) : s.nv <= 10 ? GO(1, 10) : GO(1, 16);
 #undef GO
 }
 
@@ -453,7 +635,7 @@ int spk_layer_norm_fwd(const void* x, int x_dtype, int64_t ld, const void* w, in
   if (rc != SPK_OK) return rc;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const bool wide = D % 4 == 0 && ld % 4 == 0 && aligned(x, 4 * dtype_size(x_dtype)) && aligned(y, 4 * dtype_size(y_dtype));
-  const Shape s(D, wide, kNvFwd, kNv1Fwd);
+  const Shape s(D, wide, kNvFwd, kNv1Fwd, kNv1FwdLast);
   auto go = x_dtype == SPK_F32 ? dispatch_fwd<SPK_F32> : x_dtype == SPK_F16 ? dispatch_fwd<SPK_F16> : dispatch_fwd<SPK_BF16>;
   if (!go(x, ld, w, w_dtype, b, b_dtype, eps, rows, D, s, y, y_dtype, stats, st)) {
     const int64_t cap = (int64_t)num_sms() * 4;
@@ -489,7 +671,7 @@ int spk_layer_norm_bwd(const void* g, int g_dtype, const void* x, int x_dtype, i
   float* part = gw || gb ? reinterpret_cast<float*>(workspace) : nullptr;
   const bool wide = D % 4 == 0 && ld % 4 == 0 && aligned(x, 4 * dtype_size(x_dtype)) &&
                     aligned(g, 4 * dtype_size(g_dtype)) && aligned(gx, 4 * dtype_size(x_dtype));
-  const Shape s(D, wide, kNvBwd, kNv1Bwd);
+  const Shape s(D, wide, kNvBwd, kNv1Bwd, kNv1BwdLast);
   int parts;
   if (s.nv > 0) {
 #define GO(G, X) dispatch_bwd<G, X>(g, x, ld, stats, w, w_dtype, rows, D, s, gx, part, st)
