@@ -17,7 +17,18 @@
 // t_j = (z_j - off) log2 e.  t is held at -200 or above, where 2^t is 0 already,
 // so that a barred symbol (z = -inf) adds 0 and not 0 * inf; the maximum passes
 // a NaN on.
-#include "common.cuh"
+//
+// Bound by HBM: the logits are read once in each direction, with no maximum
+// known beforehand.  A thread keeps (m, S, A) of the values that it has seen
+// against the reference of its own m and rescales when a tile raises it; the
+// states of lanes, warps and blocks are joined in the same way.  Rows up to
+// kWarpRow values belong to a warp, longer ones to a block of 8 warps; where the
+// rows are too few to fill the machine a row is cut over several blocks and a
+// second kernel joins them.  Logits come in tiles of 16-byte vectors by
+// asynchronous copies, kStages ahead, into a ring of the thread's own (no
+// barrier); a stage is one step t of one tile.  A row that does not begin on 16
+// bytes has its first and last values taken one by one.
+#include "vec.cuh"
 
 namespace spk {
 namespace lpk {
@@ -31,20 +42,50 @@ __device__ __forceinline__ float exp2_approx(float t) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(t));
   return r;
 }
+
 // What t_j is measured from: t_j = (z_j - off) log2 e - c, one of the two 0.
 struct Ref {
   float off, c;
 };
 constexpr float kFar = 1048576.0f;
 __device__ __forceinline__ Ref ref_of(float m) {
+  if (m == -INFINITY) return Ref{0.0f, 0.0f};  // nothing but barred values so far
   return fabsf(m) <= kFar ? Ref{0.0f, rintf(m * kLog2e)} : Ref{m, 0.0f};
 }
 __device__ __forceinline__ float log2_from(float z, Ref f) { return fmaf(z - f.off, kLog2e, -f.c); }
-__device__ __forceinline__ float rel_log2(float z, Ref f) {
+__device__ __forceinline__ float not_below(float t) {
   float r;
-  asm("max.NaN.f32 %0, %1, 0fC3480000;" : "=f"(r) : "f"(log2_from(z, f)));  // -200
+  asm("max.NaN.f32 %0, %1, 0fC3480000;" : "=f"(r) : "f"(t));  // -200
   return r;
 }
+
+// The values seen so far: their maximum, S and A against ref_of(m).
+struct State {
+  float m, S, A;
+  __device__ __forceinline__ void move_to(float nm) {
+    const Ref a = ref_of(m), b = ref_of(nm);
+    // never above 0; held so where there is nothing yet (m = -inf, S = A = 0)
+    const float d = fminf(fmaxf((a.c - b.c) + (a.off - b.off) * kLog2e, -200.0f), 0.0f);
+    const float k = m == -INFINITY ? 0.0f : exp2_approx(d);
+    A = k * fmaf(d, S, A);
+    S *= k;
+    m = nm;
+  }
+  __device__ __forceinline__ void join(State o) {
+    const float nm = fmaxf(m, o.m);
+    if (nm > m) move_to(nm);
+    if (nm > o.m) o.move_to(nm);
+    S += o.S;
+    A += o.A;
+  }
+  __device__ __forceinline__ void join_warp() {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1)
+      join(State{__shfl_xor_sync(0xffffffffu, m, o), __shfl_xor_sync(0xffffffffu, S, o),
+                 __shfl_xor_sync(0xffffffffu, A, o)});
+  }
+};
+
 // order of the alternatives as an unsigned number: larger logit first, -0 and +0
 // alike, NaN below -inf; 0 is no alternative at all
 __device__ __forceinline__ uint32_t order_bits(float z) {
@@ -57,173 +98,589 @@ __device__ __forceinline__ float order_value(uint32_t k) {
   return __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k);
 }
 
-// The mean over the T steps, rounded once: the sum's rounding errors are
-// collected (two-sum) and go into the quotient's remainder, so that near ties
-// keep the order that the exact means have.
-template <int DT, typename In = typename Elem<DT>::T>
-__device__ __forceinline__ float mean_over_t(const In* x, int64_t st, int T, float inv_t) {
-  float s = Elem<DT>::load(x);
-  if (T == 1) return s;
-  float err = 0.0f;
-  for (int t = 1; t < T; ++t) {
-    const float v = Elem<DT>::load(x + t * st);
-    const float n = __fadd_rn(s, v);
-    const float b = __fsub_rn(n, s);
-    err = __fadd_rn(err, __fadd_rn(__fsub_rn(s, __fsub_rn(n, b)), __fsub_rn(v, b)));
-    s = n;
-  }
-  if (!(fabsf(s) < INFINITY)) {  // an infinity or NaN, or steps whose sum alone is too large
-    double d = 0.0;
-    for (int t = 0; t < T; ++t) d += (double)Elem<DT>::load(x + t * st);
-    return (float)(d / (double)T);
-  }
+
+// ---------------------------------------------------------------- the mean over the steps
+
+// s + v with the rounding error of the sum added to err (two-sum)
+__device__ __forceinline__ void add_exactly(float& s, float& err, float v) {
+  const float n = __fadd_rn(s, v);
+  const float b = __fsub_rn(n, s);
+  err = __fadd_rn(err, __fadd_rn(__fsub_rn(s, __fsub_rn(n, b)), __fsub_rn(v, b)));
+  s = n;
+}
+
+// An infinity or NaN among the steps, or steps whose sum alone is too large.
+template <int DT>
+__device__ __noinline__ float mean_of_extremes(const typename Elem<DT>::T* x, int64_t st, int T) {
+  double d = 0.0;
+  for (int t = 0; t < T; ++t) d += (double)Elem<DT>::load(x + t * st);
+  return (float)(d / (double)T);
+}
+
+// (s + err) / T rounded once: the quotient's remainder takes the errors in, so
+// that near ties keep the order that the exact means have.  x: the value's first step.
+template <int DT>
+__device__ __forceinline__ float mean_of(float s, float err, const typename Elem<DT>::T* x, int64_t st, int T,
+                                         float inv_t) {
+  if (!(fabsf(s) < INFINITY)) return mean_of_extremes<DT>(x, st, T);
   const float q = __fmul_rn(s, inv_t);
   return fmaf(__fadd_rn(fmaf(-q, (float)T, s), err), inv_t, q);
 }
 
-constexpr int kThreads = 128;
-
-template <typename Op>
-__device__ __forceinline__ float block_all(float v, Op op) {
-  __shared__ float red[kThreads / 32];
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v = op(v, __shfl_xor_sync(0xffffffffu, v, o));
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-  __syncthreads();
-  v = red[0];
-#pragma unroll
-  for (int i = 1; i < kThreads / 32; ++i) v = op(v, red[i]);
-  return v;
+// z_j of one value
+template <int DT>
+__device__ __forceinline__ float mean_over_t(const typename Elem<DT>::T* x, int64_t st, int T, float inv_t) {
+  float s = Elem<DT>::load(x);
+  if (T == 1) return s;
+  float err = 0.0f;
+  for (int t = 1; t < T; ++t) add_exactly(s, err, Elem<DT>::load(x + t * st));
+  return mean_of<DT>(s, err, x, st, T, inv_t);
 }
 
-// largest key of the block below `limit`
-__device__ __forceinline__ unsigned long long block_max64(unsigned long long v) {
-  __shared__ unsigned long long red[kThreads / 32];
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const unsigned long long u = __shfl_xor_sync(0xffffffffu, v, o);
-    v = u > v ? u : v;
-  }
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-  __syncthreads();
-  v = red[0];
-#pragma unroll
-  for (int i = 1; i < kThreads / 32; ++i) v = red[i] > v ? red[i] : v;
-  return v;
-}
+// ---------------------------------------------------------------- tiles of a row
 
-template <int DT, typename In = typename Elem<DT>::T>
-__global__ void __launch_bounds__(kThreads) fwd_kernel(const In* __restrict__ logits, int T, int64_t rows, int V,
-                                                       int64_t st, int64_t sr, const int64_t* __restrict__ tokens,
-                                                       int64_t ignore, int K, float* logp, float* entropy,
-                                                       float* top_logp, int64_t* top_idx, float* stats, int* bad) {
-  const float inv_t = 1.0f / (float)T;
-  for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
-    const int64_t y = tokens[r];
-    const bool in = y >= 0 && y < V;
-    if (y == ignore || !in) {
-      if (threadIdx.x == 0) {
-        if (y != ignore) atomicExch(bad, 1);
-        logp[r] = entropy[r] = 0.0f;
-        reinterpret_cast<float4*>(stats)[r] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      }
-      for (int k = threadIdx.x; k < K; k += kThreads) {
-        top_logp[r * K + k] = 0.0f;
-        top_idx[r * K + k] = -1;
-      }
-      continue;
-    }
-    const In* x = logits + r * sr;
-    float m = -INFINITY;
-    for (int j = threadIdx.x; j < V; j += kThreads) m = fmaxf(m, mean_over_t<DT>(x + j, st, T, inv_t));
-    m = block_all(m, [](float a, float b) { return fmaxf(a, b); });
-    const Ref f = ref_of(m);
-    float S = 0.0f, A = 0.0f;
-    for (int j = threadIdx.x; j < V; j += kThreads) {
-      const float t = rel_log2(mean_over_t<DT>(x + j, st, T, inv_t), f);
-      const float e = exp2_approx(t);
-      S += e;
-      A = fmaf(e, t, A);
-    }
-    auto add = [](float a, float b) { return a + b; };
-    S = block_all(S, add);
-    A = block_all(A, add);
-    const float l2s = log2f(S);
-    const float H = kLn2 * (l2s - A / S);
-    if (threadIdx.x == 0) {
-      logp[r] = kLn2 * (log2_from(mean_over_t<DT>(x + y, st, T, inv_t), f) - l2s);
-      entropy[r] = H;
-      reinterpret_cast<float4*>(stats)[r] = make_float4(f.off, f.c, S, H);
-    }
-    unsigned long long limit = ~0ull;
-    for (int k = 0; k < K; ++k) {
-      unsigned long long best = 0;
-      for (int j = threadIdx.x; j < V; j += kThreads) {
-        const unsigned long long key =
-            ((unsigned long long)order_bits(mean_over_t<DT>(x + j, st, T, inv_t)) << 32) | (uint32_t)~j;
-        if (key < limit && key > best) best = key;
-      }
-      limit = block_max64(best);
-      if (threadIdx.x == 0) {
-        top_idx[r * K + k] = (int64_t)(~(uint32_t)limit);
-        top_logp[r * K + k] = kLn2 * (log2_from(order_value((uint32_t)(limit >> 32)), f) - l2s);
-      }
+constexpr int kStages = 4;
+
+struct Logits {  // element (t, r, v) at base + t st + r sr + v
+  const void* base;
+  int T, V;
+  int64_t rows, st, sr;
+  float inv_t;
+};
+
+// Values [lo, hi) of a row in tiles of GT threads x U vectors of VEC; thread
+// tid's vector u of a tile begins at lo + ((tile U + u) GT + tid) VEC.
+template <int DT, int VEC, int U, int GT>
+struct Tiles {
+  using E = typename Elem<DT>::T;
+  using W = typename Vec<DT, VEC>::W;
+  static constexpr int N = U * VEC, kSpan = GT * U * VEC;
+  static constexpr int kBytes = VEC > 1 ? kStages * U * 16 : 0;  // of shared memory a thread
+  static_assert(VEC == 1 || sizeof(W) == 16, "16-byte vectors");
+  const E* row;
+  int64_t st;
+  int T, lo, hi, tid;
+  int ft, fj;         // the stage to fetch: step, and the thread's first value in the tile
+  const E* fp;
+  uint32_t ring, at;  // the thread's ring [kStages][U][256], the slot's offset
+  __device__ __forceinline__ Tiles(void* smem, const E* r, int64_t step, int steps, int l, int h, int thread)
+      : row(r), st(step), T(steps), lo(l), hi(h), tid(thread), ft(0), fj(l + thread * VEC), fp(r), ring(0), at(0) {
+    if constexpr (VEC > 1) {
+      ring = smem_u32(smem) + threadIdx.x * 16;
+#pragma unroll
+      for (int k = 0; k < kStages; ++k) fetch();
     }
   }
+  __device__ __forceinline__ int first(int tile) const { return lo + tile * kSpan + tid * VEC; }
+  __device__ __forceinline__ void fetch() {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int j = fj + u * GT * VEC;
+      if (j < hi)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(ring + at + u * 256 * 16), "l"(fp + j) : "memory");
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    at = at + U * 256 * 16 == kStages * U * 256 * 16 ? 0 : at + U * 256 * 16;
+    if (++ft == T) {
+      ft = 0;
+      fj += kSpan;
+      fp = row;
+    } else {
+      fp += st;
+    }
+  }
+  // one step of the tile whose first value of this thread is j0; absent values stay as they are
+  __device__ __forceinline__ void take(int j0, int t, float (&v)[N]) {
+    if constexpr (VEC > 1) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (j0 + u * GT * VEC < hi) {
+          W w;
+          asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                       : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w)
+                       : "r"(ring + at + u * 256 * 16)
+                       : "memory");
+          float x[VEC];
+          Vec<DT, VEC>::unpack(w, x);
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) v[u * VEC + i] = x[i];
+        }
+    } else {
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (j0 + u * GT < hi) v[u] = Elem<DT>::load(row + t * st + j0 + u * GT);
+    }
+  }
+  // z of a tile, -inf where there is no value; the next stages are on their way
+  __device__ __forceinline__ void mean(int tile, float inv_t, float (&z)[N]) {
+    const int j0 = first(tile);
+#pragma unroll
+    for (int i = 0; i < N; ++i) z[i] = -INFINITY;
+    take(j0, 0, z);
+    if constexpr (VEC > 1) fetch();
+    if (T == 1) return;
+    float err[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) err[i] = 0.0f;
+    for (int t = 1; t < T; ++t) {
+      float v[N];
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] = 0.0f;
+      take(j0, t, v);
+      if constexpr (VEC > 1) fetch();
+#pragma unroll
+      for (int i = 0; i < N; ++i) add_exactly(z[i], err[i], v[i]);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (j0 + u * GT * VEC < hi)
+#pragma unroll
+        for (int i = 0; i < VEC; ++i)
+          z[u * VEC + i] = mean_of<DT>(z[u * VEC + i], err[u * VEC + i], row + j0 + u * GT * VEC + i, st, T, inv_t);
+  }
+  __device__ __forceinline__ int tiles() const { return hi > lo ? (hi - lo + kSpan - 1) / kSpan : 0; }
+};
+
+// values before the first 16-byte boundary of a row, with 16-byte vectors
+template <int DT, int VEC>
+__device__ __forceinline__ int head_of(const typename Elem<DT>::T* row, int V) {
+  if constexpr (VEC == 1) return 0;
+  const int h = (int)((16 - (reinterpret_cast<uintptr_t>(row) & 15)) & 15) / (int)sizeof(typename Elem<DT>::T);
+  return h < V ? h : V;
 }
 
-template <int DT, typename In = typename Elem<DT>::T>
-__global__ void __launch_bounds__(kThreads) bwd_kernel(const In* __restrict__ logits, int T, int64_t rows, int V,
-                                                       int64_t st, int64_t sr, const int64_t* __restrict__ tokens,
-                                                       int64_t ignore, int K, const int64_t* __restrict__ top_idx,
-                                                       const float* __restrict__ stats, const float* g_logp,
-                                                       const float* g_entropy, const float* g_top, In* grad) {
-  const float inv_t = 1.0f / (float)T;
-  for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
-    const int64_t y = tokens[r];
-    const bool used = y != ignore && y >= 0 && y < V;
-    const In* x = logits + r * sr;
-    const float4 sv = reinterpret_cast<const float4*>(stats)[r];
-    const Ref f = {sv.x, sv.y};
-    const float S = sv.z, H = sv.w;
-    const float gl = g_logp ? g_logp[r] : 0.0f, gh = g_entropy ? g_entropy[r] : 0.0f;
-    float G = gl;
-    for (int k = 0; g_top && k < K; ++k) G += g_top[r * K + k];
-    const float inv_s = 1.0f / S;
-    const float a = -gh * kLn2 * inv_s, b = (-G - gh * (H - kLn2 * log2f(S))) * inv_s;
-    for (int j = threadIdx.x; j < V; j += kThreads) {
-      float d = 0.0f;
-      if (used) {
-        const float t = rel_log2(mean_over_t<DT>(x + j, st, T, inv_t), f);
-        d = exp2_approx(t) * fmaf(a, t, b);
-        if (j == y) d += gl;
-        for (int k = 0; g_top && k < K; ++k)
-          if (top_idx[r * K + k] == j) d += g_top[r * K + k];
-        d *= inv_t;
-      }
-      for (int t = 0; t < T; ++t) grad[((int64_t)t * rows + r) * V + j] = Elem<DT>::make(d);
+// values [lo, hi) of split `s` of `splits`, of the vectors between head and tail
+template <int VEC>
+__device__ __forceinline__ void range_of(int V, int head, int split, int splits, int& lo, int& hi) {
+  const int vecs = (V - head) / VEC;
+  const int each = ((vecs + splits - 1) / splits + 31) / 32 * 32;
+  const int a = split * each < vecs ? split * each : vecs, b = a + each < vecs ? a + each : vecs;
+  lo = head + a * VEC;
+  hi = head + b * VEC;
+}
+
+// ---------------------------------------------------------------- alternatives
+
+// The K best (order bits, ~index) of a warp, falling; lane k holds the k-th, 0 none.
+struct Best {
+  unsigned long long key;
+  int K, lane, full;
+  float floor;  // the K-th value where there are K
+  __device__ __forceinline__ Best(int k, int l) : key(0), K(k), lane(l), full(0), floor(-INFINITY) {}
+  __device__ __forceinline__ unsigned long long last() const { return __shfl_sync(0xffffffffu, key, K - 1); }
+  __device__ __forceinline__ void insert(unsigned long long k) {  // uniform, above last()
+    const int at = __popc(__ballot_sync(0xffffffffu, key > k));
+    const unsigned long long up = __shfl_up_sync(0xffffffffu, key, 1);
+    if (lane > at) key = up;
+    if (lane == at) key = k;
+    if (lane >= K) key = 0;
+  }
+  __device__ __forceinline__ void settle() {
+    const unsigned long long k = last();
+    full = k != 0;
+    floor = full ? order_value((uint32_t)(k >> 32)) : -INFINITY;
+  }
+  // the list of another warp, falling, lane k the k-th
+  __device__ __forceinline__ void merge(unsigned long long other) {
+    for (int i = 0; i < K; ++i) {
+      const unsigned long long k = __shfl_sync(0xffffffffu, other, i);
+      if (k <= last()) break;
+      insert(k);
     }
+  }
+  // N values a lane, value i with index j[i] (< 0: none); `most`: their largest.  The best of
+  // the warp goes into the list, again and again, until none is good enough.
+  template <int N, typename J>
+  __device__ __forceinline__ void offer(const float (&z)[N], float most, bool ties, J index) {
+    if (!__any_sync(0xffffffffu, !full || most > floor || (ties && most >= floor))) return;
+    uint32_t ord[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) ord[i] = index(i) >= 0 ? order_bits(z[i]) : 0u;
+    for (int n = 0; n < K; ++n) {
+      uint32_t best = 0, j = 0xffffffffu;
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (ord[i] > best) {  // rising indexes: the first of equals
+          best = ord[i];
+          j = (uint32_t)index(i);
+        }
+      const uint32_t top = __reduce_max_sync(0xffffffffu, best);
+      if (top == 0) break;
+      const uint32_t at = __reduce_min_sync(0xffffffffu, best == top ? j : 0xffffffffu);
+      const unsigned long long k = ((unsigned long long)top << 32) | (uint32_t)~at;
+      if (k <= last()) break;
+      insert(k);
+      if (best == top && j == at)
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+          if ((uint32_t)index(i) == at) ord[i] = 0;
+    }
+    settle();
+  }
+};
+
+// a tile into the thread's state
+template <int N>
+__device__ __forceinline__ void absorb(State& s, float (&z)[N], float most) {
+  if (most > s.m) s.move_to(most);
+  const Ref f = ref_of(s.m);
+  if (f.off != 0.0f)
+#pragma unroll
+    for (int i = 0; i < N; ++i) z[i] -= f.off;
+  float2 S2 = make_float2(0.0f, 0.0f), A2 = S2;
+  const float2 l2 = make_float2(kLog2e, kLog2e), c2 = make_float2(-f.c, -f.c);
+#pragma unroll
+  for (int i = 0; i < N; i += 2) {
+    float2 t = fma2(make_float2(z[i], z[i + 1]), l2, c2);
+    t = make_float2(not_below(t.x), not_below(t.y));
+    const float2 e = make_float2(exp2_approx(t.x), exp2_approx(t.y));
+    S2 = add2(S2, e);
+    A2 = fma2(e, t, A2);
+  }
+  s.S += S2.x + S2.y;
+  s.A += A2.x + A2.y;
+}
+
+struct Out {
+  float *logp, *entropy, *top_logp;
+  int64_t* top_idx;
+  float4* stats;
+};
+
+// the row's results from its state and list (one warp)
+template <int DT>
+__device__ __forceinline__ void write_row(const Logits& x, const typename Elem<DT>::T* row, int64_t r, int64_t y,
+                                          State s, unsigned long long key, int K, int lane, const Out& o) {
+  const Ref f = ref_of(s.m);
+  const float l2s = log2f(s.S), H = kLn2 * (l2s - s.A / s.S);
+  if (lane == 0) {
+    o.logp[r] = kLn2 * (log2_from(mean_over_t<DT>(row + y, x.st, x.T, x.inv_t), f) - l2s);
+    o.entropy[r] = H;
+    o.stats[r] = make_float4(f.off, f.c, s.S, H);
+  }
+  if (lane < K) {
+    o.top_idx[r * K + lane] = (int64_t)(~(uint32_t)key);
+    // a row without a distribution has none for the alternatives either
+    o.top_logp[r * K + lane] = kLn2 * (log2_from(order_value((uint32_t)(key >> 32)), f) - l2s);
   }
 }
 
-inline bool float_type(int dt) { return dt == SPK_F32 || dt == SPK_F16 || dt == SPK_BF16; }
+__device__ __forceinline__ void write_unused(int64_t r, int K, int lane, const Out& o) {
+  if (lane == 0) {
+    o.logp[r] = o.entropy[r] = 0.0f;
+    o.stats[r] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  }
+  if (lane < K) {
+    o.top_logp[r * K + lane] = 0.0f;
+    o.top_idx[r * K + lane] = -1;
+  }
+}
+
+constexpr int kWarpRow = 1024;  // values of a row that one warp takes (fewer rows than warps aside)
+
+// GT = 32: a warp a row.  GT = 256: a block a (row, split); with several splits
+// the state and list go to part / keys.
+template <int DT, int VEC, int U, int GT>
+__global__ void __launch_bounds__(256) fwd_kernel(Logits x, const int64_t* __restrict__ tokens, int64_t ignore, int K,
+                                                  int splits, Out o, float4* part, unsigned long long* keys, int* bad,
+                                                  int scan_bad) {
+  using E = typename Elem<DT>::T;
+  extern __shared__ uint4 ring[];
+  if (scan_bad && blockIdx.x == gridDim.x - 1) {
+    scan_tokens(tokens, x.rows, x.V, ignore, bad);
+    return;
+  }
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t unit = GT == 32 ? (int64_t)blockIdx.x * 8 + warp : (int64_t)blockIdx.x;
+  const int64_t r = GT == 32 ? unit : unit / splits;
+  const int split = GT == 32 ? 0 : (int)(unit - r * splits);
+  if (r >= x.rows) return;
+  const int64_t y = __ldg(tokens + r);
+  if (y == ignore || y < 0 || y >= x.V) {
+    if (split == 0 && (GT == 32 || warp == 0)) {
+      write_unused(r, K, lane, o);
+      if (!scan_bad && y != ignore && lane == 0) atomicExch(bad, 1);
+    }
+    return;
+  }
+  const E* row = reinterpret_cast<const E*>(x.base) + r * x.sr;
+  const int head = head_of<DT, VEC>(row, x.V), tail = (x.V - head) % VEC;
+  int lo, hi;
+  range_of<VEC>(x.V, head, split, splits, lo, hi);
+  const int tid = GT == 32 ? lane : (int)threadIdx.x;
+  Tiles<DT, VEC, U, GT> tl(ring, row, x.st, x.T, lo, hi, tid);
+  State s{-INFINITY, 0.0f, 0.0f};
+  Best best(K > 0 ? K : 1, lane);
+  const int tiles = tl.tiles();
+  constexpr int N = Tiles<DT, VEC, U, GT>::N;
+  for (int k = 0; k < tiles; ++k) {
+    float z[N];
+    tl.mean(k, x.inv_t, z);
+    float most = z[0];
+#pragma unroll
+    for (int i = 1; i < N; ++i) most = fmaxf(most, z[i]);
+    const int j0 = tl.first(k);
+    if (K > 0)
+      best.offer(z, most, false, [&](int i) {
+        const int j = j0 + (i / VEC) * GT * VEC;
+        return j < hi ? j + i % VEC : -1;
+      });
+    absorb(s, z, most);
+  }
+  if constexpr (VEC > 1) asm volatile("cp.async.wait_all;" ::: "memory");
+  if (VEC > 1 && split == 0 && head + tail > 0) {  // the values beside the vectors
+    const int j = tid < head ? tid : tid >= GT - tail ? x.V - (GT - tid) : -1;
+    float z[2] = {j >= 0 ? mean_over_t<DT>(row + j, x.st, x.T, x.inv_t) : -INFINITY, -INFINITY};
+    if (K > 0) best.offer(z, z[0], true, [&](int i) { return i == 0 ? j : -1; });
+    absorb(s, z, z[0]);
+  }
+  s.join_warp();
+  if constexpr (GT > 32) {
+    __shared__ State ws[8];
+    __shared__ unsigned long long wk[8][kMaxTop];
+    if (lane == 0) ws[warp] = s;
+    wk[warp][lane] = best.key;
+    __syncthreads();
+    if (warp > 0) return;
+    s = State{-INFINITY, 0.0f, 0.0f};
+    for (int w = 0; w < 8; ++w) s.join(ws[w]);
+    if (K > 0)
+      for (int w = 1; w < 8; ++w) best.merge(wk[w][lane]);
+    if (splits > 1) {
+      if (lane == 0) part[unit] = make_float4(s.m, s.S, s.A, 0.0f);
+      if (lane < K) keys[unit * K + lane] = best.key;
+      return;
+    }
+  }
+  write_row<DT>(x, row, r, y, s, best.key, K, lane, o);
+}
+
+// a warp a row: the splits' states and lists, in order
+template <int DT>
+__global__ void __launch_bounds__(256) join_kernel(Logits x, const int64_t* __restrict__ tokens, int64_t ignore, int K,
+                                                   int splits, Out o, const float4* part,
+                                                   const unsigned long long* keys) {
+  pdl_wait();
+  const int lane = threadIdx.x & 31;
+  const int64_t r = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (r >= x.rows) return;
+  const int64_t y = tokens[r];
+  if (y == ignore || y < 0 || y >= x.V) return;
+  State s{-INFINITY, 0.0f, 0.0f};
+  if (lane < splits) {
+    const float4 p = part[r * splits + lane];
+    s = State{p.x, p.y, p.z};
+  }
+  s.join_warp();
+  Best best(K > 0 ? K : 1, lane);
+  for (int k = 0; k < splits && K > 0; ++k) best.merge(lane < K ? keys[(r * splits + k) * K + lane] : 0ull);
+  write_row<DT>(x, reinterpret_cast<const typename Elem<DT>::T*>(x.base) + r * x.sr, r, y, s, best.key, K, lane, o);
+}
+
+// ---------------------------------------------------------------- backward
+
+struct Grads {
+  const float *logp, *entropy, *top;
+  const int64_t* top_idx;
+  const float4* stats;
+};
+
+// dz_j = 2^t_j (a t_j + b), and g_logp, g_top added at their symbols
+template <int DT, int VEC, int U, int GT>
+__global__ void __launch_bounds__(256) bwd_kernel(Logits x, const int64_t* __restrict__ tokens, int64_t ignore, int K,
+                                                  int splits, Grads g, typename Elem<DT>::T* __restrict__ grad) {
+  using E = typename Elem<DT>::T;
+  using TL = Tiles<DT, VEC, U, GT>;
+  extern __shared__ uint4 ring[];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t unit = GT == 32 ? (int64_t)blockIdx.x * 8 + warp : (int64_t)blockIdx.x;
+  const int64_t r = GT == 32 ? unit : unit / splits;
+  const int split = GT == 32 ? 0 : (int)(unit - r * splits);
+  if (r >= x.rows) return;
+  const int64_t y = __ldg(tokens + r);
+  const bool used = y != ignore && y >= 0 && y < x.V;
+  const E* row = reinterpret_cast<const E*>(x.base) + r * x.sr;
+  E* out = grad + r * x.V;
+  const int64_t ot = x.rows * x.V;  // step stride of the gradient
+  const int head = head_of<DT, VEC>(row, x.V), tail = (x.V - head) % VEC;
+  int lo, hi;
+  range_of<VEC>(x.V, head, split, splits, lo, hi);
+  const int tid = GT == 32 ? lane : (int)threadIdx.x;
+  const int edge = VEC == 1 || split > 0 ? -1 : tid < head ? tid : tid >= GT - tail ? x.V - (GT - tid) : -1;
+  if (!used) {
+    float zero[VEC];
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) zero[i] = 0.0f;
+    for (int t = 0; t < x.T; ++t) {
+      for (int j = lo + tid * VEC; j < hi; j += GT * VEC) Vec<DT, VEC>::store(out + t * ot + j, zero);
+      if (edge >= 0) out[t * ot + edge] = Elem<DT>::make(0.0f);
+    }
+    return;
+  }
+  TL tl(ring, row, x.st, x.T, lo, hi, tid);
+  const float4 sv = g.stats[r];
+  const Ref f = {sv.x, sv.y};
+  const float gl = g.logp ? g.logp[r] : 0.0f, gh = g.entropy ? g.entropy[r] : 0.0f;
+  float G = gl;
+  if (g.top)
+    for (int k = 0; k < K; ++k) G += g.top[r * K + k];
+  const float scale = x.inv_t / sv.z;  // 1 / (T S)
+  const float a = -gh * kLn2 * scale, b = -(G + gh * (sv.w - kLn2 * log2f(sv.z))) * scale;
+  const float2 l2 = make_float2(kLog2e, kLog2e), c2 = make_float2(-f.c, -f.c), a2 = make_float2(a, a),
+               b2 = make_float2(b, b);
+  auto at_one = [&](float z) {
+    const float t = not_below(log2_from(z, f));
+    return exp2_approx(t) * fmaf(a, t, b);
+  };
+  const int tiles = tl.tiles();
+  for (int k = 0; k < tiles; ++k) {
+    float z[TL::N];
+    tl.mean(k, x.inv_t, z);
+    if (f.off != 0.0f)
+#pragma unroll
+      for (int i = 0; i < TL::N; ++i) z[i] -= f.off;
+#pragma unroll
+    for (int i = 0; i < TL::N; i += 2) {
+      float2 t = fma2(make_float2(z[i], z[i + 1]), l2, c2);
+      t = make_float2(not_below(t.x), not_below(t.y));
+      const float2 d = mul2(make_float2(exp2_approx(t.x), exp2_approx(t.y)), fma2(a2, t, b2));
+      z[i] = d.x;
+      z[i + 1] = d.y;
+    }
+    const int j0 = tl.first(k);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int j = j0 + u * GT * VEC;
+      if (j < hi) {
+        float v[VEC];
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) v[i] = z[u * VEC + i];
+        const typename Vec<DT, VEC>::W w = Vec<DT, VEC>::pack(v);
+        for (int t = 0; t < x.T; ++t) *reinterpret_cast<typename Vec<DT, VEC>::W*>(out + t * ot + j) = w;
+      }
+    }
+  }
+  if constexpr (VEC > 1) asm volatile("cp.async.wait_all;" ::: "memory");
+  if (edge >= 0) {
+    const E d = Elem<DT>::make(at_one(mean_over_t<DT>(row + edge, x.st, x.T, x.inv_t)));
+    for (int t = 0; t < x.T; ++t) out[t * ot + edge] = d;
+  }
+  // the named symbols once more, by one warp after the others' writes: lane k the k-th
+  // alternative, then the token where it is none of them
+  if constexpr (GT > 32) __syncthreads();
+  else __syncwarp();
+  if (GT > 32 && warp > 0) return;
+  auto mine = [&](int64_t j) {  // of this block's share of the row
+    return (j >= lo && j < hi) || (split == 0 && VEC > 1 && (j < head || j >= x.V - tail));
+  };
+  auto put = [&](int64_t j, float add) {
+    const E d = Elem<DT>::make(fmaf(add, x.inv_t, at_one(mean_over_t<DT>(row + j, x.st, x.T, x.inv_t))));
+    for (int t = 0; t < x.T; ++t) out[t * ot + j] = d;
+  };
+  bool is_top = false;
+  if (g.top && lane < K) {
+    const int64_t j = g.top_idx[r * K + lane];
+    is_top = j == y;
+    if (mine(j)) put(j, g.top[r * K + lane] + (is_top ? gl : 0.0f));
+  }
+  is_top = __any_sync(0xffffffffu, is_top);
+  if (lane == 0 && !is_top && mine(y)) put(y, gl);
+}
+
+// ---------------------------------------------------------------- host
+
+// blocks that a row is cut over, so that there are two for every SM
+inline int splits_of(int64_t rows, int64_t V) {
+  if (V <= kWarpRow * 4) return 1;
+  int64_t s = (2 * (int64_t)num_sms() + rows - 1) / rows;
+  const int64_t most = V / 2048;
+  if (s > most) s = most;
+  return (int)(s > 32 ? 32 : s < 1 ? 1 : s);
+}
+inline bool warp_rows(int64_t V) { return V <= kWarpRow; }
+
+// 48 KB of dynamic shared memory without asking, the kernel's static arrays included
+template <typename K>
+bool ask_smem(K kernel, int bytes) {
+  return bytes <= (40 << 10) ||
+         cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) == cudaSuccess;
+}
+
+template <int DT, int VEC, int U, int GT>
+int launch_fwd(const Logits& x, const int64_t* tokens, int64_t ignore, int K, int splits, const Out& o, float4* part,
+               unsigned long long* keys, int* bad, cudaStream_t st) {
+  const int64_t units = GT == 32 ? (x.rows + 7) / 8 : x.rows * splits;
+  const bool scan = x.rows <= kScanTokens;
+  if (!scan) cudaMemsetAsync(bad, 0, sizeof(int), st);
+  constexpr int smem = Tiles<DT, VEC, U, GT>::kBytes * 256;
+  if (!ask_smem(fwd_kernel<DT, VEC, U, GT>, smem)) return check_launch("token_logprobs_fwd");
+  fwd_kernel<DT, VEC, U, GT><<<(unsigned)(units + (scan ? 1 : 0)), 256, smem, st>>>(x, tokens, ignore, K, splits, o, part,
+                                                                                   keys, bad, scan ? 1 : 0);
+  if (splits > 1) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)((x.rows + 7) / 8));
+    cfg.blockDim = dim3(256);
+    cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    add_pdl_attr(cfg, at);
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, join_kernel<DT>, x, tokens, ignore, K, splits, o, (const float4*)part,
+                                             (const unsigned long long*)keys);
+    if (e != cudaSuccess) return fail(SPK_ERR_LAUNCH, "token_logprobs_fwd: %s", cudaGetErrorString(e));
+  }
+  return check_launch("token_logprobs_fwd");
+}
+
+template <int DT>
+int dispatch_fwd(bool wide, const Logits& x, const int64_t* tokens, int64_t ignore, int K, int splits, const Out& o,
+                 float4* part, unsigned long long* keys, int* bad, cudaStream_t st) {
+  constexpr int kWide = 16 / (int)sizeof(typename Elem<DT>::T);
+#define GO(VEC, U, GT) launch_fwd<DT, VEC, U, GT>(x, tokens, ignore, K, splits, o, part, keys, bad, st)
+  if (warp_rows(x.V)) return wide ? GO(kWide, 16 / kWide / 2, 32) : GO(1, 8, 32);
+  return wide ? GO(kWide, 16 / kWide, 256) : GO(1, 8, 256);
+#undef GO
+}
+
+template <int DT, int VEC, int U, int GT>
+int launch_bwd(const Logits& x, const int64_t* tokens, int64_t ignore, int K, int splits, const Grads& g, void* grad,
+               cudaStream_t st) {
+  const int64_t units = GT == 32 ? (x.rows + 7) / 8 : x.rows * splits;
+  constexpr int smem = Tiles<DT, VEC, U, GT>::kBytes * 256;
+  if (!ask_smem(bwd_kernel<DT, VEC, U, GT>, smem)) return check_launch("token_logprobs_bwd");
+  bwd_kernel<DT, VEC, U, GT><<<(unsigned)units, 256, smem, st>>>(x, tokens, ignore, K, splits, g,
+                                                                reinterpret_cast<typename Elem<DT>::T*>(grad));
+  return check_launch("token_logprobs_bwd");
+}
+
+template <int DT>
+int dispatch_bwd(bool wide, const Logits& x, const int64_t* tokens, int64_t ignore, int K, int splits, const Grads& g,
+                 void* grad, cudaStream_t st) {
+  constexpr int kWide = 16 / (int)sizeof(typename Elem<DT>::T);
+#define GO(VEC, U, GT) launch_bwd<DT, VEC, U, GT>(x, tokens, ignore, K, splits, g, grad, st)
+  if (warp_rows(x.V)) return wide ? GO(kWide, 16 / kWide / 2, 32) : GO(1, 8, 32);
+  return wide ? GO(kWide, 16 / kWide, 256) : GO(1, 8, 256);
+#undef GO
+}
 
 }  // namespace lpk
 }  // namespace spk
 
 #define SPK_LP_SIZES()                                                                                              \
   SPK_REQUIRE(float_type(dtype), SPK_ERR_INVALID, "logits must be fp32, fp16 or bf16");                            \
-  SPK_REQUIRE(T >= 1 && T <= 64 && rows >= 1 && rows < (1ll << 31) && V >= 1 && V < (1ll << 30), SPK_ERR_SHAPE,     \
+  SPK_REQUIRE(T >= 1 && T <= 64 && rows >= 1 && rows < (1ll << 25) && V >= 1 && V < (1ll << 30), SPK_ERR_SHAPE,     \
               "unsupported sizes T=%lld rows=%lld V=%lld", (long long)T, (long long)rows, (long long)V);            \
   SPK_REQUIRE((T == 1 || step_stride >= 0) && (rows == 1 || row_stride >= 0), SPK_ERR_SHAPE, "negative stride");    \
   SPK_REQUIRE(top_k >= 0 && top_k <= kMaxTop && top_k <= V, SPK_ERR_SHAPE, "top_k=%lld: at most %d and V",          \
-              (long long)top_k, kMaxTop)
+              (long long)top_k, kMaxTop);                                                                           \
+  SPK_REQUIRE(aligned(stats, 16), SPK_ERR_ALIGN, "stats must be 16-byte aligned")
 
 extern "C" {
 
-int64_t spk_token_logprobs_workspace_bytes(int64_t, int64_t, int64_t, int64_t) { return 16; }
+int64_t spk_token_logprobs_workspace_bytes(int64_t, int64_t rows, int64_t V, int64_t top_k) {
+  if (rows < 1 || V < 1 || top_k < 0) return 16;
+  const int64_t s = spk::lpk::splits_of(rows, V);
+  return s > 1 ? rows * s * (16 + 8 * top_k) : 16;
+}
 
 int spk_token_logprobs_fwd(const void* logits, int dtype, int64_t T, int64_t rows, int64_t V, int64_t step_stride,
                            int64_t row_stride, const int64_t* tokens, int64_t ignore_index, int64_t top_k, float* logp,
@@ -234,24 +691,21 @@ int spk_token_logprobs_fwd(const void* logits, int dtype, int64_t T, int64_t row
   SPK_REQUIRE(logits && tokens && logp && entropy && stats && bad_token, SPK_ERR_INVALID, "null pointer argument");
   SPK_LP_SIZES();
   SPK_REQUIRE(top_k == 0 || (top_logp && top_idx), SPK_ERR_INVALID, "null top_logp or top_idx");
-  SPK_REQUIRE(aligned(stats, 16), SPK_ERR_ALIGN, "stats must be 16-byte aligned");
   SPK_REQUIRE(workspace && workspace_bytes >= spk_token_logprobs_workspace_bytes(T, rows, V, top_k), SPK_ERR_INVALID,
               "workspace smaller than spk_token_logprobs_workspace_bytes()");
+  SPK_REQUIRE(aligned(workspace, 16), SPK_ERR_ALIGN, "workspace must be 16-byte aligned");
   int rc = check_stream_device(stream);
   if (rc != SPK_OK) return rc;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  cudaMemsetAsync(bad_token, 0, sizeof(int), s);
-  const int64_t cap = (int64_t)num_sms() * 16;
-  const unsigned grid = (unsigned)(rows < cap ? rows : cap);
-#define LAUNCH(DT)                                                                                                  \
-  fwd_kernel<DT><<<grid, kThreads, 0, s>>>(reinterpret_cast<const Elem<DT>::T*>(logits), (int)T, rows, (int)V,      \
-                                           step_stride, row_stride, tokens, ignore_index, (int)top_k, logp, entropy, \
-                                           top_logp, top_idx, stats, bad_token)
-  if (dtype == SPK_F32) LAUNCH(SPK_F32);
-  else if (dtype == SPK_F16) LAUNCH(SPK_F16);
-  else LAUNCH(SPK_BF16);
-#undef LAUNCH
-  return check_launch("token_logprobs_fwd");
+  const Logits x = {logits, (int)T, (int)V, rows, step_stride, row_stride, 1.0f / (float)T};
+  const Out o = {logp, entropy, top_logp, top_idx, reinterpret_cast<float4*>(stats)};
+  const int splits = splits_of(rows, V), K = (int)top_k;
+  float4* part = reinterpret_cast<float4*>(workspace);
+  unsigned long long* keys = reinterpret_cast<unsigned long long*>(part + rows * splits);
+  // the steps of a value lie alike to 16 bytes
+  const bool wide = aligned(logits, dtype_size(dtype)) && (T == 1 || step_stride * dtype_size(dtype) % 16 == 0);
+  auto go = dtype == SPK_F32 ? dispatch_fwd<SPK_F32> : dtype == SPK_F16 ? dispatch_fwd<SPK_F16> : dispatch_fwd<SPK_BF16>;
+  return go(wide, x, tokens, ignore_index, K, splits, o, part, keys, bad_token, s);
 }
 
 int spk_token_logprobs_bwd(const void* logits, int dtype, int64_t T, int64_t rows, int64_t V, int64_t step_stride,
@@ -263,21 +717,18 @@ int spk_token_logprobs_bwd(const void* logits, int dtype, int64_t T, int64_t row
   SPK_REQUIRE(logits && tokens && stats && grad, SPK_ERR_INVALID, "null pointer argument");
   SPK_LP_SIZES();
   SPK_REQUIRE(!g_top || top_idx, SPK_ERR_INVALID, "null top_idx");
-  SPK_REQUIRE(aligned(stats, 16), SPK_ERR_ALIGN, "stats must be 16-byte aligned");
   int rc = check_stream_device(stream);
   if (rc != SPK_OK) return rc;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  const int64_t cap = (int64_t)num_sms() * 16;
-  const unsigned grid = (unsigned)(rows < cap ? rows : cap);
-#define LAUNCH(DT)                                                                                               \
-  bwd_kernel<DT><<<grid, kThreads, 0, s>>>(reinterpret_cast<const Elem<DT>::T*>(logits), (int)T, rows, (int)V,   \
-                                           step_stride, row_stride, tokens, ignore_index, (int)top_k, top_idx,   \
-                                           stats, g_logp, g_entropy, g_top, reinterpret_cast<Elem<DT>::T*>(grad))
-  if (dtype == SPK_F32) LAUNCH(SPK_F32);
-  else if (dtype == SPK_F16) LAUNCH(SPK_F16);
-  else LAUNCH(SPK_BF16);
-#undef LAUNCH
-  return check_launch("token_logprobs_bwd");
+  const Logits x = {logits, (int)T, (int)V, rows, step_stride, row_stride, 1.0f / (float)T};
+  const Grads g = {g_logp, g_entropy, g_top, top_idx, reinterpret_cast<const float4*>(stats)};
+  const int64_t e = dtype_size(dtype);
+  // the steps of a value, and its gradient's, lie alike to 16 bytes
+  const bool wide = aligned(logits, (int)e) && (T == 1 || (step_stride * e % 16 == 0 && rows * V * e % 16 == 0)) &&
+                    (rows == 1 || (row_stride - V) * e % 16 == 0) &&
+                    (reinterpret_cast<uintptr_t>(logits) - reinterpret_cast<uintptr_t>(grad)) % 16 == 0;
+  auto go = dtype == SPK_F32 ? dispatch_bwd<SPK_F32> : dtype == SPK_F16 ? dispatch_bwd<SPK_F16> : dispatch_bwd<SPK_BF16>;
+  return go(wide, x, tokens, ignore_index, (int)top_k, splits_of(rows, V), g, grad, s);
 }
 
 }  // extern "C"

@@ -52,6 +52,23 @@ __device__ __forceinline__ void st_any(void* p, int dt, int64_t i, float v) {
   else reinterpret_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
 }
 
+// Whether a token lies outside [0, V) and is not `ignore`, by one block: the only
+// writer of *bad, so nothing has to clear it first.  For up to kScanTokens tokens
+// (a few microseconds beside the other blocks); more are marked by the blocks
+// that meet them, after a memset.
+constexpr int64_t kScanTokens = 16384;
+__device__ __forceinline__ void scan_tokens(const int64_t* __restrict__ tokens, int64_t n, int64_t V, int64_t ignore,
+                                            int* bad) {
+  int any = 0;
+#pragma unroll 8
+  for (int64_t i = threadIdx.x; i < n; i += blockDim.x) {
+    const int64_t t = __ldg(tokens + i);
+    any |= t != ignore && (t < 0 || t >= V);
+  }
+  any = __syncthreads_or(any);
+  if (threadIdx.x == 0) *bad = any;
+}
+
 inline bool float_type(int dt) { return dt == SPK_F32 || dt == SPK_F16 || dt == SPK_BF16; }
 
 }  // namespace spk
