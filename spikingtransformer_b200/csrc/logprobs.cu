@@ -71,18 +71,16 @@ struct State {
     S *= k;
     m = nm;
   }
-  __device__ __forceinline__ void join(State o) {
-    const float nm = fmaxf(m, o.m);
-    if (nm > m) move_to(nm);
-    if (nm > o.m) o.move_to(nm);
-    S += o.S;
-    A += o.A;
-  }
   __device__ __forceinline__ void join_warp() {
+    float nm = m;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1)
-      join(State{__shfl_xor_sync(0xffffffffu, m, o), __shfl_xor_sync(0xffffffffu, S, o),
-                 __shfl_xor_sync(0xffffffffu, A, o)});
+    for (int o = 16; o > 0; o >>= 1) nm = fmaxf(nm, __shfl_xor_sync(0xffffffffu, nm, o));
+    if (nm > m) move_to(nm);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      S += __shfl_xor_sync(0xffffffffu, S, o);
+      A += __shfl_xor_sync(0xffffffffu, A, o);
+    }
   }
 };
 
@@ -106,6 +104,13 @@ __device__ __forceinline__ void add_exactly(float& s, float& err, float v) {
   const float n = __fadd_rn(s, v);
   const float b = __fsub_rn(n, s);
   err = __fadd_rn(err, __fadd_rn(__fsub_rn(s, __fsub_rn(n, b)), __fsub_rn(v, b)));
+  s = n;
+}
+__device__ __forceinline__ float2 sub2(float2 a, float2 b) { return fma2(b, make_float2(-1.0f, -1.0f), a); }
+__device__ __forceinline__ void add_exactly(float2& s, float2& err, float2 v) {
+  const float2 n = add2(s, v);
+  const float2 b = sub2(n, s);
+  err = add2(err, add2(sub2(s, sub2(n, b)), sub2(v, b)));
   s = n;
 }
 
@@ -148,6 +153,32 @@ struct Logits {  // element (t, r, v) at base + t st + r sr + v
   float inv_t;
 };
 
+// A tile's values as words (a 16-bit value alone is a word's lower half), and as pairs of fp32.
+template <int DT>
+__device__ __forceinline__ uint32_t one_word(const typename Elem<DT>::T* p) {
+  if constexpr (DT == SPK_F32) return __float_as_uint(*p);
+  else return *reinterpret_cast<const uint16_t*>(p);
+}
+template <int DT>
+__device__ __forceinline__ float2 unpack_pair(uint32_t w) {  // two 16-bit values
+  if constexpr (DT == SPK_BF16) return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+  else return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+template <int DT, int VEC, int WORDS, int P>
+__device__ __forceinline__ void unpack_words(const uint32_t (&w)[WORDS], float2 (&z)[P]) {
+#pragma unroll
+  for (int i = 0; i < P; ++i) {
+    if constexpr (DT == SPK_F32) z[i] = make_float2(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
+    else if constexpr (VEC > 1) z[i] = unpack_pair<DT>(w[i]);
+    else z[i] = make_float2(unpack_pair<DT>(w[2 * i]).x, unpack_pair<DT>(w[2 * i + 1]).x);
+  }
+}
+// a value's bits where there is none: -inf, in both halves of a word of two
+template <int DT>
+__device__ __forceinline__ constexpr uint32_t no_value() {
+  return DT == SPK_F32 ? 0xff800000u : DT == SPK_BF16 ? 0xff80ff80u : 0xfc00fc00u;
+}
+
 // Values [lo, hi) of a row in tiles of GT threads x U vectors of VEC; thread
 // tid's vector u of a tile begins at lo + ((tile U + u) GT + tid) VEC.
 template <int DT, int VEC, int U, int GT>
@@ -155,8 +186,10 @@ struct Tiles {
   using E = typename Elem<DT>::T;
   using W = typename Vec<DT, VEC>::W;
   static constexpr int N = U * VEC, kSpan = GT * U * VEC;
+  static constexpr int kWords = VEC > 1 ? U * 4 : U;
   static constexpr int kBytes = VEC > 1 ? kStages * U * 16 : 0;  // of shared memory a thread
   static_assert(VEC == 1 || sizeof(W) == 16, "16-byte vectors");
+  static_assert(N % 2 == 0, "pairs");
   const E* row;
   int64_t st;
   int T, lo, hi, tid;
@@ -189,56 +222,68 @@ struct Tiles {
       fp += st;
     }
   }
-  // one step of the tile whose first value of this thread is j0; absent values stay as they are
-  __device__ __forceinline__ void take(int j0, int t, float (&v)[N]) {
+  // the words of one step of the tile whose first value of this thread is j0; `none` where there is no value
+  __device__ __forceinline__ void take(int j0, int t, uint32_t none, uint32_t (&w)[kWords]) {
     if constexpr (VEC > 1) {
       asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
 #pragma unroll
-      for (int u = 0; u < U; ++u)
-        if (j0 + u * GT * VEC < hi) {
-          W w;
-          asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
-                       : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w)
-                       : "r"(ring + at + u * 256 * 16)
-                       : "memory");
-          float x[VEC];
-          Vec<DT, VEC>::unpack(w, x);
-#pragma unroll
-          for (int i = 0; i < VEC; ++i) v[u * VEC + i] = x[i];
-        }
+      for (int u = 0; u < U; ++u) {
+        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(w[4 * u]), "=r"(w[4 * u + 1]), "=r"(w[4 * u + 2]), "=r"(w[4 * u + 3])
+                     : "r"(ring + at + u * 256 * 16)
+                     : "memory");
+        if (j0 + u * GT * VEC >= hi) w[4 * u] = w[4 * u + 1] = w[4 * u + 2] = w[4 * u + 3] = none;
+      }
+      fetch();
     } else {
 #pragma unroll
-      for (int u = 0; u < U; ++u)
-        if (j0 + u * GT < hi) v[u] = Elem<DT>::load(row + t * st + j0 + u * GT);
+      for (int u = 0; u < U; ++u) {
+        w[u] = none;
+        if (j0 + u * GT < hi) w[u] = one_word<DT>(row + t * st + j0 + u * GT);
+      }
     }
   }
-  // z of a tile, -inf where there is no value; the next stages are on their way
-  __device__ __forceinline__ void mean(int tile, float inv_t, float (&z)[N]) {
-    const int j0 = first(tile);
+  // z of a tile of several steps, -inf where there is no value
+  __device__ __forceinline__ void mean(int j0, float inv_t, float2 (&z)[N / 2]) {
+    uint32_t w[kWords];
+    float2 err[N / 2];
+    take(j0, 0, 0u, w);
+    unpack_words<DT, VEC>(w, z);
 #pragma unroll
-    for (int i = 0; i < N; ++i) z[i] = -INFINITY;
-    take(j0, 0, z);
-    if constexpr (VEC > 1) fetch();
-    if (T == 1) return;
-    float err[N];
-#pragma unroll
-    for (int i = 0; i < N; ++i) err[i] = 0.0f;
+    for (int i = 0; i < N / 2; ++i) err[i] = make_float2(0.0f, 0.0f);
     for (int t = 1; t < T; ++t) {
-      float v[N];
+      float2 v[N / 2];
+      take(j0, t, 0u, w);
+      unpack_words<DT, VEC>(w, v);
 #pragma unroll
-      for (int i = 0; i < N; ++i) v[i] = 0.0f;
-      take(j0, t, v);
-      if constexpr (VEC > 1) fetch();
+      for (int i = 0; i < N / 2; ++i) add_exactly(z[i], err[i], v[i]);
+    }
+    float2 odd = make_float2(0.0f, 0.0f);  // NaN if a sum is not finite
 #pragma unroll
-      for (int i = 0; i < N; ++i) add_exactly(z[i], err[i], v[i]);
+    for (int i = 0; i < N / 2; ++i) odd = fma2(z[i], odd, odd);
+    if (odd.x + odd.y == 0.0f) {
+      const float2 r2 = make_float2(inv_t, inv_t), t2 = make_float2(-(float)T, -(float)T);
+#pragma unroll
+      for (int i = 0; i < N / 2; ++i) {
+        const float2 q = mul2(z[i], r2);
+        z[i] = fma2(add2(fma2(q, t2, z[i]), err[i]), r2, q);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const int j = j0 + place(i);
+        if (j < hi) {
+          float& v = i & 1 ? z[i / 2].y : z[i / 2].x;
+          v = mean_of<DT>(v, i & 1 ? err[i / 2].y : err[i / 2].x, row + j, st, T, inv_t);
+        }
+      }
     }
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (j0 + u * GT * VEC < hi)
-#pragma unroll
-        for (int i = 0; i < VEC; ++i)
-          z[u * VEC + i] = mean_of<DT>(z[u * VEC + i], err[u * VEC + i], row + j0 + u * GT * VEC + i, st, T, inv_t);
+    for (int i = 0; i < N; ++i)
+      if (j0 + place(i) >= hi) (i & 1 ? z[i / 2].y : z[i / 2].x) = -INFINITY;
   }
+  // value i's place after the thread's first value of the tile
+  __device__ static __forceinline__ constexpr int place(int i) { return (i / VEC) * GT * VEC + i % VEC; }
   __device__ __forceinline__ int tiles() const { return hi > lo ? (hi - lo + kSpan - 1) / kSpan : 0; }
 };
 
@@ -281,22 +326,15 @@ struct Best {
     full = k != 0;
     floor = full ? order_value((uint32_t)(k >> 32)) : -INFINITY;
   }
-  // the list of another warp, falling, lane k the k-th
-  __device__ __forceinline__ void merge(unsigned long long other) {
-    for (int i = 0; i < K; ++i) {
-      const unsigned long long k = __shfl_sync(0xffffffffu, other, i);
-      if (k <= last()) break;
-      insert(k);
-    }
-  }
-  // N values a lane, value i with index j[i] (< 0: none); `most`: their largest.  The best of
-  // the warp goes into the list, again and again, until none is good enough.
+  // N values a lane, value i with index index(i), rising in i (< 0: none); `most`: their
+  // largest.  The best of the warp goes into the list, again and again, until none is good enough.
   template <int N, typename J>
-  __device__ __forceinline__ void offer(const float (&z)[N], float most, bool ties, J index) {
+  __device__ __forceinline__ void offer(const float2 (&z)[N / 2], float most, bool ties, J index) {
     if (!__any_sync(0xffffffffu, !full || most > floor || (ties && most >= floor))) return;
     uint32_t ord[N];
 #pragma unroll
-    for (int i = 0; i < N; ++i) ord[i] = index(i) >= 0 ? order_bits(z[i]) : 0u;
+    for (int i = 0; i < N; ++i) ord[i] = index(i) >= 0 ? order_bits(i & 1 ? z[i / 2].y : z[i / 2].x) : 0u;
+    const bool fresh = last() == 0 && __shfl_sync(0xffffffffu, key, 0) == 0;
     for (int n = 0; n < K; ++n) {
       uint32_t best = 0, j = 0xffffffffu;
 #pragma unroll
@@ -309,8 +347,12 @@ struct Best {
       if (top == 0) break;
       const uint32_t at = __reduce_min_sync(0xffffffffu, best == top ? j : 0xffffffffu);
       const unsigned long long k = ((unsigned long long)top << 32) | (uint32_t)~at;
-      if (k <= last()) break;
-      insert(k);
+      if (fresh) {  // into an empty list they come in order
+        if (lane == n) key = k;
+      } else {
+        if (k <= last()) break;
+        insert(k);
+      }
       if (best == top && j == at)
 #pragma unroll
         for (int i = 0; i < N; ++i)
@@ -321,18 +363,18 @@ struct Best {
 };
 
 // a tile into the thread's state
-template <int N>
-__device__ __forceinline__ void absorb(State& s, float (&z)[N], float most) {
+template <int P>
+__device__ __forceinline__ void absorb(State& s, float2 (&z)[P], float most) {
   if (most > s.m) s.move_to(most);
   const Ref f = ref_of(s.m);
   if (f.off != 0.0f)
 #pragma unroll
-    for (int i = 0; i < N; ++i) z[i] -= f.off;
+    for (int i = 0; i < P; ++i) z[i] = add2(z[i], make_float2(-f.off, -f.off));
   float2 S2 = make_float2(0.0f, 0.0f), A2 = S2;
   const float2 l2 = make_float2(kLog2e, kLog2e), c2 = make_float2(-f.c, -f.c);
 #pragma unroll
-  for (int i = 0; i < N; i += 2) {
-    float2 t = fma2(make_float2(z[i], z[i + 1]), l2, c2);
+  for (int i = 0; i < P; ++i) {
+    float2 t = fma2(z[i], l2, c2);
     t = make_float2(not_below(t.x), not_below(t.y));
     const float2 e = make_float2(exp2_approx(t.x), exp2_approx(t.y));
     S2 = add2(S2, e);
@@ -340,6 +382,73 @@ __device__ __forceinline__ void absorb(State& s, float (&z)[N], float most) {
   }
   s.S += S2.x + S2.y;
   s.A += A2.x + A2.y;
+}
+
+// The same for 16-bit logits of one step, in pairs before they are unpacked: the
+// maximum, and instead of holding t at -200 the logits at a finite value whose
+// 2^t is 0 too (-1e30, and fp16's lowest), half an instruction each.  A
+// maximum beyond kFar, or near fp16's lowest, takes the way above.
+template <int DT, int WORDS>
+__device__ __forceinline__ float most_of(const uint32_t (&w)[WORDS]) {
+  uint32_t m = w[0];
+#pragma unroll
+  for (int i = 1; i < WORDS; ++i) {
+    if constexpr (DT == SPK_BF16) asm("max.bf16x2 %0, %1, %2;" : "=r"(m) : "r"(m), "r"(w[i]));
+    else asm("max.f16x2 %0, %1, %2;" : "=r"(m) : "r"(m), "r"(w[i]));
+  }
+  const float2 v = unpack_pair<DT>(m);
+  return fmaxf(v.x, v.y);
+}
+template <int DT, int WORDS>
+__device__ __forceinline__ void absorb_words(State& s, const uint32_t (&w)[WORDS], float most) {
+  if (most > s.m) s.move_to(most);
+  const Ref f = ref_of(s.m);
+  if (f.off != 0.0f || s.m < -32768.0f) {
+    float2 z[WORDS];
+#pragma unroll
+    for (int i = 0; i < WORDS; ++i) z[i] = unpack_pair<DT>(w[i]);
+    absorb(s, z, most);
+    return;
+  }
+  float2 S2 = make_float2(0.0f, 0.0f), A2 = S2;
+  const float2 l2 = make_float2(kLog2e, kLog2e), c2 = make_float2(-f.c, -f.c);
+#pragma unroll
+  for (int i = 0; i < WORDS; ++i) {
+    uint32_t v;
+    if constexpr (DT == SPK_BF16) asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(v) : "r"(w[i]), "r"(0xf149f149u));
+    else asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(v) : "r"(w[i]), "r"(0xfbfffbffu));
+    const float2 t = fma2(unpack_pair<DT>(v), l2, c2);
+    const float2 e = make_float2(exp2_approx(t.x), exp2_approx(t.y));
+    S2 = add2(S2, e);
+    A2 = fma2(e, t, A2);
+  }
+  s.S += S2.x + S2.y;
+  s.A += A2.x + A2.y;
+}
+
+template <int P>
+__device__ __forceinline__ float most_of(const float2 (&z)[P]) {
+  float m = fmaxf(z[0].x, z[0].y);
+#pragma unroll
+  for (int i = 1; i < P; ++i) m = fmaxf(m, fmaxf(z[i].x, z[i].y));
+  return m;
+}
+
+// The K best of up to 32 falling lists of 64-bit keys in shared memory (lane l
+// walks list l): lane k gets the k-th.
+__device__ __forceinline__ unsigned long long best_of_lists(const unsigned long long* list, int lists, int stride, int K,
+                                                            int lane) {
+  unsigned long long mine = 0;
+  int at = 0;
+  for (int n = 0; n < K; ++n) {
+    const unsigned long long head = lane < lists && at < K ? list[lane * stride + at] : 0ull;
+    const uint32_t hi = __reduce_max_sync(0xffffffffu, (uint32_t)(head >> 32));
+    const uint32_t lo = __reduce_max_sync(0xffffffffu, (uint32_t)(head >> 32) == hi ? (uint32_t)head : 0u);
+    const unsigned long long top = ((unsigned long long)hi << 32) | lo;
+    if (lane == n) mine = top;
+    if (head == top) ++at;
+  }
+  return mine;
 }
 
 struct Out {
@@ -377,7 +486,8 @@ __device__ __forceinline__ void write_unused(int64_t r, int K, int lane, const O
   }
 }
 
-constexpr int kWarpRow = 1024;  // values of a row that one warp takes (fewer rows than warps aside)
+// Values of a row that one warp takes, where there are rows for 16 warps on every SM.
+constexpr int kWarpRow = 1024;
 
 // GT = 32: a warp a row.  GT = 256: a block a (row, split); with several splits
 // the state and list go to part / keys.
@@ -413,27 +523,42 @@ __global__ void __launch_bounds__(256) fwd_kernel(Logits x, const int64_t* __res
   State s{-INFINITY, 0.0f, 0.0f};
   Best best(K > 0 ? K : 1, lane);
   const int tiles = tl.tiles();
-  constexpr int N = Tiles<DT, VEC, U, GT>::N;
+  using TL = Tiles<DT, VEC, U, GT>;
+  constexpr int N = TL::N;
   for (int k = 0; k < tiles; ++k) {
-    float z[N];
-    tl.mean(k, x.inv_t, z);
-    float most = z[0];
-#pragma unroll
-    for (int i = 1; i < N; ++i) most = fmaxf(most, z[i]);
     const int j0 = tl.first(k);
-    if (K > 0)
-      best.offer(z, most, false, [&](int i) {
-        const int j = j0 + (i / VEC) * GT * VEC;
-        return j < hi ? j + i % VEC : -1;
-      });
+    auto index = [&](int i) {
+      const int j = j0 + TL::place(i);
+      return j < hi ? j : -1;
+    };
+    float2 z[N / 2];
+    if (x.T == 1) {
+      uint32_t w[TL::kWords];
+      tl.take(j0, 0, no_value<DT>(), w);
+      if constexpr (VEC > 1 && DT != SPK_F32) {
+        const float most = most_of<DT>(w);
+        if (K > 0) {
+          unpack_words<DT, VEC>(w, z);
+          best.template offer<N>(z, most, false, index);
+        }
+        absorb_words<DT>(s, w, most);
+        continue;
+      }
+      unpack_words<DT, VEC>(w, z);
+    } else {
+      tl.mean(j0, x.inv_t, z);
+    }
+    const float most = most_of(z);
+    if (K > 0) best.template offer<N>(z, most, false, index);
     absorb(s, z, most);
   }
   if constexpr (VEC > 1) asm volatile("cp.async.wait_all;" ::: "memory");
   if (VEC > 1 && split == 0 && head + tail > 0) {  // the values beside the vectors
     const int j = tid < head ? tid : tid >= GT - tail ? x.V - (GT - tid) : -1;
-    float z[2] = {j >= 0 ? mean_over_t<DT>(row + j, x.st, x.T, x.inv_t) : -INFINITY, -INFINITY};
-    if (K > 0) best.offer(z, z[0], true, [&](int i) { return i == 0 ? j : -1; });
-    absorb(s, z, z[0]);
+    float2 z[1] = {make_float2(j >= 0 ? mean_over_t<DT>(row + j, x.st, x.T, x.inv_t) : -INFINITY, -INFINITY)};
+    const float most = z[0].x;
+    if (K > 0) best.template offer<2>(z, most, true, [&](int i) { return i == 0 ? j : -1; });
+    absorb(s, z, most);
   }
   s.join_warp();
   if constexpr (GT > 32) {
@@ -443,10 +568,9 @@ __global__ void __launch_bounds__(256) fwd_kernel(Logits x, const int64_t* __res
     wk[warp][lane] = best.key;
     __syncthreads();
     if (warp > 0) return;
-    s = State{-INFINITY, 0.0f, 0.0f};
-    for (int w = 0; w < 8; ++w) s.join(ws[w]);
-    if (K > 0)
-      for (int w = 1; w < 8; ++w) best.merge(wk[w][lane]);
+    s = lane < 8 ? ws[lane] : State{-INFINITY, 0.0f, 0.0f};
+    s.join_warp();
+    if (K > 0) best.key = best_of_lists(wk[0], 8, kMaxTop, K, lane);
     if (splits > 1) {
       if (lane == 0) part[unit] = make_float4(s.m, s.S, s.A, 0.0f);
       if (lane < K) keys[unit * K + lane] = best.key;
@@ -456,26 +580,26 @@ __global__ void __launch_bounds__(256) fwd_kernel(Logits x, const int64_t* __res
   write_row<DT>(x, row, r, y, s, best.key, K, lane, o);
 }
 
-// a warp a row: the splits' states and lists, in order
+// a block of one warp a row: the splits' states and lists
 template <int DT>
-__global__ void __launch_bounds__(256) join_kernel(Logits x, const int64_t* __restrict__ tokens, int64_t ignore, int K,
-                                                   int splits, Out o, const float4* part,
-                                                   const unsigned long long* keys) {
+__global__ void __launch_bounds__(32) join_kernel(Logits x, const int64_t* __restrict__ tokens, int64_t ignore, int K,
+                                                  int splits, Out o, const float4* part, const unsigned long long* keys) {
+  __shared__ unsigned long long list[32 * kMaxTop];
+  const int lane = threadIdx.x;
+  const int64_t r = blockIdx.x, y = tokens[r];
   pdl_wait();
-  const int lane = threadIdx.x & 31;
-  const int64_t r = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-  if (r >= x.rows) return;
-  const int64_t y = tokens[r];
   if (y == ignore || y < 0 || y >= x.V) return;
   State s{-INFINITY, 0.0f, 0.0f};
   if (lane < splits) {
     const float4 p = part[r * splits + lane];
     s = State{p.x, p.y, p.z};
   }
+#pragma unroll 8
+  for (int i = lane; i < splits * K; i += 32) list[i] = keys[r * splits * K + i];
+  __syncwarp();
   s.join_warp();
-  Best best(K > 0 ? K : 1, lane);
-  for (int k = 0; k < splits && K > 0; ++k) best.merge(lane < K ? keys[(r * splits + k) * K + lane] : 0ull);
-  write_row<DT>(x, reinterpret_cast<const typename Elem<DT>::T*>(x.base) + r * x.sr, r, y, s, best.key, K, lane, o);
+  const unsigned long long key = K > 0 ? best_of_lists(list, splits, K, K, lane) : 0ull;
+  write_row<DT>(x, reinterpret_cast<const typename Elem<DT>::T*>(x.base) + r * x.sr, r, y, s, key, K, lane, o);
 }
 
 // ---------------------------------------------------------------- backward
@@ -535,27 +659,31 @@ __global__ void __launch_bounds__(256) bwd_kernel(Logits x, const int64_t* __res
   };
   const int tiles = tl.tiles();
   for (int k = 0; k < tiles; ++k) {
-    float z[TL::N];
-    tl.mean(k, x.inv_t, z);
+    const int j0 = tl.first(k);
+    float2 z[TL::N / 2];
+    if (x.T == 1) {
+      uint32_t w[TL::kWords];
+      tl.take(j0, 0, no_value<DT>(), w);
+      unpack_words<DT, VEC>(w, z);
+    } else {
+      tl.mean(j0, x.inv_t, z);
+    }
     if (f.off != 0.0f)
 #pragma unroll
-      for (int i = 0; i < TL::N; ++i) z[i] -= f.off;
+      for (int i = 0; i < TL::N / 2; ++i) z[i] = add2(z[i], make_float2(-f.off, -f.off));
 #pragma unroll
-    for (int i = 0; i < TL::N; i += 2) {
-      float2 t = fma2(make_float2(z[i], z[i + 1]), l2, c2);
+    for (int i = 0; i < TL::N / 2; ++i) {
+      float2 t = fma2(z[i], l2, c2);
       t = make_float2(not_below(t.x), not_below(t.y));
-      const float2 d = mul2(make_float2(exp2_approx(t.x), exp2_approx(t.y)), fma2(a2, t, b2));
-      z[i] = d.x;
-      z[i + 1] = d.y;
+      z[i] = mul2(make_float2(exp2_approx(t.x), exp2_approx(t.y)), fma2(a2, t, b2));
     }
-    const int j0 = tl.first(k);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int j = j0 + u * GT * VEC;
       if (j < hi) {
         float v[VEC];
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) v[i] = z[u * VEC + i];
+        for (int i = 0; i < VEC; ++i) v[i] = (u * VEC + i) & 1 ? z[(u * VEC + i) / 2].y : z[(u * VEC + i) / 2].x;
         const typename Vec<DT, VEC>::W w = Vec<DT, VEC>::pack(v);
         for (int t = 0; t < x.T; ++t) *reinterpret_cast<typename Vec<DT, VEC>::W*>(out + t * ot + j) = w;
       }
@@ -598,7 +726,7 @@ inline int splits_of(int64_t rows, int64_t V) {
   if (s > most) s = most;
   return (int)(s > 32 ? 32 : s < 1 ? 1 : s);
 }
-inline bool warp_rows(int64_t V) { return V <= kWarpRow; }
+inline bool warp_rows(int64_t rows, int64_t V) { return V <= kWarpRow && (V <= 256 || rows >= 16 * (int64_t)num_sms()); }
 
 // 48 KB of dynamic shared memory without asking, the kernel's static arrays included
 template <typename K>
@@ -619,8 +747,8 @@ int launch_fwd(const Logits& x, const int64_t* tokens, int64_t ignore, int K, in
                                                                                    keys, bad, scan ? 1 : 0);
   if (splits > 1) {
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)((x.rows + 7) / 8));
-    cfg.blockDim = dim3(256);
+    cfg.gridDim = dim3((unsigned)x.rows);
+    cfg.blockDim = dim3(32);
     cfg.stream = st;
     cudaLaunchAttribute at[1];
     add_pdl_attr(cfg, at);
@@ -636,8 +764,9 @@ int dispatch_fwd(bool wide, const Logits& x, const int64_t* tokens, int64_t igno
                  float4* part, unsigned long long* keys, int* bad, cudaStream_t st) {
   constexpr int kWide = 16 / (int)sizeof(typename Elem<DT>::T);
 #define GO(VEC, U, GT) launch_fwd<DT, VEC, U, GT>(x, tokens, ignore, K, splits, o, part, keys, bad, st)
-  if (warp_rows(x.V)) return wide ? GO(kWide, 16 / kWide / 2, 32) : GO(1, 8, 32);
-  return wide ? GO(kWide, 16 / kWide, 256) : GO(1, 8, 256);
+  if (warp_rows(x.rows, x.V)) return wide ? GO(kWide, 8 / kWide, 32) : GO(1, 8, 32);
+  if (x.V <= 4096) return wide ? GO(kWide, 1, 256) : GO(1, 4, 256);  // shorter tiles: fewer threads without a value
+  return wide ? GO(kWide, 4, 256) : GO(1, 8, 256);
 #undef GO
 }
 
@@ -657,7 +786,8 @@ int dispatch_bwd(bool wide, const Logits& x, const int64_t* tokens, int64_t igno
                  void* grad, cudaStream_t st) {
   constexpr int kWide = 16 / (int)sizeof(typename Elem<DT>::T);
 #define GO(VEC, U, GT) launch_bwd<DT, VEC, U, GT>(x, tokens, ignore, K, splits, g, grad, st)
-  if (warp_rows(x.V)) return wide ? GO(kWide, 16 / kWide / 2, 32) : GO(1, 8, 32);
+  if (warp_rows(x.rows, x.V)) return wide ? GO(kWide, 8 / kWide, 32) : GO(1, 8, 32);
+  if (x.V <= 4096) return wide ? GO(kWide, 1, 256) : GO(1, 4, 256);  // shorter tiles: fewer threads without a value
   return wide ? GO(kWide, 16 / kWide, 256) : GO(1, 8, 256);
 #undef GO
 }

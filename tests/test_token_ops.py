@@ -631,6 +631,36 @@ def test_barred_symbols_and_rows_without_a_distribution(ops, T, V, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("V", [48, 300, 9000])
+@pytest.mark.parametrize("dtype", FLOATS)
+def test_lowest_values_are_above_minus_infinity(ops, V, dtype):
+    """Rows with the type's lowest value at every third symbol and -inf elsewhere: the
+    former share the probability, the latter have none."""
+    rows = 4
+    x = torch.full((1, rows, V), float("-inf"))
+    x[:, :, ::3] = torch.finfo(dtype).min
+    x[:, 1, 3] = 0.0  # one symbol above them takes it all
+    tok = torch.tensor([0, 3, 1, 0])
+    xd = x.to(dtype).to(DEV).requires_grad_(True)
+    logp, H, top, idx, _ = ops.token_logprobs(xd, tok.to(DEV), top_k=2)
+    (gx,) = torch.autograd.grad(logp[0] + H[3], xd)
+    n = (V + 2) // 3
+    ln = torch.tensor(float(n), dtype=torch.float64).log()
+    tol = (V / 128 + 80) * U + 2.0 ** -22 + 8 * U * ln
+    logp, H, top = (t.detach().double().cpu() for t in (logp, H, top))
+    assert abs(logp[0] + ln) <= tol and abs(H[0] - ln) <= 2 * tol
+    assert logp[1] == 0 and H[1] == 0 and idx[1, 0] == 3 and idx[1, 1] == 0
+    assert logp[2] == float("-inf") and abs(H[2] - ln) <= 2 * tol
+    assert idx[0].tolist() == [0, 3] and ((top[0] + ln).abs() <= tol).all()
+    want = torch.zeros(V, dtype=torch.float64)
+    want[::3] = -1.0 / n
+    want[0] += 1.0
+    assert_within(gx[0, 0], want, (tol + half_step(dtype)) * want.abs() + tol / n + tiny(dtype), "grad")
+    # entropy's gradient -p (log p + H) is 0 where all are alike: the error of log p + H
+    assert gx[0, 3].abs().max() <= 4 * tol / n and not gx[0, 2].any()
+
+
+@pytest.mark.gpu
 def test_token_logprobs_near_one_keeps_its_digits(ops):
     """p_y = 1 - 1e-7 or so: logp comes from t_y - log2 S, not from the difference
     of two numbers near 20."""
@@ -675,6 +705,7 @@ def test_token_logprobs_layouts_bad_tokens_and_empty_input(ops):
         xl = x.detach().requires_grad_(True)
         logp, H, top, idx, bad = ops.token_logprobs(xl, t, top_k=2)
         (gx,) = torch.autograd.grad(logp.sum() + H.sum() + top.sum(), xl)
+        logp, H = logp.detach(), H.detach()
         assert int(bad) == 1 and float(logp[1, 2]) == 0 and float(H[1, 2]) == 0
         assert (idx[1, 2] == -1).all() and not gx[:, 1, 2].any() and torch.isfinite(gx).all()
         assert torch.equal(logp[0], full[0][0])
@@ -739,8 +770,9 @@ def test_the_operators_together_train_as_the_plain_model(ops):
     y = torch.nn.functional.layer_norm(h, (h.shape[-1],), gamma, beta)
     lp = (y @ out_w.t()).log_softmax(-1)
     H2 = -(lp.exp() * lp).sum(-1)
+    loss = loss.detach()
     loss2 = -lp.gather(-1, tgt[..., None]).mean() - 0.01 * H2.mean() + 0.1 * lp.gather(-1, idx).mean()
-    assert abs(float(loss) - float(loss2)) < 1e-5
+    assert abs(float(loss) - float(loss2.detach())) < 1e-5
     for a, b in zip(grads, torch.autograd.grad(loss2, qs)):
         # K = 96 and 132-row fp32 products (at most 132 u of the terms' size) dominate
         assert (a.double() - b).abs().max() <= 2e-5 * b.abs().max()
