@@ -62,14 +62,18 @@ __device__ __forceinline__ float not_below(float t) {
 // The values seen so far: their maximum, S and A against ref_of(m).
 struct State {
   float m, S, A;
+  Ref f;
+  __device__ __forceinline__ State(float max = -INFINITY, float s = 0.0f, float a = 0.0f)
+      : m(max), S(s), A(a), f(ref_of(max)) {}
   __device__ __forceinline__ void move_to(float nm) {
-    const Ref a = ref_of(m), b = ref_of(nm);
+    const Ref a = f, b = ref_of(nm);
     // never above 0; held so where there is nothing yet (m = -inf, S = A = 0)
     const float d = fminf(fmaxf((a.c - b.c) + (a.off - b.off) * kLog2e, -200.0f), 0.0f);
     const float k = m == -INFINITY ? 0.0f : exp2_approx(d);
     A = k * fmaf(d, S, A);
     S *= k;
     m = nm;
+    f = b;
   }
   __device__ __forceinline__ void join_warp() {
     float nm = m;
@@ -222,38 +226,66 @@ struct Tiles {
       fp += st;
     }
   }
-  // the words of one step of the tile whose first value of this thread is j0; `none` where there is no value
-  __device__ __forceinline__ void take(int j0, int t, uint32_t none, uint32_t (&w)[kWords]) {
+  // the words of one step of the tile whose first value of this thread is j0, in the order of
+  // the stages; `none` where there is no value
+  __device__ __forceinline__ void take(int j0, uint32_t none, uint32_t (&w)[kWords], int t) {
     if constexpr (VEC > 1) {
       asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
-                     : "=r"(w[4 * u]), "=r"(w[4 * u + 1]), "=r"(w[4 * u + 2]), "=r"(w[4 * u + 3])
-                     : "r"(ring + at + u * 256 * 16)
-                     : "memory");
-        if (j0 + u * GT * VEC >= hi) w[4 * u] = w[4 * u + 1] = w[4 * u + 2] = w[4 * u + 3] = none;
-      }
+      from_ring(at, w);
+      blank(j0, none, w);
       fetch();
     } else {
+      from_row(j0, t, none, w);
+    }
+  }
+  __device__ __forceinline__ void from_ring(uint32_t slot, uint32_t (&w)[kWords]) const {
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
+    for (int u = 0; u < U; ++u)
+      asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                   : "=r"(w[4 * u]), "=r"(w[4 * u + 1]), "=r"(w[4 * u + 2]), "=r"(w[4 * u + 3])
+                   : "r"(ring + slot + u * 256 * 16)
+                   : "memory");
+  }
+  __device__ __forceinline__ void blank(int j0, uint32_t none, uint32_t (&w)[kWords]) const {
+    if (j0 + (U - 1) * GT * VEC >= hi)
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (j0 + u * GT * VEC >= hi) w[4 * u] = w[4 * u + 1] = w[4 * u + 2] = w[4 * u + 3] = none;
+  }
+  __device__ __forceinline__ void from_row(int j0, int t, uint32_t none, uint32_t (&w)[kWords]) const {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int j = j0 + u * GT * VEC;
+      if constexpr (VEC > 1) {
+        uint4 v = make_uint4(none, none, none, none);
+        if (j < hi) v = *reinterpret_cast<const uint4*>(row + t * st + j);
+        w[4 * u] = v.x;
+        w[4 * u + 1] = v.y;
+        w[4 * u + 2] = v.z;
+        w[4 * u + 3] = v.w;
+      } else {
         w[u] = none;
-        if (j0 + u * GT < hi) w[u] = one_word<DT>(row + t * st + j0 + u * GT);
+        if (j < hi) w[u] = one_word<DT>(row + t * st + j);
       }
     }
   }
-  // z of a tile of several steps, -inf where there is no value
-  __device__ __forceinline__ void mean(int j0, float inv_t, float2 (&z)[N / 2]) {
+  // z of a tile, -inf where there is no value; get(t, none, w): the words of step t
+  template <typename G>
+  __device__ __forceinline__ void mean(int j0, float inv_t, G get, float2 (&z)[N / 2]) const {
     uint32_t w[kWords];
+    if (T == 1) {
+      get(0, no_value<DT>(), w);
+      unpack_words<DT, VEC>(w, z);
+      return;
+    }
     float2 err[N / 2];
-    take(j0, 0, 0u, w);
+    get(0, 0u, w);
     unpack_words<DT, VEC>(w, z);
 #pragma unroll
     for (int i = 0; i < N / 2; ++i) err[i] = make_float2(0.0f, 0.0f);
     for (int t = 1; t < T; ++t) {
       float2 v[N / 2];
-      take(j0, t, 0u, w);
+      get(t, 0u, w);
       unpack_words<DT, VEC>(w, v);
 #pragma unroll
       for (int i = 0; i < N / 2; ++i) add_exactly(z[i], err[i], v[i]);
@@ -278,9 +310,30 @@ struct Tiles {
         }
       }
     }
+    if (j0 + place(N - 1) >= hi)
 #pragma unroll
-    for (int i = 0; i < N; ++i)
-      if (j0 + place(i) >= hi) (i & 1 ? z[i / 2].y : z[i / 2].x) = -INFINITY;
+      for (int i = 0; i < N; ++i)
+        if (j0 + place(i) >= hi) (i & 1 ? z[i / 2].y : z[i / 2].x) = -INFINITY;
+  }
+  __device__ __forceinline__ void mean(int j0, float inv_t, float2 (&z)[N / 2]) {
+    mean(j0, inv_t, [&](int t, uint32_t none, uint32_t (&w)[kWords]) { take(j0, none, w, t); }, z);
+  }
+  // z of a tile that has been taken already
+  __device__ __forceinline__ void again(int tile, float inv_t, float2 (&z)[N / 2]) const {
+    const int j0 = first(tile);
+    const bool kept = VEC > 1 && tiles() * T <= kStages;  // the whole row is in the ring still
+    mean(j0, inv_t,
+         [&](int t, uint32_t none, uint32_t (&w)[kWords]) {
+           if constexpr (VEC > 1) {
+             if (kept) {
+               from_ring((tile * T + t) * U * 256 * 16, w);
+               blank(j0, none, w);
+               return;
+             }
+           }
+           from_row(j0, t, none, w);
+         },
+         z);
   }
   // value i's place after the thread's first value of the tile
   __device__ static __forceinline__ constexpr int place(int i) { return (i / VEC) * GT * VEC + i % VEC; }
@@ -307,66 +360,107 @@ __device__ __forceinline__ void range_of(int V, int head, int split, int splits,
 
 // ---------------------------------------------------------------- alternatives
 
-// The K best (order bits, ~index) of a warp, falling; lane k holds the k-th, 0 none.
-struct Best {
-  unsigned long long key;
-  int K, lane, full;
-  float floor;  // the K-th value where there are K
-  __device__ __forceinline__ Best(int k, int l) : key(0), K(k), lane(l), full(0), floor(-INFINITY) {}
-  __device__ __forceinline__ unsigned long long last() const { return __shfl_sync(0xffffffffu, key, K - 1); }
-  __device__ __forceinline__ void insert(unsigned long long k) {  // uniform, above last()
-    const int at = __popc(__ballot_sync(0xffffffffu, key > k));
-    const unsigned long long up = __shfl_up_sync(0xffffffffu, key, 1);
-    if (lane > at) key = up;
-    if (lane == at) key = k;
-    if (lane >= K) key = 0;
+// The K best keys (order bits, ~index) of a row, after its one pass: every thread
+// knows the maximum of its values.  The K-th largest of 32 maxima (of a lane, or
+// of 8 threads of a block) is a floor: K values at least lie at or above it, and
+// few more.  Only the threads whose maximum reaches it look at their values again
+// (in the ring, or by then in L2) and put the keys above the floor into shared
+// memory, where the K best are ranked.  More keys than it holds (ties, or rows
+// without 32 numbers, where there is no floor): the K-th of those gathered is the
+// next floor, and the threads look again; every turn leaves out kGather - K keys
+// for good.  The K best do not depend on the order in which the keys came.
+template <int GT>
+struct Gather {
+  static constexpr int kGather = GT == 32 ? 128 : 512;
+  unsigned long long key[kGather], best[kMaxTop];
+  uint32_t group[32];
+  int count;
+  __device__ __forceinline__ static void sync() {
+    if constexpr (GT == 32) __syncwarp();
+    else __syncthreads();
   }
-  __device__ __forceinline__ void settle() {
-    const unsigned long long k = last();
-    full = k != 0;
-    floor = full ? order_value((uint32_t)(k >> 32)) : -INFINITY;
-  }
-  // N values a lane, value i with index index(i), rising in i (< 0: none); `most`: their
-  // largest.  The best of the warp goes into the list, again and again, until none is good enough.
-  template <int N, typename J>
-  __device__ __forceinline__ void offer(const float2 (&z)[N / 2], float most, bool ties, J index) {
-    if (!__any_sync(0xffffffffu, !full || most > floor || (ties && most >= floor))) return;
-    uint32_t ord[N];
+  // order bits of the K-th largest of 32 group maxima; most: the thread's
+  __device__ __forceinline__ uint32_t kth_group(uint32_t most, int K, int tid) {
+    const int lane = tid & 31;
+    if constexpr (GT > 32) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) ord[i] = index(i) >= 0 ? order_bits(i & 1 ? z[i / 2].y : z[i / 2].x) : 0u;
-    const bool fresh = last() == 0 && __shfl_sync(0xffffffffu, key, 0) == 0;
-    for (int n = 0; n < K; ++n) {
-      uint32_t best = 0, j = 0xffffffffu;
-#pragma unroll
-      for (int i = 0; i < N; ++i)
-        if (ord[i] > best) {  // rising indexes: the first of equals
-          best = ord[i];
-          j = (uint32_t)index(i);
-        }
-      const uint32_t top = __reduce_max_sync(0xffffffffu, best);
-      if (top == 0) break;
-      const uint32_t at = __reduce_min_sync(0xffffffffu, best == top ? j : 0xffffffffu);
-      const unsigned long long k = ((unsigned long long)top << 32) | (uint32_t)~at;
-      if (fresh) {  // into an empty list they come in order
-        if (lane == n) key = k;
-      } else {
-        if (k <= last()) break;
-        insert(k);
-      }
-      if (best == top && j == at)
-#pragma unroll
-        for (int i = 0; i < N; ++i)
-          if ((uint32_t)index(i) == at) ord[i] = 0;
+      for (int o = GT / 64; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+      if (tid % (GT / 32) == 0) group[tid / (GT / 32)] = most;
+      sync();
+      most = group[lane];
     }
-    settle();
+#pragma unroll
+    for (int size = 2; size <= 32; size *= 2)  // a bitonic sort, falling
+#pragma unroll
+      for (int step = size / 2; step > 0; step /= 2) {
+        const uint32_t o = __shfl_xor_sync(0xffffffffu, most, step);
+        const bool larger = ((lane & step) == 0) == ((lane & size) == 0 || size == 32);
+        most = larger ? max(most, o) : min(most, o);
+      }
+    return __shfl_sync(0xffffffffu, most, K - 1);
+  }
+  // the K best of the n keys into best[], falling, zeros where there are fewer
+  __device__ __forceinline__ void rank(int n, int K, int tid) {
+    if (tid < kMaxTop) best[tid] = 0;
+    sync();
+    for (int i = tid; i < n; i += GT) {
+      const unsigned long long k = key[i];
+      int above = 0;
+#pragma unroll 4
+      for (int o = 0; o < n; ++o) above += key[o] > k;
+      if (above < K) best[above] = k;
+    }
+    sync();
+  }
+  // offers(put): the thread's values by put(value, index)
+  template <typename F>
+  __device__ __forceinline__ void select(float most, int K, int tid, F offers) {
+    const uint32_t mine = order_bits(most), kth = kth_group(mine, K, tid);
+    // -inf stands for a thread without a number too: no floor
+    unsigned long long floor = kth > 0x007fffffu ? ((unsigned long long)kth << 32) - 1 : 0;
+    for (;;) {
+      if (tid == 0) count = 0;
+      sync();
+      if (floor == 0 || mine >= (uint32_t)(floor >> 32))
+        offers([&](float v, int j) {
+          const uint32_t bits = order_bits(v);
+          const unsigned long long k = ((unsigned long long)bits << 32) | (uint32_t)~j;
+          if (k > floor) {
+            const int at = atomicAdd(&count, 1);
+            if (at < kGather) key[at] = k;
+          }
+        });
+      sync();
+      const int n = count;
+      rank(n < kGather ? n : kGather, K, tid);
+      if (n <= kGather) return;
+      floor = best[K - 1] - 1;
+    }
   }
 };
+
+// The K best of up to 32 falling lists of 64-bit keys in shared memory (lane l
+// walks list l): lane k gets the k-th.
+__device__ __forceinline__ unsigned long long best_of_lists(const unsigned long long* list, int lists, int stride, int K,
+                                                            int lane) {
+  unsigned long long mine = 0;
+  int at = 0;
+  for (int n = 0; n < K; ++n) {
+    const unsigned long long head = lane < lists && at < K ? list[lane * stride + at] : 0ull;
+    const uint32_t hi = __reduce_max_sync(0xffffffffu, (uint32_t)(head >> 32));
+    const uint32_t lo = __reduce_max_sync(0xffffffffu, (uint32_t)(head >> 32) == hi ? (uint32_t)head : 0u);
+    const unsigned long long top = ((unsigned long long)hi << 32) | lo;
+    if (lane == n) mine = top;
+    if (head == top) ++at;
+  }
+  return mine;
+}
 
 // a tile into the thread's state
 template <int P>
 __device__ __forceinline__ void absorb(State& s, float2 (&z)[P], float most) {
   if (most > s.m) s.move_to(most);
-  const Ref f = ref_of(s.m);
+  const Ref f = s.f;
   if (f.off != 0.0f)
 #pragma unroll
     for (int i = 0; i < P; ++i) z[i] = add2(z[i], make_float2(-f.off, -f.off));
@@ -402,7 +496,7 @@ __device__ __forceinline__ float most_of(const uint32_t (&w)[WORDS]) {
 template <int DT, int WORDS>
 __device__ __forceinline__ void absorb_words(State& s, const uint32_t (&w)[WORDS], float most) {
   if (most > s.m) s.move_to(most);
-  const Ref f = ref_of(s.m);
+  const Ref f = s.f;
   if (f.off != 0.0f || s.m < -32768.0f) {
     float2 z[WORDS];
 #pragma unroll
@@ -434,23 +528,6 @@ __device__ __forceinline__ float most_of(const float2 (&z)[P]) {
   return m;
 }
 
-// The K best of up to 32 falling lists of 64-bit keys in shared memory (lane l
-// walks list l): lane k gets the k-th.
-__device__ __forceinline__ unsigned long long best_of_lists(const unsigned long long* list, int lists, int stride, int K,
-                                                            int lane) {
-  unsigned long long mine = 0;
-  int at = 0;
-  for (int n = 0; n < K; ++n) {
-    const unsigned long long head = lane < lists && at < K ? list[lane * stride + at] : 0ull;
-    const uint32_t hi = __reduce_max_sync(0xffffffffu, (uint32_t)(head >> 32));
-    const uint32_t lo = __reduce_max_sync(0xffffffffu, (uint32_t)(head >> 32) == hi ? (uint32_t)head : 0u);
-    const unsigned long long top = ((unsigned long long)hi << 32) | lo;
-    if (lane == n) mine = top;
-    if (head == top) ++at;
-  }
-  return mine;
-}
-
 struct Out {
   float *logp, *entropy, *top_logp;
   int64_t* top_idx;
@@ -461,7 +538,7 @@ struct Out {
 template <int DT>
 __device__ __forceinline__ void write_row(const Logits& x, const typename Elem<DT>::T* row, int64_t r, int64_t y,
                                           State s, unsigned long long key, int K, int lane, const Out& o) {
-  const Ref f = ref_of(s.m);
+  const Ref f = s.f;
   const float l2s = log2f(s.S), H = kLn2 * (l2s - s.A / s.S);
   if (lane == 0) {
     o.logp[r] = kLn2 * (log2_from(mean_over_t<DT>(row + y, x.st, x.T, x.inv_t), f) - l2s);
@@ -491,93 +568,98 @@ constexpr int kWarpRow = 1024;
 
 // GT = 32: a warp a row.  GT = 256: a block a (row, split); with several splits
 // the state and list go to part / keys.
-template <int DT, int VEC, int U, int GT>
-__global__ void __launch_bounds__(256) fwd_kernel(Logits x, const int64_t* __restrict__ tokens, int64_t ignore, int K,
+template <int DT, int VEC, int U, int GT, bool TOP>
+__global__ void __launch_bounds__(256, 4) fwd_kernel(Logits x, const int64_t* __restrict__ tokens, int64_t ignore, int K,
                                                   int splits, Out o, float4* part, unsigned long long* keys, int* bad,
                                                   int scan_bad) {
   using E = typename Elem<DT>::T;
   extern __shared__ uint4 ring[];
-  if (scan_bad && blockIdx.x == gridDim.x - 1) {
+  if (scan_bad && blockIdx.x == 0) {  // the first block, so that it is not the last to end
     scan_tokens(tokens, x.rows, x.V, ignore, bad);
     return;
   }
+  const int64_t block = (int64_t)blockIdx.x - scan_bad;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t unit = GT == 32 ? (int64_t)blockIdx.x * 8 + warp : (int64_t)blockIdx.x;
+  const int64_t unit = GT == 32 ? block * 8 + warp : block;
   const int64_t r = GT == 32 ? unit : unit / splits;
   const int split = GT == 32 ? 0 : (int)(unit - r * splits);
   if (r >= x.rows) return;
   const int64_t y = __ldg(tokens + r);
+  const E* row = reinterpret_cast<const E*>(x.base) + r * x.sr;
+  const int head = head_of<DT, VEC>(row, x.V), tail = (x.V - head) % VEC;
+  int lo, hi;
+  range_of<VEC>(x.V, head, split, splits, lo, hi);
+  const int tid = GT == 32 ? lane : (int)threadIdx.x;
+  Tiles<DT, VEC, U, GT> tl(ring, row, x.st, x.T, lo, hi, tid);  // the first copies go out before the token is here
   if (y == ignore || y < 0 || y >= x.V) {
+    if constexpr (VEC > 1) asm volatile("cp.async.wait_all;" ::: "memory");
     if (split == 0 && (GT == 32 || warp == 0)) {
       write_unused(r, K, lane, o);
       if (!scan_bad && y != ignore && lane == 0) atomicExch(bad, 1);
     }
     return;
   }
-  const E* row = reinterpret_cast<const E*>(x.base) + r * x.sr;
-  const int head = head_of<DT, VEC>(row, x.V), tail = (x.V - head) % VEC;
-  int lo, hi;
-  range_of<VEC>(x.V, head, split, splits, lo, hi);
-  const int tid = GT == 32 ? lane : (int)threadIdx.x;
-  Tiles<DT, VEC, U, GT> tl(ring, row, x.st, x.T, lo, hi, tid);
-  State s{-INFINITY, 0.0f, 0.0f};
-  Best best(K > 0 ? K : 1, lane);
+  State s;
   const int tiles = tl.tiles();
   using TL = Tiles<DT, VEC, U, GT>;
   constexpr int N = TL::N;
   for (int k = 0; k < tiles; ++k) {
     const int j0 = tl.first(k);
-    auto index = [&](int i) {
-      const int j = j0 + TL::place(i);
-      return j < hi ? j : -1;
-    };
-    float2 z[N / 2];
-    if (x.T == 1) {
-      uint32_t w[TL::kWords];
-      tl.take(j0, 0, no_value<DT>(), w);
-      if constexpr (VEC > 1 && DT != SPK_F32) {
-        const float most = most_of<DT>(w);
-        if (K > 0) {
-          unpack_words<DT, VEC>(w, z);
-          best.template offer<N>(z, most, false, index);
-        }
-        absorb_words<DT>(s, w, most);
+    if constexpr (VEC > 1 && DT != SPK_F32)
+      if (x.T == 1) {
+        uint32_t w[TL::kWords];
+        tl.take(j0, no_value<DT>(), w, 0);
+        absorb_words<DT>(s, w, most_of<DT>(w));
         continue;
       }
-      unpack_words<DT, VEC>(w, z);
-    } else {
-      tl.mean(j0, x.inv_t, z);
-    }
-    const float most = most_of(z);
-    if (K > 0) best.template offer<N>(z, most, false, index);
-    absorb(s, z, most);
+    float2 z[N / 2];
+    tl.mean(j0, x.inv_t, z);
+    absorb(s, z, most_of(z));
   }
   if constexpr (VEC > 1) asm volatile("cp.async.wait_all;" ::: "memory");
-  if (VEC > 1 && split == 0 && head + tail > 0) {  // the values beside the vectors
-    const int j = tid < head ? tid : tid >= GT - tail ? x.V - (GT - tid) : -1;
-    float2 z[1] = {make_float2(j >= 0 ? mean_over_t<DT>(row + j, x.st, x.T, x.inv_t) : -INFINITY, -INFINITY)};
-    const float most = z[0].x;
-    if (K > 0) best.template offer<2>(z, most, true, [&](int i) { return i == 0 ? j : -1; });
-    absorb(s, z, most);
+  // the values beside the vectors
+  const int edge = VEC == 1 || split > 0 ? -1 : tid < head ? tid : tid >= GT - tail ? x.V - (GT - tid) : -1;
+  float beside = -INFINITY;
+  if (edge >= 0) {
+    beside = mean_over_t<DT>(row + edge, x.st, x.T, x.inv_t);
+    float2 z[1] = {make_float2(beside, -INFINITY)};
+    absorb(s, z, fmaxf(beside, -INFINITY));
   }
+  __shared__ Gather<GT> mem[TOP ? 256 / GT : 1];
+  Gather<GT>& top = mem[TOP && GT == 32 ? warp : 0];
+  if constexpr (TOP)
+    top.select(s.m, K, tid, [&](auto put) {
+      for (int k = 0; k < tiles; ++k) {
+        float2 z[N / 2];
+        tl.again(k, x.inv_t, z);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          const int j = tl.first(k) + TL::place(i);
+          if (j < hi) put(i & 1 ? z[i / 2].y : z[i / 2].x, j);
+        }
+      }
+      if (edge >= 0) put(beside, edge);
+    });
   s.join_warp();
   if constexpr (GT > 32) {
-    __shared__ State ws[8];
-    __shared__ unsigned long long wk[8][kMaxTop];
-    if (lane == 0) ws[warp] = s;
-    wk[warp][lane] = best.key;
+    __shared__ float ws[8][3];
+    if (lane == 0) {
+      ws[warp][0] = s.m;
+      ws[warp][1] = s.S;
+      ws[warp][2] = s.A;
+    }
     __syncthreads();
     if (warp > 0) return;
-    s = lane < 8 ? ws[lane] : State{-INFINITY, 0.0f, 0.0f};
+    s = lane < 8 ? State(ws[lane][0], ws[lane][1], ws[lane][2]) : State();
     s.join_warp();
-    if (K > 0) best.key = best_of_lists(wk[0], 8, kMaxTop, K, lane);
-    if (splits > 1) {
-      if (lane == 0) part[unit] = make_float4(s.m, s.S, s.A, 0.0f);
-      if (lane < K) keys[unit * K + lane] = best.key;
-      return;
-    }
   }
-  write_row<DT>(x, row, r, y, s, best.key, K, lane, o);
+  const unsigned long long key = TOP && lane < K ? top.best[lane] : 0ull;
+  if (GT > 32 && splits > 1) {
+    if (lane == 0) part[unit] = make_float4(s.m, s.S, s.A, 0.0f);
+    if (lane < K) keys[unit * K + lane] = key;
+    return;
+  }
+  write_row<DT>(x, row, r, y, s, key, K, lane, o);
 }
 
 // a block of one warp a row: the splits' states and lists
@@ -589,10 +671,10 @@ __global__ void __launch_bounds__(32) join_kernel(Logits x, const int64_t* __res
   const int64_t r = blockIdx.x, y = tokens[r];
   pdl_wait();
   if (y == ignore || y < 0 || y >= x.V) return;
-  State s{-INFINITY, 0.0f, 0.0f};
+  State s;
   if (lane < splits) {
     const float4 p = part[r * splits + lane];
-    s = State{p.x, p.y, p.z};
+    s = State(p.x, p.y, p.z);
   }
 #pragma unroll 8
   for (int i = lane; i < splits * K; i += 32) list[i] = keys[r * splits * K + i];
@@ -661,13 +743,7 @@ __global__ void __launch_bounds__(256) bwd_kernel(Logits x, const int64_t* __res
   for (int k = 0; k < tiles; ++k) {
     const int j0 = tl.first(k);
     float2 z[TL::N / 2];
-    if (x.T == 1) {
-      uint32_t w[TL::kWords];
-      tl.take(j0, 0, no_value<DT>(), w);
-      unpack_words<DT, VEC>(w, z);
-    } else {
-      tl.mean(j0, x.inv_t, z);
-    }
+    tl.mean(j0, x.inv_t, z);
     if (f.off != 0.0f)
 #pragma unroll
       for (int i = 0; i < TL::N / 2; ++i) z[i] = add2(z[i], make_float2(-f.off, -f.off));
@@ -742,9 +818,10 @@ int launch_fwd(const Logits& x, const int64_t* tokens, int64_t ignore, int K, in
   const bool scan = x.rows <= kScanTokens;
   if (!scan) cudaMemsetAsync(bad, 0, sizeof(int), st);
   constexpr int smem = Tiles<DT, VEC, U, GT>::kBytes * 256;
-  if (!ask_smem(fwd_kernel<DT, VEC, U, GT>, smem)) return check_launch("token_logprobs_fwd");
-  fwd_kernel<DT, VEC, U, GT><<<(unsigned)(units + (scan ? 1 : 0)), 256, smem, st>>>(x, tokens, ignore, K, splits, o, part,
-                                                                                   keys, bad, scan ? 1 : 0);
+  auto kernel = K > 0 ? fwd_kernel<DT, VEC, U, GT, true> : fwd_kernel<DT, VEC, U, GT, false>;
+  if (!ask_smem(kernel, smem)) return check_launch("token_logprobs_fwd");
+  kernel<<<(unsigned)(units + (scan ? 1 : 0)), 256, smem, st>>>(x, tokens, ignore, K, splits, o, part, keys, bad,
+                                                                scan ? 1 : 0);
   if (splits > 1) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)x.rows);
@@ -766,7 +843,7 @@ int dispatch_fwd(bool wide, const Logits& x, const int64_t* tokens, int64_t igno
 #define GO(VEC, U, GT) launch_fwd<DT, VEC, U, GT>(x, tokens, ignore, K, splits, o, part, keys, bad, st)
   if (warp_rows(x.rows, x.V)) return wide ? GO(kWide, 8 / kWide, 32) : GO(1, 8, 32);
   if (x.V <= 4096) return wide ? GO(kWide, 1, 256) : GO(1, 4, 256);  // shorter tiles: fewer threads without a value
-  return wide ? GO(kWide, 4, 256) : GO(1, 8, 256);
+  return wide ? GO(kWide, 16 / kWide, 256) : GO(1, 8, 256);
 #undef GO
 }
 
