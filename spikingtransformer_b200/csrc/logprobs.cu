@@ -318,22 +318,64 @@ struct Tiles {
   __device__ __forceinline__ void mean(int j0, float inv_t, float2 (&z)[N / 2]) {
     mean(j0, inv_t, [&](int t, uint32_t none, uint32_t (&w)[kWords]) { take(j0, none, w, t); }, z);
   }
-  // z of a tile that has been taken already
-  __device__ __forceinline__ void again(int tile, float inv_t, float2 (&z)[N / 2]) const {
-    const int j0 = first(tile);
-    const bool kept = VEC > 1 && tiles() * T <= kStages;  // the whole row is in the ring still
-    mean(j0, inv_t,
-         [&](int t, uint32_t none, uint32_t (&w)[kWords]) {
-           if constexpr (VEC > 1) {
-             if (kept) {
-               from_ring((tile * T + t) * U * 256 * 16, w);
-               blank(j0, none, w);
-               return;
-             }
-           }
-           from_row(j0, t, none, w);
-         },
-         z);
+  // The thread's values once more, when all have been taken: put(index) of those at or above
+  // `least`, or of all.  kAgain stages are read together; what is put is rare, and read singly.
+  static constexpr int kAgain = GT == 32 ? 1 : kWords >= 16 ? 2 : 4;
+  __device__ static __forceinline__ uint32_t at_least(const float2 (&z)[N / 2], float least, bool all) {
+    uint32_t who = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (all || (i & 1 ? z[i / 2].y : z[i / 2].x) >= least) who |= 1u << i;
+    return who;
+  }
+  template <typename F>
+  __device__ __forceinline__ void again(float inv_t, float least, bool all, F put) const {
+    const int n = tiles();
+    const bool kept = VEC > 1 && n * T <= kStages;  // the whole row is in the ring still
+    auto stage = [&](int tile, int t, uint32_t none, uint32_t (&w)[kWords]) {
+      if (kept) {
+        from_ring((tile * T + t) * U * 256 * 16, w);
+        blank(first(tile), none, w);
+      } else {
+        from_row(first(tile), t, none, w);
+      }
+    };
+    auto wanted = [&](const float2 (&z)[N / 2]) { return at_least(z, least, all); };
+    auto put_all = [&](int tile, uint32_t who) {
+      for (; who; who &= who - 1) {
+        const int j = first(tile) + place(__ffs(who) - 1);
+        if (j < hi) put(j);
+      }
+    };
+    if (T == 1) {
+      for (int k = 0; k < n; k += kAgain) {
+        uint32_t w[kAgain][kWords], who[kAgain], any = 0;
+#pragma unroll
+        for (int q = 0; q < kAgain; ++q)
+          if (k + q < n) stage(k + q, 0, no_value<DT>(), w[q]);
+#pragma unroll
+        for (int q = 0; q < kAgain; ++q) {
+          float2 z[N / 2];
+          unpack_words<DT, VEC>(w[q], z);
+          who[q] = k + q < n ? wanted(z) : 0;
+          any |= who[q];
+        }
+        if (any)
+#pragma unroll 1
+          for (int q = 0; q < kAgain; ++q) {
+            uint32_t mine = who[0];
+#pragma unroll
+            for (int i = 1; i < kAgain; ++i) mine = q == i ? who[i] : mine;
+            put_all(k + q, mine);
+          }
+      }
+      return;
+    }
+    for (int k = 0; k < n; ++k) {
+      float2 z[N / 2];
+      mean(first(k), inv_t, [&](int t, uint32_t none, uint32_t (&v)[kWords]) { stage(k, t, none, v); }, z);
+      put_all(k, wanted(z));
+    }
   }
   // value i's place after the thread's first value of the tile
   __device__ static __forceinline__ constexpr int place(int i) { return (i / VEC) * GT * VEC + i % VEC; }
@@ -412,7 +454,7 @@ struct Gather {
     }
     sync();
   }
-  // offers(put): the thread's values by put(value, index)
+  // offers(least, all, put): put(value, index) of the thread's values at or above least, or of all
   template <typename F>
   __device__ __forceinline__ void select(float most, int K, int tid, F offers) {
     const uint32_t mine = order_bits(most), kth = kth_group(mine, K, tid);
@@ -422,7 +464,7 @@ struct Gather {
       if (tid == 0) count = 0;
       sync();
       if (floor == 0 || mine >= (uint32_t)(floor >> 32))
-        offers([&](float v, int j) {
+        offers(order_value((uint32_t)((floor + 1) >> 32)), floor == 0, [&](float v, int j) {
           const uint32_t bits = order_bits(v);
           const unsigned long long k = ((unsigned long long)bits << 32) | (uint32_t)~j;
           if (k > floor) {
@@ -456,16 +498,26 @@ __device__ __forceinline__ unsigned long long best_of_lists(const unsigned long 
   return mine;
 }
 
+template <int P>
+__device__ __forceinline__ void add_terms(State& s, const float2 (&z)[P], float c);
 // a tile into the thread's state
 template <int P>
-__device__ __forceinline__ void absorb(State& s, float2 (&z)[P], float most) {
+__device__ __forceinline__ void absorb(State& s, const float2 (&z)[P], float most) {
   if (most > s.m) s.move_to(most);
   const Ref f = s.f;
-  if (f.off != 0.0f)
+  if (f.off != 0.0f) {
+    float2 d[P];
 #pragma unroll
-    for (int i = 0; i < P; ++i) z[i] = add2(z[i], make_float2(-f.off, -f.off));
+    for (int i = 0; i < P; ++i) d[i] = add2(z[i], make_float2(-f.off, -f.off));
+    add_terms(s, d, 0.0f);
+  } else {
+    add_terms(s, z, f.c);
+  }
+}
+template <int P>
+__device__ __forceinline__ void add_terms(State& s, const float2 (&z)[P], float c) {
   float2 S2 = make_float2(0.0f, 0.0f), A2 = S2;
-  const float2 l2 = make_float2(kLog2e, kLog2e), c2 = make_float2(-f.c, -f.c);
+  const float2 l2 = make_float2(kLog2e, kLog2e), c2 = make_float2(-c, -c);
 #pragma unroll
   for (int i = 0; i < P; ++i) {
     float2 t = fma2(z[i], l2, c2);
@@ -569,7 +621,7 @@ constexpr int kWarpRow = 1024;
 // GT = 32: a warp a row.  GT = 256: a block a (row, split); with several splits
 // the state and list go to part / keys.
 template <int DT, int VEC, int U, int GT, bool TOP>
-__global__ void __launch_bounds__(256, 4) fwd_kernel(Logits x, const int64_t* __restrict__ tokens, int64_t ignore, int K,
+__global__ void __launch_bounds__(256, TOP ? 3 : 4) fwd_kernel(Logits x, const int64_t* __restrict__ tokens, int64_t ignore, int K,
                                                   int splits, Out o, float4* part, unsigned long long* keys, int* bad,
                                                   int scan_bad) {
   using E = typename Elem<DT>::T;
@@ -603,16 +655,17 @@ __global__ void __launch_bounds__(256, 4) fwd_kernel(Logits x, const int64_t* __
   const int tiles = tl.tiles();
   using TL = Tiles<DT, VEC, U, GT>;
   constexpr int N = TL::N;
+  float2 z[N / 2];
   for (int k = 0; k < tiles; ++k) {
     const int j0 = tl.first(k);
     if constexpr (VEC > 1 && DT != SPK_F32)
       if (x.T == 1) {
         uint32_t w[TL::kWords];
         tl.take(j0, no_value<DT>(), w, 0);
+        if constexpr (TOP && GT == 32) unpack_words<DT, VEC>(w, z);
         absorb_words<DT>(s, w, most_of<DT>(w));
         continue;
       }
-    float2 z[N / 2];
     tl.mean(j0, x.inv_t, z);
     absorb(s, z, most_of(z));
   }
@@ -628,15 +681,17 @@ __global__ void __launch_bounds__(256, 4) fwd_kernel(Logits x, const int64_t* __
   __shared__ Gather<GT> mem[TOP ? 256 / GT : 1];
   Gather<GT>& top = mem[TOP && GT == 32 ? warp : 0];
   if constexpr (TOP)
-    top.select(s.m, K, tid, [&](auto put) {
-      for (int k = 0; k < tiles; ++k) {
-        float2 z[N / 2];
-        tl.again(k, x.inv_t, z);
+    top.select(s.m, K, tid, [&](float least, bool all, auto put) {
+      if (GT == 32 && tiles == 1) {  // a short row's values are here still
+        for (uint32_t who = TL::at_least(z, least, all); who; who &= who - 1) {
+          const int at = __ffs(who) - 1, j = tl.first(0) + TL::place(at);
+          float v = z[0].x;
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-          const int j = tl.first(k) + TL::place(i);
-          if (j < hi) put(i & 1 ? z[i / 2].y : z[i / 2].x, j);
+          for (int i = 1; i < N; ++i) v = at == i ? (i & 1 ? z[i / 2].y : z[i / 2].x) : v;
+          if (j < hi) put(v, j);
         }
+      } else {
+        tl.again(x.inv_t, least, all, [&](int j) { put(mean_over_t<DT>(row + j, x.st, x.T, x.inv_t), j); });
       }
       if (edge >= 0) put(beside, edge);
     });
