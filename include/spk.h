@@ -510,16 +510,23 @@ int spk_layer_norm_bwd(const void* g, int g_dtype, const void* x, int x_dtype, i
  * of its weight.  out[i] = scale * weight[tokens[i]], [n][D] of out_dtype;
  * weight: [V][D] of w_dtype with row stride ldw.  A token outside [0, V) reads
  * as zeros and sets *bad_token (which the call clears first).
+ * With `plan` (spk_embedding_plan_bytes(n) bytes, 16-byte aligned) the call also
+ * sorts the positions by token into it, for the backward, beside the lookup;
+ * NULL where no gradient will be wanted.
  * Backward: gw [V][D] dense of w_dtype = scale * the sum of g's rows over each
  * token's positions in ascending order (fp32), zeros for rows without a token
- * and for row padding_idx (-1: none); tokens outside [0, V) are skipped.
+ * and for row padding_idx (-1: none); tokens outside [0, V) are skipped.  With
+ * tokens NULL the plan is the forward's (same n, V, padding_idx); else the call
+ * sorts the tokens into it first.
  */
+int64_t spk_embedding_plan_bytes(int64_t n);
 int spk_embedding_fwd(const int64_t* tokens, const void* weight, int w_dtype, int64_t ldw, float scale, int64_t n,
-                      int64_t V, int64_t D, void* out, int out_dtype, int* bad_token, void* stream);
+                      int64_t V, int64_t D, void* out, int out_dtype, int* bad_token, int64_t padding_idx, void* plan,
+                      int64_t plan_bytes, void* stream);
 int64_t spk_embedding_bwd_workspace_bytes(int64_t n, int64_t V, int64_t D);
 int spk_embedding_bwd(const int64_t* tokens, const void* g, int g_dtype, float scale, int64_t padding_idx, int64_t n,
-                      int64_t V, int64_t D, void* gw, int w_dtype, void* workspace, int64_t workspace_bytes,
-                      void* stream);
+                      int64_t V, int64_t D, void* gw, int w_dtype, void* plan, int64_t plan_bytes, void* workspace,
+                      int64_t workspace_bytes, void* stream);
 
 /*
  * Log probabilities of given tokens under the mean over T of the logits, with
@@ -527,7 +534,7 @@ int spk_embedding_bwd(const int64_t* tokens, const void* g, int g_dtype, float s
  * lower index, NaN smallest).  logits: element (t, r, v) of dtype
  * (F32/F16/BF16) at t*step_stride + r*row_stride + v; tokens: [rows];
  * logp, entropy: [rows]; top_logp, top_idx: [rows][top_k] (NULL with top_k 0);
- * stats: [rows][4] for the backward, 16-byte aligned.  Rows whose token is ignore_index give
+ * stats: [rows][4] for the backward, 16-byte aligned (NULL: none).  Rows whose token is ignore_index give
  * zeros and top_idx -1; so do tokens outside [0, V), which set *bad_token
  * (cleared first).
  * Backward: grad [T][rows][V] dense of dtype from g_logp [rows], g_entropy

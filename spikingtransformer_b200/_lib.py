@@ -69,9 +69,10 @@ SIGNATURES = {
     "spk_layer_norm_fwd": ([_p, _i, _i64, _p, _i, _p, _i, _f, _i64, _i64, _p, _i, _p, _p], _i),
     "spk_layer_norm_bwd_workspace_bytes": ([_i64, _i64], _i64),
     "spk_layer_norm_bwd": ([_p, _i, _p, _i, _i64, _p, _p, _i, _i64, _i64, _p, _p, _p, _i, _p, _i64, _p], _i),
-    "spk_embedding_fwd": ([_p, _p, _i, _i64, _f, _i64, _i64, _i64, _p, _i, _p, _p], _i),
+    "spk_embedding_plan_bytes": ([_i64], _i64),
+    "spk_embedding_fwd": ([_p, _p, _i, _i64, _f, _i64, _i64, _i64, _p, _i, _p, _i64, _p, _i64, _p], _i),
     "spk_embedding_bwd_workspace_bytes": ([_i64, _i64, _i64], _i64),
-    "spk_embedding_bwd": ([_p, _p, _i, _f, _i64, _i64, _i64, _i64, _p, _i, _p, _i64, _p], _i),
+    "spk_embedding_bwd": ([_p, _p, _i, _f, _i64, _i64, _i64, _i64, _p, _i, _p, _i64, _p, _i64, _p], _i),
     "spk_token_logprobs_workspace_bytes": ([_i64, _i64, _i64, _i64], _i64),
     "spk_token_logprobs_fwd": ([_p, _i, _i64, _i64, _i64, _i64, _i64, _p, _i64, _i64, _p, _p, _p, _p, _p, _p, _p, _i64,
                                 _p], _i),
@@ -191,10 +192,29 @@ def call(name, *args, tag=None, work=None):
         e1.record()
         rec.records.append((tag or name, e0, e1, work or {}))
     if rc != 0:
-        msg = lib.spk_last_error().decode(errors="replace")
-        status = lib.spk_status_string(rc).decode()
-        raise RuntimeError("%s failed (%s): %s" % (name, status, msg))
+        _raise(name, rc)
     return rc
+
+
+def _raise(name, rc):
+    lib = load()
+    msg = lib.spk_last_error().decode(errors="replace")
+    status = lib.spk_status_string(rc).decode()
+    raise RuntimeError("%s failed (%s): %s" % (name, status, msg))
+
+
+def launch(device, name, tag, nbytes, *args):
+    """``call`` of an entry point whose last argument is the stream, on ``device`` (made
+    current for the call where it is not) and its current stream.  Kept short:
+    the smallest calls are bound by the host."""
+    index = device.index
+    if _counter is None and _recorder is None and torch.cuda.current_device() == index:
+        rc = getattr(_lib or load(), name)(*args, torch._C._cuda_getCurrentRawStream(index))
+        if rc != 0:
+            _raise(name, rc)
+        return
+    with torch.cuda.device(device):
+        call(name, *args, torch.cuda.current_stream(device).cuda_stream, tag=tag, work=dict(bytes=nbytes))
 
 
 def stream_ptr(device=None):

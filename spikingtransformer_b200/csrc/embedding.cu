@@ -6,14 +6,16 @@
 // Tokens outside [0, V) read as a row of zeros, take no gradient and raise the
 // caller's flag.
 //
-// The gradient runs in three launches, without atomics, so equal inputs give
-// equal bits:
-//   sort    one cluster of blocks sorts the positions by token (stable, radix);
-//           the other blocks of the launch meanwhile fill g_W with zeros.
+// The gradient needs the positions sorted by token (stable, radix).  One cluster
+// of blocks does that; a forward whose gradient will be wanted launches it just
+// before the gather, which runs beside it, so that the sort costs little.  The
+// gradient itself is two launches, without atomics, so equal inputs give equal
+// bits:
 //   sum     a warp adds the rows of g of one chunk of the sorted positions, a
 //           tile of columns at a time.  A token whose positions all lie in the
 //           chunk is written out; a token that reaches over the chunk's ends
-//           leaves its part in a workspace.
+//           leaves its part in a workspace.  Further blocks write zeros to the
+//           rows of tokens that do not occur.
 //   join    adds the parts of the tokens that reach over chunks, in order.
 // A chunk costs the same whatever its tokens are, so a token that fills half the
 // batch (padding, a space) is spread over the machine like any other.
@@ -33,9 +35,21 @@ template <int WDT, int ODT, int VEC>
 __global__ void __launch_bounds__(256) gather_kernel(const int64_t* __restrict__ tokens,
                                                      const typename Elem<WDT>::T* __restrict__ w, int64_t ldw,
                                                      float scale, int64_t n, int64_t V, int D, int tiles,
-                                                     typename Elem<ODT>::T* __restrict__ out, int* bad) {
+                                                     typename Elem<ODT>::T* __restrict__ out, int* bad, int scan_bad,
+                                                     int after_sort) {
+  // the sort before this kernel may still be running; whoever comes next finds it done
+  struct AtEnd {
+    int on;
+    __device__ ~AtEnd() {
+      if (on) pdl_wait();
+    }
+  } at_end{after_sort};
+  if (scan_bad && blockIdx.x == 0) {  // the first block, so that it is not the last to end
+    scan_tokens(tokens, n, V, 0, bad);
+    return;
+  }
   const int lane = threadIdx.x & 31;
-  const int64_t item = blockIdx.x * (int64_t)8 + (threadIdx.x >> 5);
+  const int64_t item = ((int64_t)blockIdx.x - scan_bad) * 8 + (threadIdx.x >> 5);
   const int64_t group = item / tiles;
   const int col = (int)(item - group * tiles) * 32 * VEC + lane * VEC;
   const int64_t i0 = group * kDeep;
@@ -45,7 +59,7 @@ __global__ void __launch_bounds__(256) gather_kernel(const int64_t* __restrict__
     tok = __ldg(tokens + i0 + lane);
     if (tok < 0 || tok >= V) {
       tok = -1;
-      atomicExch(bad, 1);
+      if (!scan_bad) atomicExch(bad, 1);
     }
   }
   typename Vec<WDT, VEC>::W x[kDeep];
@@ -102,30 +116,18 @@ __device__ __forceinline__ uint32_t same_digit(uint32_t d, int bits, bool in) {
   return same;
 }
 
-// Cluster 0 sorts, the others clear gw.  A pass of the radix sort over a digit
-// of `bits` bits: every warp owns a run of consecutive positions and counts its
-// digits; the counts are summed over the
-// warps of a block, over the blocks of the cluster and over the digits, which
-// gives every (warp, digit) its place; the warp then writes its items there in
-// order.  Positions without a gradient get the key V and end up last.
-__global__ void __launch_bounds__(kSortThreads) sort_clear_kernel(const int64_t* tokens, int64_t n, int64_t V,
-                                                                  int64_t padding_idx, int bits, int passes,
-                                                                  uint2* item0, uint2* item1, void* gw,
-                                                                  int64_t gw_bytes) {
+// One cluster.  A pass of the radix sort over a digit of `bits` bits: every warp
+// owns a run of consecutive positions and counts its digits; the counts are
+// summed over the warps of a block, over the blocks of the cluster and over the
+// digits, which gives every (warp, digit) its place; the warp then writes its
+// items there in order.  Positions without a gradient get the key V and end up
+// last.  131072 tokens of 17 bits: 43 us, much of it the scattered writes.
+__global__ void __launch_bounds__(kSortThreads) sort_kernel(const int64_t* tokens, int64_t n, int64_t V,
+                                                            int64_t padding_idx, int bits, int passes, uint2* item0,
+                                                            uint2* item1) {
   extern __shared__ uint32_t sm[];
-  const uint32_t ncta = cluster_size(), rank = cluster_ctarank(), cl = cluster_id_x();
-  if (cl > 0) {
-    const int64_t stride = (int64_t)(cluster_count_x() - 1) * ncta * kSortThreads;
-    const int64_t me = ((int64_t)(cl - 1) * ncta + rank) * kSortThreads + threadIdx.x;
-    if ((reinterpret_cast<uintptr_t>(gw) & 15) == 0) {
-      const int64_t n16 = gw_bytes / 16;
-      for (int64_t i = me; i < n16; i += stride) reinterpret_cast<uint4*>(gw)[i] = make_uint4(0, 0, 0, 0);
-      for (int64_t i = n16 * 8 + me; i < gw_bytes / 2; i += stride) reinterpret_cast<uint16_t*>(gw)[i] = 0;
-    } else {
-      for (int64_t i = me; i < gw_bytes / 2; i += stride) reinterpret_cast<uint16_t*>(gw)[i] = 0;
-    }
-    return;
-  }
+  pdl_trigger();
+  const uint32_t ncta = cluster_size(), rank = cluster_ctarank();
   const int bins = 1 << bits;
   uint32_t* count = sm;                         // [warps][bins]
   uint32_t* total = sm + kSortWarps * bins;     // [bins], read by the cluster's other blocks
@@ -230,6 +232,27 @@ __device__ __forceinline__ void copy_async(uint32_t dst, const void* src, int by
   else asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
 }
 
+// zeros to those of 32 rows whose token does not occur (a search of the sorted keys a lane)
+template <int WDT, int VEC>
+__device__ __forceinline__ void clear_rows(const uint2* __restrict__ items, int64_t n, uint32_t V, int D, int64_t group,
+                                           int lane, typename Elem<WDT>::T* __restrict__ gw) {
+  const int64_t row = group * 32 + lane;
+  int64_t a = 0, b = n;  // the first item with a key of at least `row`
+  while (a < b) {
+    const int64_t mid = (a + b) / 2;
+    if (items[mid].x < row) a = mid + 1;
+    else b = mid;
+  }
+  uint32_t absent = __ballot_sync(0xffffffffu, row < V && (a >= n || items[a].x != row));
+  float zero[VEC];
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) zero[i] = 0.0f;
+  for (; absent; absent &= absent - 1) {
+    typename Elem<WDT>::T* to = gw + (group * 32 + __ffs(absent) - 1) * D;
+    for (int c = lane * VEC; c < D; c += 32 * VEC) Vec<WDT, VEC>::store(to + c, zero);
+  }
+}
+
 // A warp per (chunk of sorted positions, tile of 32 * VEC columns).  With
 // VEC > 1 a lane's vectors of the next kRing rows are on their way into a
 // ring of its own in shared memory (a lane reads back only what it copied
@@ -242,10 +265,16 @@ template <int GDT, int WDT, int VEC>
 __global__ void __launch_bounds__(256) sum_kernel(const uint2* __restrict__ items,
                                                   const typename Elem<GDT>::T* __restrict__ g, float scale, int64_t n,
                                                   uint32_t V, int D, int chunk, int tiles, int64_t chunks,
-                                                  typename Elem<WDT>::T* __restrict__ gw, float* __restrict__ part) {
+                                                  int64_t sum_blocks, typename Elem<WDT>::T* __restrict__ gw,
+                                                  float* __restrict__ part) {
   using W = typename Vec<GDT, VEC>::W;
   extern __shared__ uint4 ring_mem[];
+  pdl_trigger();
   const int lane = threadIdx.x & 31;
+  if (blockIdx.x >= sum_blocks) {
+    clear_rows<WDT, VEC>(items, n, V, D, ((int64_t)blockIdx.x - sum_blocks) * 8 + (threadIdx.x >> 5), lane, gw);
+    return;
+  }
   const int64_t item = blockIdx.x * (int64_t)8 + (threadIdx.x >> 5);
   if (item >= chunks * tiles) return;
   const int64_t c = item / tiles;
@@ -362,6 +391,7 @@ __global__ void __launch_bounds__(256) join_kernel(const uint2* __restrict__ ite
                                                    typename Elem<WDT>::T* __restrict__ gw,
                                                    const float* __restrict__ part) {
   __shared__ float red[8][32 * VEC];
+  pdl_wait();
   const int64_t c = blockIdx.x;
   const int64_t lo = c * chunk, hi = lo + chunk;
   const uint32_t k = items[hi - 1].x;
@@ -428,7 +458,7 @@ inline int64_t align16(int64_t b) { return (b + 15) / 16 * 16; }
 // positions enough, of 16 to 1024 positions.
 struct Plan {
   int bits, passes, chunk, tiles;
-  int64_t chunks, items;  // items: bytes of one array of (key, position)
+  int64_t chunks, items;  // items: bytes of one of the two arrays of (key, position)
   Plan(int64_t n, int64_t V, int64_t D, int vec) {
     int b = 1;
     while ((V >> b) != 0) ++b;  // keys 0 .. V
@@ -454,14 +484,21 @@ int launch_bwd(const Plan& pl, const uint2* items, const void* g, float scale, i
                                                smem);
     if (e != cudaSuccess) return fail(SPK_ERR_LAUNCH, "embedding_bwd: %s", cudaGetErrorString(e));
   }
-  sum_kernel<GDT, WDT, VEC><<<(unsigned)blocks, 256, smem, st>>>(items, reinterpret_cast<const typename Elem<GDT>::T*>(g),
-                                                                scale, n, (uint32_t)V, D, pl.chunk, pl.tiles, pl.chunks,
-                                                                out, part);
+  const int64_t clear = (V + 255) / 256;  // 32 rows a warp
+  sum_kernel<GDT, WDT, VEC><<<(unsigned)(blocks + clear), 256, smem, st>>>(
+      items, reinterpret_cast<const typename Elem<GDT>::T*>(g), scale, n, (uint32_t)V, D, pl.chunk, pl.tiles, pl.chunks,
+      blocks, out, part);
   if (pl.chunks > 1) {
+    cudaLaunchConfig_t cfg = {};
     // a few blocks a chunk: a token of many parts has its columns spread over them
-    const dim3 grid((unsigned)(pl.chunks - 1), D >= 512 ? 4 : 1);
-    join_kernel<WDT, VEC == 1 ? 1 : 4><<<grid, 256, 0, st>>>(items, scale, n, (uint32_t)V, D, pl.chunk, pl.chunks, out,
-                                                             part);
+    cfg.gridDim = dim3((unsigned)(pl.chunks - 1), D >= 512 ? 4 : 1);
+    cfg.blockDim = dim3(256);
+    cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    add_pdl_attr(cfg, at);
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, join_kernel<WDT, VEC == 1 ? 1 : 4>, items, scale, n, (uint32_t)V, D,
+                                             pl.chunk, pl.chunks, out, (const float*)part);
+    if (e != cudaSuccess) return fail(SPK_ERR_LAUNCH, "embedding_bwd: %s", cudaGetErrorString(e));
   }
   return check_launch("embedding_bwd");
 }
@@ -472,19 +509,53 @@ inline int bwd_vec(const void* g, int g_dtype, const void* gw, int w_dtype, int6
   return D % v == 0 && aligned(g, v * dtype_size(g_dtype)) && aligned(gw, v * dtype_size(w_dtype)) ? v : 1;
 }
 
+// The items in order: in plan, or in plan + its second half.
+int launch_sort(const Plan& pl, const int64_t* tokens, int64_t n, int64_t V, int64_t padding_idx, void* plan,
+                cudaStream_t st) {
+  uint2* item0 = reinterpret_cast<uint2*>(plan);
+  uint2* item1 = reinterpret_cast<uint2*>(reinterpret_cast<char*>(plan) + pl.items);
+  const int csize = n <= 4096 ? 1 : n <= 32768 ? 8 : 16;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)csize);
+  cfg.blockDim = dim3(kSortThreads);
+  cfg.dynamicSmemBytes = (size_t)((kSortWarps + 2) << pl.bits) * 4;
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim = {(unsigned)csize, 1, 1};
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  cudaError_t e = cudaSuccess;
+  if (cfg.dynamicSmemBytes > (40u << 10))
+    e = cudaFuncSetAttribute(sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)cfg.dynamicSmemBytes);
+  if (e == cudaSuccess && csize > 8) e = cudaFuncSetAttribute(sort_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  if (e == cudaSuccess)
+    e = cudaLaunchKernelEx(&cfg, sort_kernel, tokens, n, V, padding_idx, pl.bits, pl.passes, item0, item1);
+  return e == cudaSuccess ? SPK_OK : fail(SPK_ERR_LAUNCH, "embedding sort: %s", cudaGetErrorString(e));
+}
+inline const uint2* sorted_items(const Plan& pl, const void* plan) {
+  return reinterpret_cast<const uint2*>(reinterpret_cast<const char*>(plan) + (pl.passes & 1 ? 0 : pl.items));
+}
+
 template <int WDT, int ODT>
-void launch_gather(const int64_t* tokens, const void* w, int64_t ldw, float scale, int64_t n, int64_t V, int D,
-                   void* out, int* bad, cudaStream_t st) {
+int launch_gather(const int64_t* tokens, const void* w, int64_t ldw, float scale, int64_t n, int64_t V, int D,
+                  void* out, int* bad, bool after_sort, cudaStream_t st) {
   constexpr int kWide = WDT == SPK_F32 || ODT == SPK_F32 ? 4 : 8;
   const bool wide = D % kWide == 0 && ldw % kWide == 0 && aligned(w, kWide * dtype_size(WDT)) &&
                     aligned(out, kWide * dtype_size(ODT));
   const int tiles = (D + 32 * (wide ? kWide : 1) - 1) / (32 * (wide ? kWide : 1));
-  const int64_t grid = ((n + kDeep - 1) / kDeep * tiles + 7) / 8;
-  auto* wp = reinterpret_cast<const typename Elem<WDT>::T*>(w);
-  auto* op = reinterpret_cast<typename Elem<ODT>::T*>(out);
-  if (wide)
-    gather_kernel<WDT, ODT, kWide><<<(unsigned)grid, 256, 0, st>>>(tokens, wp, ldw, scale, n, V, D, tiles, op, bad);
-  else gather_kernel<WDT, ODT, 1><<<(unsigned)grid, 256, 0, st>>>(tokens, wp, ldw, scale, n, V, D, tiles, op, bad);
+  const int scan = n <= kScanTokens ? 1 : 0;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(((n + kDeep - 1) / kDeep * tiles + 7) / 8 + scan));
+  cfg.blockDim = dim3(256);
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  if (after_sort) add_pdl_attr(cfg, at);  // beside the sort, whose results it does not read
+  const cudaError_t e = cudaLaunchKernelEx(
+      &cfg, wide ? gather_kernel<WDT, ODT, kWide> : gather_kernel<WDT, ODT, 1>, tokens,
+      reinterpret_cast<const typename Elem<WDT>::T*>(w), ldw, scale, n, V, D, tiles,
+      reinterpret_cast<typename Elem<ODT>::T*>(out), bad, scan, after_sort ? 1 : 0);
+  return e == cudaSuccess ? check_launch("embedding_fwd") : fail(SPK_ERR_LAUNCH, "embedding_fwd: %s", cudaGetErrorString(e));
 }
 
 #define SPK_EMB_TYPES(A, B, CALL)                                                  \
@@ -505,8 +576,11 @@ void launch_gather(const int64_t* tokens, const void* w, int64_t ldw, float scal
 
 extern "C" {
 
+int64_t spk_embedding_plan_bytes(int64_t n) { return n < 1 ? 16 : 2 * spk::embg::align16(8 * n); }
+
 int spk_embedding_fwd(const int64_t* tokens, const void* weight, int w_dtype, int64_t ldw, float scale, int64_t n,
-                      int64_t V, int64_t D, void* out, int out_dtype, int* bad_token, void* stream) {
+                      int64_t V, int64_t D, void* out, int out_dtype, int* bad_token, int64_t padding_idx, void* plan,
+                      int64_t plan_bytes, void* stream) {
   using namespace spk;
   using namespace spk::embg;
   SPK_REQUIRE(tokens && weight && out && bad_token, SPK_ERR_INVALID, "null pointer argument");
@@ -514,68 +588,54 @@ int spk_embedding_fwd(const int64_t* tokens, const void* weight, int w_dtype, in
   SPK_REQUIRE(n >= 1 && V >= 1 && D >= 1 && D <= (1 << 20) && ldw >= D && n < (1ll << 31) && V < (1ll << 31),
               SPK_ERR_SHAPE, "unsupported sizes n=%lld V=%lld D=%lld row stride %lld", (long long)n, (long long)V,
               (long long)D, (long long)ldw);
+  SPK_REQUIRE(!plan || plan_bytes >= spk_embedding_plan_bytes(n), SPK_ERR_INVALID,
+              "plan smaller than spk_embedding_plan_bytes()");
+  SPK_REQUIRE(aligned(plan, 16), SPK_ERR_ALIGN, "plan must be 16-byte aligned");
   int rc = check_stream_device(stream);
   if (rc != SPK_OK) return rc;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  cudaMemsetAsync(bad_token, 0, sizeof(int), st);
-#define CALL(W, O) launch_gather<W, O>(tokens, weight, ldw, scale, n, V, (int)D, out, bad_token, st)
+  if (n > kScanTokens) cudaMemsetAsync(bad_token, 0, sizeof(int), st);
+  if (plan) {
+    rc = launch_sort(Plan(n, V, D, 8), tokens, n, V, padding_idx, plan, st);
+    if (rc != SPK_OK) return rc;
+  }
+#define CALL(W, O) return launch_gather<W, O>(tokens, weight, ldw, scale, n, V, (int)D, out, bad_token, plan != nullptr, st)
   SPK_EMB_TYPES(w_dtype, out_dtype, CALL);
 #undef CALL
-  return check_launch("embedding_fwd");
 }
 
 int64_t spk_embedding_bwd_workspace_bytes(int64_t n, int64_t V, int64_t D) {
   using namespace spk::embg;
   if (n < 1 || V < 1 || D < 1) return 16;
   const Plan pl(n, V, D, 8);  // the widest tiles make the most chunks
-  return 2 * pl.items + pl.chunks * 2 * D * (int64_t)sizeof(float);
+  return pl.chunks * 2 * D * (int64_t)sizeof(float);
 }
 
 int spk_embedding_bwd(const int64_t* tokens, const void* g, int g_dtype, float scale, int64_t padding_idx, int64_t n,
-                      int64_t V, int64_t D, void* gw, int w_dtype, void* workspace, int64_t workspace_bytes,
-                      void* stream) {
+                      int64_t V, int64_t D, void* gw, int w_dtype, void* plan, int64_t plan_bytes, void* workspace,
+                      int64_t workspace_bytes, void* stream) {
   using namespace spk;
   using namespace spk::embg;
-  SPK_REQUIRE(tokens && g && gw, SPK_ERR_INVALID, "null pointer argument");
+  SPK_REQUIRE(g && gw && plan, SPK_ERR_INVALID, "null pointer argument");
   SPK_REQUIRE(float_type(w_dtype) && float_type(g_dtype), SPK_ERR_INVALID, "embedding takes fp32, fp16 and bf16");
   SPK_REQUIRE(n >= 1 && V >= 1 && D >= 1 && D <= (1 << 20) && n < (1ll << 31) && V < (1ll << 31), SPK_ERR_SHAPE,
               "unsupported sizes n=%lld V=%lld D=%lld", (long long)n, (long long)V, (long long)D);
+  SPK_REQUIRE(plan_bytes >= spk_embedding_plan_bytes(n), SPK_ERR_INVALID,
+              "plan smaller than spk_embedding_plan_bytes()");
   SPK_REQUIRE(workspace && workspace_bytes >= spk_embedding_bwd_workspace_bytes(n, V, D), SPK_ERR_INVALID,
               "workspace smaller than spk_embedding_bwd_workspace_bytes()");
-  SPK_REQUIRE(aligned(workspace, 16), SPK_ERR_ALIGN, "workspace must be 16-byte aligned");
+  SPK_REQUIRE(aligned(workspace, 16) && aligned(plan, 16), SPK_ERR_ALIGN, "plan and workspace must be 16-byte aligned");
   int rc = check_stream_device(stream);
   if (rc != SPK_OK) return rc;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const int vec = bwd_vec(g, g_dtype, gw, w_dtype, D);
   const Plan pl(n, V, D, vec);
-  char* ws = reinterpret_cast<char*>(workspace);
-  uint2* item0 = reinterpret_cast<uint2*>(ws);
-  uint2* item1 = reinterpret_cast<uint2*>(ws + pl.items);
-  float* part = reinterpret_cast<float*>(ws + 2 * pl.items);
-  const int64_t gw_bytes = V * D * dtype_size(w_dtype);
-
-  const int csize = n <= 4096 ? 1 : n <= 32768 ? 8 : 16;
-  int64_t fill = (gw_bytes + (int64_t)csize * (64 << 10) - 1) / ((int64_t)csize * (64 << 10));
-  const int64_t most = num_sms() / csize;
-  if (fill > most) fill = most;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)((1 + fill) * csize));
-  cfg.blockDim = dim3(kSortThreads);
-  cfg.dynamicSmemBytes = (size_t)((kSortWarps + 2) << pl.bits) * 4;
-  cfg.stream = st;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim = {(unsigned)csize, 1, 1};
-  cfg.attrs = at;
-  cfg.numAttrs = 1;
-  cudaError_t e = cudaFuncSetAttribute(sort_clear_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       (int)((kSortWarps + 2) << kMaxDigit) * 4);
-  if (e == cudaSuccess) e = cudaFuncSetAttribute(sort_clear_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-  if (e == cudaSuccess)
-    e = cudaLaunchKernelEx(&cfg, sort_clear_kernel, tokens, n, V, padding_idx, pl.bits, pl.passes, item0, item1, gw,
-                           gw_bytes);
-  if (e != cudaSuccess) return fail(SPK_ERR_LAUNCH, "embedding_bwd: %s", cudaGetErrorString(e));
-  const uint2* items = pl.passes & 1 ? item0 : item1;
+  if (tokens) {
+    rc = launch_sort(pl, tokens, n, V, padding_idx, plan, st);
+    if (rc != SPK_OK) return rc;
+  }
+  const uint2* items = sorted_items(pl, plan);
+  float* part = reinterpret_cast<float*>(workspace);
 #define CALL(G, W)                                                                                        \
   constexpr int kWide = G == SPK_F32 || W == SPK_F32 ? 4 : 8;                                             \
   return vec == kWide ? launch_bwd<G, W, kWide>(pl, items, g, scale, n, V, (int)D, gw, part, st)          \

@@ -538,15 +538,29 @@ struct Shape {
 
 constexpr int kBwdPerSm = 3, kLongChunks = 64;
 
-// blocks of a kernel that walks over the rows: what the machine holds at once
+// Blocks of a kernel that walks over the rows: what the machine holds at once.
+// The answer for the last (device, threads, shared memory) is kept: asking takes
+// as long as a launch.
+struct Resident {
+  int dev = -1, threads = 0, per_sm = 1;
+  size_t smem = 0;
+};
 template <typename K>
-unsigned blocks_of(K kernel, int64_t rows, const Shape& s, size_t smem, int most) {
-  int per_sm = 1;
-  if (smem > (40u << 10))  // 48 KB without asking, the kernel's static arrays included
-    cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-  if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, s.threads(), smem) != cudaSuccess || per_sm < 1)
-    per_sm = 1;
-  if (per_sm > most) per_sm = most;
+unsigned blocks_of(K kernel, Resident& last, int64_t rows, const Shape& s, size_t smem, int most) {
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (last.dev != dev || last.threads != s.threads() || last.smem != smem) {
+    int per_sm = 1;
+    if (smem > (40u << 10))  // 48 KB without asking, the kernel's static arrays included
+      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, s.threads(), smem) != cudaSuccess || per_sm < 1)
+      per_sm = 1;
+    last.dev = dev;
+    last.threads = s.threads();
+    last.smem = smem;
+    last.per_sm = per_sm;
+  }
+  const int64_t per_sm = last.per_sm > most ? most : last.per_sm;
   const int64_t need = (rows + s.groups() - 1) / s.groups(), cap = (int64_t)num_sms() * per_sm;
   return (unsigned)(need < cap ? need : cap);
 }
@@ -561,7 +575,8 @@ template <int XDT, int VEC, int NV>
 void launch_fwd(const void* x, int64_t ld, const void* w, int wdt, const void* b, int bdt, float eps, int64_t rows,
                 int64_t D, const Shape& s, void* y, int ydt, float* stats, cudaStream_t st) {
   const size_t smem = (size_t)Fwd<XDT, VEC, NV>::X::kBytes * s.threads();
-  const unsigned blocks = blocks_of(fwd_kernel<XDT, VEC, NV>, rows, s, smem, 8);
+  static thread_local Resident last;
+  const unsigned blocks = blocks_of(fwd_kernel<XDT, VEC, NV>, last, rows, s, smem, 8);
   fwd_kernel<XDT, VEC, NV><<<blocks, s.threads(), smem, st>>>(reinterpret_cast<const typename Elem<XDT>::T*>(x), ld, w,
                                                              wdt, b, bdt, eps, rows, (int)D, s.wpr, y, ydt,
                                                              reinterpret_cast<float2*>(stats));
@@ -574,7 +589,8 @@ int launch_bwd(const void* g, const void* x, int64_t ld, const float* stats, con
   size_t smem = (size_t)(T::X::kBytes + T::G::kBytes) * s.threads();
   const size_t sums = part && s.groups() > 1 ? (size_t)s.groups() * 2 * D * sizeof(float) : 0;
   if (sums > smem) smem = sums;
-  const unsigned blocks = blocks_of(bwd_kernel<GDT, XDT, VEC, NV>, rows, s, smem, kBwdPerSm);
+  static thread_local Resident last;
+  const unsigned blocks = blocks_of(bwd_kernel<GDT, XDT, VEC, NV>, last, rows, s, smem, kBwdPerSm);
   bwd_kernel<GDT, XDT, VEC, NV><<<blocks, s.threads(), smem, st>>>(
       reinterpret_cast<const typename Elem<GDT>::T*>(g), reinterpret_cast<const typename Elem<XDT>::T*>(x), ld,
       reinterpret_cast<const float2*>(stats), w, wdt, rows, (int)D, s.wpr,

@@ -595,7 +595,7 @@ __device__ __forceinline__ void write_row(const Logits& x, const typename Elem<D
   if (lane == 0) {
     o.logp[r] = kLn2 * (log2_from(mean_over_t<DT>(row + y, x.st, x.T, x.inv_t), f) - l2s);
     o.entropy[r] = H;
-    o.stats[r] = make_float4(f.off, f.c, s.S, H);
+    if (o.stats) o.stats[r] = make_float4(f.off, f.c, s.S, H);
   }
   if (lane < K) {
     o.top_idx[r * K + lane] = (int64_t)(~(uint32_t)key);
@@ -607,7 +607,7 @@ __device__ __forceinline__ void write_row(const Logits& x, const typename Elem<D
 __device__ __forceinline__ void write_unused(int64_t r, int K, int lane, const Out& o) {
   if (lane == 0) {
     o.logp[r] = o.entropy[r] = 0.0f;
-    o.stats[r] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (o.stats) o.stats[r] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   }
   if (lane < K) {
     o.top_logp[r * K + lane] = 0.0f;
@@ -939,9 +939,9 @@ int dispatch_bwd(bool wide, const Logits& x, const int64_t* tokens, int64_t igno
 extern "C" {
 
 int64_t spk_token_logprobs_workspace_bytes(int64_t, int64_t rows, int64_t V, int64_t top_k) {
-  if (rows < 1 || V < 1 || top_k < 0) return 16;
+  if (rows < 1 || V < 1 || top_k < 0) return 0;
   const int64_t s = spk::lpk::splits_of(rows, V);
-  return s > 1 ? rows * s * (16 + 8 * top_k) : 16;
+  return s > 1 ? rows * s * (16 + 8 * top_k) : 0;
 }
 
 int spk_token_logprobs_fwd(const void* logits, int dtype, int64_t T, int64_t rows, int64_t V, int64_t step_stride,
@@ -950,10 +950,11 @@ int spk_token_logprobs_fwd(const void* logits, int dtype, int64_t T, int64_t row
                            void* workspace, int64_t workspace_bytes, void* stream) {
   using namespace spk;
   using namespace spk::lpk;
-  SPK_REQUIRE(logits && tokens && logp && entropy && stats && bad_token, SPK_ERR_INVALID, "null pointer argument");
+  SPK_REQUIRE(logits && tokens && logp && entropy && bad_token, SPK_ERR_INVALID, "null pointer argument");
   SPK_LP_SIZES();
   SPK_REQUIRE(top_k == 0 || (top_logp && top_idx), SPK_ERR_INVALID, "null top_logp or top_idx");
-  SPK_REQUIRE(workspace && workspace_bytes >= spk_token_logprobs_workspace_bytes(T, rows, V, top_k), SPK_ERR_INVALID,
+  const int64_t need = spk_token_logprobs_workspace_bytes(T, rows, V, top_k);
+  SPK_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), SPK_ERR_INVALID,
               "workspace smaller than spk_token_logprobs_workspace_bytes()");
   SPK_REQUIRE(aligned(workspace, 16), SPK_ERR_ALIGN, "workspace must be 16-byte aligned");
   int rc = check_stream_device(stream);

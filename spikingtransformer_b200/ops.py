@@ -638,21 +638,14 @@ def _float_code(dtype, what):
 
 def _one_device(first, *ts):
     """All CUDA tensors on one device; returns it."""
-    _cuda(first, *ts)
     dev = first.device
+    if dev.type != "cuda":
+        _cuda(first)
     for t in ts:
         if t is not None and t.device != dev:
+            _cuda(t)
             raise RuntimeError("tensors on different devices: %s and %s" % (dev, t.device))
     return dev
-
-
-def _call_on(dev, name, *args, tag, work):
-    """``_lib.call`` with ``dev`` current and its current stream as the last argument."""
-    stream = torch.cuda.current_stream(dev).cuda_stream
-    if torch.cuda.current_device() == dev.index:
-        return _lib.call(name, *args, stream, tag=tag, work=work)
-    with torch.cuda.device(dev):
-        return _lib.call(name, *args, stream, tag=tag, work=work)
 
 
 def _rows_of(x):
@@ -667,10 +660,6 @@ def _rows_of(x):
     return x, ld
 
 
-def _needs_grad(*ts):
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
-
-
 def _check_layer_norm(x, weight, bias):
     if x.dim() < 1 or x.shape[-1] < 1:
         raise RuntimeError("layer_norm needs a last dimension of at least 1 (got %s)" % (tuple(x.shape),))
@@ -682,29 +671,43 @@ def _check_layer_norm(x, weight, bias):
                 raise RuntimeError("layer_norm %s %s does not match the last dimension %d" % (what, tuple(t.shape), D))
 
 
+def _check_layer_norm_fwd(x, weight, bias, out_dtype):
+    """``(device, output type)`` of a forward with these arguments."""
+    dev = _one_device(x, weight, bias)
+    _float_code(x.dtype, "layer_norm input")
+    _check_layer_norm(x, weight, bias)
+    dt = x.dtype if out_dtype is None else out_dtype
+    _float_code(dt, "layer_norm output")
+    return dev, dt
+
+
 def layer_norm_fwd(x, weight=None, bias=None, eps=1e-5, out_dtype=None, want_stats=True):
     """LayerNorm over the last dimension of ``x`` (fp32, fp16 or bf16; any leading
     dimensions; a column slice of a wider tensor is read in place).  ``weight``
     and ``bias`` ``[D]`` or None, each of any of the three types.  Returns ``(y
     in out_dtype (x's by default), stats fp32 [rows, 2] (mean, 1 / std) or
     None)``; no autograd (``layer_norm`` has it)."""
-    dev = _one_device(x, weight, bias)
-    xc = _float_code(x.dtype, "layer_norm input")
-    _check_layer_norm(x, weight, bias)
-    dt = x.dtype if out_dtype is None else out_dtype
-    yc = _float_code(dt, "layer_norm output")
+    dev, dt = _check_layer_norm_fwd(x, weight, bias, out_dtype)
+    return _layer_norm_fwd(dev, x, weight, bias, eps, dt, want_stats)
+
+
+def _layer_norm_fwd(dev, x, weight, bias, eps, dt, want_stats):
     D = x.shape[-1]
     x, ld = _rows_of(x)
     rows = x.numel() // D
     y = torch.empty(x.shape, dtype=dt, device=dev)
     stats = torch.empty((rows, 2), dtype=torch.float32, device=dev) if want_stats else None
     if rows:
-        weight = None if weight is None else weight.contiguous()
-        bias = None if bias is None else bias.contiguous()
-        _call_on(dev, "spk_layer_norm_fwd", x.data_ptr(), xc, ld, _lib.ptr(weight),
-                 0 if weight is None else _FLOATS[weight.dtype], _lib.ptr(bias),
-                 0 if bias is None else _FLOATS[bias.dtype], float(eps), rows, D, y.data_ptr(), yc, _lib.ptr(stats),
-                 tag="layer_norm_fwd", work=dict(bytes=rows * D * (x.element_size() + y.element_size())))
+        wp = wc = bp = bc = 0
+        if weight is not None:
+            weight = weight.contiguous()
+            wp, wc = weight.data_ptr(), _FLOATS[weight.dtype]
+        if bias is not None:
+            bias = bias.contiguous()
+            bp, bc = bias.data_ptr(), _FLOATS[bias.dtype]
+        _lib.launch(dev, "spk_layer_norm_fwd", "layer_norm_fwd", rows * D * (x.itemsize + y.itemsize), x.data_ptr(),
+                    _FLOATS[x.dtype], ld, wp, wc, bp, bc, float(eps), rows, D, y.data_ptr(), _FLOATS[dt],
+                    stats.data_ptr() if want_stats else None)
     return y, stats
 
 
@@ -714,53 +717,60 @@ def layer_norm_bwd(g, x, stats, weight=None, need_x=True, need_weight=True, need
     default))``, None where not needed.  Sums are fp32 and their order is
     fixed: equal calls give equal bits."""
     dev = _one_device(x, g, stats, weight)
-    xc, gc = _float_code(x.dtype, "layer_norm input"), _float_code(g.dtype, "layer_norm gradient")
+    _float_code(x.dtype, "layer_norm input")
+    _float_code(g.dtype, "layer_norm gradient")
     _check_layer_norm(x, weight, None)
     if g.shape != x.shape:
         raise RuntimeError("gradient %s does not match input %s" % (tuple(g.shape), tuple(x.shape)))
-    D = x.shape[-1]
-    x, ld = _rows_of(x)
-    rows = x.numel() // D
-    if stats.dtype != torch.float32 or stats.numel() != 2 * rows or not stats.is_contiguous():
+    if stats.dtype != torch.float32 or stats.numel() != 2 * (x.numel() // x.shape[-1]) or not stats.is_contiguous():
         raise RuntimeError("layer_norm stats must be the contiguous fp32 [rows, 2] of layer_norm_fwd")
     wt = torch.float32 if weight is None else weight.dtype
     bt = wt if bias_dtype is None else bias_dtype
-    bc = _float_code(bt, "layer_norm bias gradient")
+    _float_code(bt, "layer_norm bias gradient")
+    return _layer_norm_bwd(dev, g, x, stats, weight, need_x, need_weight, need_bias, wt, bt)
+
+
+def _layer_norm_bwd(dev, g, x, stats, weight, need_x, need_weight, need_bias, wt, bt):
+    D = x.shape[-1]
+    x, ld = _rows_of(x)
+    rows = x.numel() // D
     gx = torch.empty(x.shape, dtype=x.dtype, device=dev) if need_x else None
     gw = torch.empty(D, dtype=wt, device=dev) if need_weight else None
     gb = torch.empty(D, dtype=bt, device=dev) if need_bias else None
     if not rows:
         return gx, None if gw is None else gw.zero_(), None if gb is None else gb.zero_()
-    if not (need_x or need_weight or need_bias):
-        return None, None, None
-    g = g.contiguous()
-    weight = None if weight is None else weight.contiguous()
     ws, wsb = None, 0
     if need_weight or need_bias:
-        wsb = int(_lib.load().spk_layer_norm_bwd_workspace_bytes(rows, D))
+        wsb = _lib.load().spk_layer_norm_bwd_workspace_bytes(rows, D)
         ws = torch.empty(wsb, dtype=torch.uint8, device=dev)
-    _call_on(dev, "spk_layer_norm_bwd", g.data_ptr(), gc, x.data_ptr(), xc, ld, stats.data_ptr(), _lib.ptr(weight),
-             _FLOATS[wt], rows, D, _lib.ptr(gx), _lib.ptr(gw), _lib.ptr(gb), bc, _lib.ptr(ws), wsb,
-             tag="layer_norm_bwd", work=dict(bytes=rows * D * (g.element_size() + 2 * x.element_size())))
+    elif not need_x:
+        return None, None, None
+    g = g.contiguous()
+    if weight is not None:
+        weight = weight.contiguous()
+    ptr = _lib.ptr
+    _lib.launch(dev, "spk_layer_norm_bwd", "layer_norm_bwd", rows * D * (g.itemsize + 2 * x.itemsize), g.data_ptr(),
+                _FLOATS[g.dtype], x.data_ptr(), _FLOATS[x.dtype], ld, stats.data_ptr(), ptr(weight), _FLOATS[wt], rows,
+                D, ptr(gx), ptr(gw), ptr(gb), _FLOATS[bt], ptr(ws), wsb)
     return gx, gw, gb
 
 
 class _LayerNorm(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, bias, eps, out_dtype):
-        y, stats = layer_norm_fwd(x, weight, bias, eps, out_dtype)
+    def forward(ctx, x, weight, bias, eps, dev, dt):
+        y, stats = _layer_norm_fwd(dev, x, weight, bias, eps, dt, True)
         ctx.save_for_backward(x, stats, weight)
-        ctx.bias_dtype = None if bias is None else bias.dtype
+        ctx.meta = dev, torch.float32 if weight is None else weight.dtype, torch.float32 if bias is None else bias.dtype
         return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g):
         x, stats, weight = ctx.saved_tensors
+        dev, wt, bt = ctx.meta
         need = ctx.needs_input_grad
-        gx, gw, gb = layer_norm_bwd(g, x, stats, weight, need_x=need[0], need_weight=need[1], need_bias=need[2],
-                                    bias_dtype=ctx.bias_dtype)
-        return gx, gw, gb, None, None
+        gx, gw, gb = _layer_norm_bwd(dev, g, x, stats, weight, need[0], need[1], need[2], wt, bt)
+        return gx, gw, gb, None, None, None
 
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5, out_dtype=None):
@@ -768,28 +778,44 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, out_dtype=None):
     without a LIF behind it, for the shapes and uses ``ln_lif_fwd`` does not
     cover): ``layer_norm_fwd`` with gradients of ``x``, ``weight`` and
     ``bias``."""
-    if not _needs_grad(x, weight, bias):
-        return layer_norm_fwd(x, weight, bias, eps, out_dtype, want_stats=False)[0]
-    return _LayerNorm.apply(x, weight, bias, eps, out_dtype)
+    dev, dt = _check_layer_norm_fwd(x, weight, bias, out_dtype)
+    if torch.is_grad_enabled() and (x.requires_grad or weight is not None and weight.requires_grad
+                                    or bias is not None and bias.requires_grad):
+        return _LayerNorm.apply(x, weight, bias, eps, dev, dt)
+    return _layer_norm_fwd(dev, x, weight, bias, eps, dt, False)[0]
+
+
+_INTS = (torch.int64, torch.int32, torch.int16, torch.int8, torch.uint8)
 
 
 def _tokens_i64(tokens):
-    if tokens.dtype not in (torch.int64, torch.int32, torch.int16, torch.int8, torch.uint8):
+    if tokens.dtype is torch.int64 and tokens.is_contiguous():
+        return tokens
+    if tokens.dtype not in _INTS:
         raise TypeError("tokens must be integers (got %s)" % tokens.dtype)
     return tokens.to(torch.int64).contiguous()
+
+
+def _check_embedding(tokens, weight, out_dtype):
+    """``(device, output type, int64 tokens)`` of a lookup with these arguments."""
+    dev = _one_device(weight, tokens)
+    if weight.dim() != 2 or weight.shape[0] < 1 or weight.shape[1] < 1:
+        raise RuntimeError("embedding weight must be [V, D] (got %s)" % (tuple(weight.shape),))
+    _float_code(weight.dtype, "embedding weight")
+    dt = weight.dtype if out_dtype is None else out_dtype
+    _float_code(dt, "embedding output")
+    return dev, dt, _tokens_i64(tokens)
 
 
 def embedding_fwd(tokens, weight, scale=1.0, out_dtype=None):
     """``scale * weight[tokens]`` (rounded once) without autograd: ``(out
     [*tokens.shape, D] in out_dtype (the weight's by default), bad)``; ``bad`` is
     a device flag, 1 if a token lies outside ``[0, V)`` (its row is zeros)."""
-    dev = _one_device(weight, tokens)
-    if weight.dim() != 2 or weight.shape[0] < 1 or weight.shape[1] < 1:
-        raise RuntimeError("embedding weight must be [V, D] (got %s)" % (tuple(weight.shape),))
-    wc = _float_code(weight.dtype, "embedding weight")
-    dt = weight.dtype if out_dtype is None else out_dtype
-    oc = _float_code(dt, "embedding output")
-    tokens = _tokens_i64(tokens)
+    dev, dt, tokens = _check_embedding(tokens, weight, out_dtype)
+    return _embedding_fwd(dev, tokens, weight, scale, dt, None, -1)
+
+
+def _embedding_fwd(dev, tokens, weight, scale, dt, plan, padding_idx):
     V, D = weight.shape
     weight, ld = _rows_of(weight)
     n = tokens.numel()
@@ -797,9 +823,10 @@ def embedding_fwd(tokens, weight, scale=1.0, out_dtype=None):
     if n == 0:
         return out, torch.zeros(1, dtype=torch.int32, device=dev)
     bad = torch.empty(1, dtype=torch.int32, device=dev)
-    _call_on(dev, "spk_embedding_fwd", tokens.data_ptr(), weight.data_ptr(), wc, ld, float(scale), n, V, D,
-             out.data_ptr(), oc, bad.data_ptr(), tag="embedding_fwd",
-             work=dict(bytes=n * (8 + D * (weight.element_size() + out.element_size()))))
+    _lib.launch(dev, "spk_embedding_fwd", "embedding_fwd", n * (8 + D * (weight.itemsize + out.itemsize)),
+                tokens.data_ptr(), weight.data_ptr(), _FLOATS[weight.dtype], ld, float(scale), n, V, D, out.data_ptr(),
+                _FLOATS[dt], bad.data_ptr(), padding_idx, None if plan is None else plan.data_ptr(),
+                0 if plan is None else plan.numel())
     return out, bad
 
 
@@ -809,49 +836,69 @@ def embedding_bwd(g, tokens, V, scale=1.0, padding_idx=None, dtype=torch.float32
     order of the tokens (equal calls give equal bits).  Rows without a token,
     and row ``padding_idx``, are zeros."""
     dev = _one_device(g, tokens)
-    gc, wc = _float_code(g.dtype, "embedding gradient"), _float_code(dtype, "embedding weight gradient")
+    _float_code(g.dtype, "embedding gradient")
+    _float_code(dtype, "embedding weight gradient")
     tokens = _tokens_i64(tokens)
     if g.dim() != tokens.dim() + 1 or g.shape[:-1] != tokens.shape or g.shape[-1] < 1 or V < 1:
         raise RuntimeError("gradient %s does not match tokens %s" % (tuple(g.shape), tuple(tokens.shape)))
-    n, D = tokens.numel(), g.shape[-1]
+    return _embedding_bwd(dev, g, tokens, _embedding_plan(dev, tokens), V, scale,
+                          -1 if padding_idx is None else int(padding_idx), dtype)
+
+
+def _embedding_plan(dev, tokens):
+    """Room for the positions sorted by token."""
+    return torch.empty(_lib.load().spk_embedding_plan_bytes(tokens.numel()), dtype=torch.uint8, device=dev)
+
+
+def _embedding_bwd(dev, g, tokens, plan, V, scale, padding_idx, dtype):
+    """``tokens`` None: ``plan`` is sorted already."""
+    D = g.shape[-1]
+    n = g.numel() // D
     if n == 0:
         return torch.zeros((V, D), dtype=dtype, device=dev)
     g = g.contiguous()
     gw = torch.empty((V, D), dtype=dtype, device=dev)
-    wsb = int(_lib.load().spk_embedding_bwd_workspace_bytes(n, V, D))
+    wsb = _lib.load().spk_embedding_bwd_workspace_bytes(n, V, D)
     ws = torch.empty(wsb, dtype=torch.uint8, device=dev)
-    _call_on(dev, "spk_embedding_bwd", tokens.data_ptr(), g.data_ptr(), gc, float(scale),
-             -1 if padding_idx is None else int(padding_idx), n, V, D, gw.data_ptr(), wc, ws.data_ptr(), wsb,
-             tag="embedding_bwd", work=dict(bytes=n * (8 + D * g.element_size()) + gw.numel() * gw.element_size()))
+    _lib.launch(dev, "spk_embedding_bwd", "embedding_bwd", n * (8 + D * g.itemsize) + V * D * gw.itemsize,
+                None if tokens is None else tokens.data_ptr(), g.data_ptr(), _FLOATS[g.dtype], float(scale),
+                padding_idx, n, V, D, gw.data_ptr(), _FLOATS[dtype], plan.data_ptr(), plan.numel(), ws.data_ptr(), wsb)
     return gw
 
 
 class _Embedding(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, tokens, weight, scale, padding_idx, out_dtype):
-        out, bad = embedding_fwd(tokens, weight, scale, out_dtype)
-        ctx.save_for_backward(tokens)
-        ctx.meta = (weight.shape[0], weight.dtype, float(scale), padding_idx)
+    def forward(ctx, weight, tokens, scale, padding_idx, dev, dt):
+        plan = _embedding_plan(dev, tokens)
+        out, bad = _embedding_fwd(dev, tokens, weight, scale, dt, plan, padding_idx)
+        ctx.save_for_backward(plan)
+        ctx.meta = dev, weight.shape[0], scale, padding_idx, weight.dtype
         ctx.mark_non_differentiable(bad)
+        ctx.set_materialize_grads(False)
         return out, bad
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g, _g_bad):
-        V, dtype, scale, padding_idx = ctx.meta
-        return None, embedding_bwd(g, ctx.saved_tensors[0], V, scale, padding_idx, dtype), None, None, None
+        if g is None:
+            return None, None, None, None, None, None
+        dev, V, scale, padding_idx, dtype = ctx.meta
+        return _embedding_bwd(dev, g, None, ctx.saved_tensors[0], V, scale, padding_idx, dtype), None, None, None, None, None
 
 
 def embedding(tokens, weight, scale=1.0, padding_idx=None, out_dtype=None):
     """Differentiable scaled token embedding (``Seq2Seq.py:29-36``: ``embedding(tokens)
-    * sqrt(D)``): ``embedding_fwd`` with the weight's gradient from
+    * sqrt(D)``): ``embedding_fwd`` with the weight's gradient of
     ``embedding_bwd``.  ``padding_idx`` (0 <= padding_idx < V, or None): the row
     that takes no gradient.  Returns ``(out, bad)``."""
-    if padding_idx is not None and not 0 <= padding_idx < weight.shape[0]:
+    dev, dt, tokens = _check_embedding(tokens, weight, out_dtype)
+    if padding_idx is None:
+        padding_idx = -1
+    elif not 0 <= padding_idx < weight.shape[0]:
         raise ValueError("padding_idx %d outside [0, %d)" % (padding_idx, weight.shape[0]))
-    if not _needs_grad(weight):
-        return embedding_fwd(tokens, weight, scale, out_dtype)
-    return _Embedding.apply(tokens, weight, scale, padding_idx, out_dtype)
+    if torch.is_grad_enabled() and weight.requires_grad:
+        return _Embedding.apply(weight, tokens, scale, padding_idx, dev, dt)
+    return _embedding_fwd(dev, tokens, weight, scale, dt, None, -1)
 
 
 MAX_TOP_K = 32  # alternatives that token_logprobs can return
@@ -861,63 +908,68 @@ def _logit_rows(logits):
     """``(logits, step stride, row stride)`` of ``[T, ..., V]`` as ``[T, rows, V]``,
     read in place where the layout allows."""
     V = logits.shape[-1]
-    T, rows = logits.shape[0], logits[0].numel() // V
     if logits.is_contiguous():
+        rows = logits.numel() // (logits.shape[0] * V)
         return logits, rows * V, V
+    rows = logits[0].numel() // V
     ld = _row_stride(logits[0]) if logits.dim() > 2 else (V if logits.stride(-1) == 1 else None)
     if ld is None or (ld < V and rows > 1) or logits.stride(0) < 0:
         return logits.contiguous(), rows * V, V
     return logits, logits.stride(0), ld
 
 
-def _token_logprobs_fwd(logits, tokens, top_k, ignore_index):
-    dev = logits.device
+def _token_logprobs_fwd(dev, logits, tokens, top_k, ignore_index, want_stats):
     T, V, rows = logits.shape[0], logits.shape[-1], tokens.numel()
     shape = tokens.shape
-    f32 = dict(dtype=torch.float32, device=dev)
-    logp, entropy, stats = torch.empty(shape, **f32), torch.empty(shape, **f32), torch.empty((rows, 4), **f32)
-    top_logp = torch.empty((*shape, top_k), **f32) if top_k else None
+    f32 = torch.float32
+    logp, entropy = torch.empty(shape, dtype=f32, device=dev), torch.empty(shape, dtype=f32, device=dev)
+    stats = torch.empty((rows, 4), dtype=f32, device=dev) if want_stats else None
+    top_logp = torch.empty((*shape, top_k), dtype=f32, device=dev) if top_k else None
     top_idx = torch.empty((*shape, top_k), dtype=torch.int64, device=dev) if top_k else None
     if rows == 0:
         return logp, entropy, top_logp, top_idx, torch.zeros(1, dtype=torch.int32, device=dev), stats
     bad = torch.empty(1, dtype=torch.int32, device=dev)
     logits, st, sr = _logit_rows(logits)
-    wsb = int(_lib.load().spk_token_logprobs_workspace_bytes(T, rows, V, top_k))
-    ws = torch.empty(wsb, dtype=torch.uint8, device=dev)
-    _call_on(dev, "spk_token_logprobs_fwd", logits.data_ptr(), _FLOATS[logits.dtype], T, rows, V, st, sr,
-             tokens.data_ptr(), ignore_index, top_k, logp.data_ptr(), entropy.data_ptr(), _lib.ptr(top_logp),
-             _lib.ptr(top_idx), stats.data_ptr(), bad.data_ptr(), ws.data_ptr(), wsb, tag="token_logprobs_fwd",
-             work=dict(bytes=T * rows * V * logits.element_size()))
+    wsb = _lib.load().spk_token_logprobs_workspace_bytes(T, rows, V, top_k)
+    ws = torch.empty(wsb, dtype=torch.uint8, device=dev) if wsb else None
+    ptr = _lib.ptr
+    _lib.launch(dev, "spk_token_logprobs_fwd", "token_logprobs_fwd", T * rows * V * logits.itemsize,
+                logits.data_ptr(), _FLOATS[logits.dtype], T, rows, V, st, sr, tokens.data_ptr(), ignore_index, top_k,
+                logp.data_ptr(), entropy.data_ptr(), ptr(top_logp), ptr(top_idx), ptr(stats), bad.data_ptr(), ptr(ws),
+                wsb)
     return logp, entropy, top_logp, top_idx, bad, stats
 
 
 class _TokenLogprobs(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logits, tokens, top_k, ignore_index):
-        logp, entropy, top_logp, top_idx, bad, stats = _token_logprobs_fwd(logits, tokens, top_k, ignore_index)
+    def forward(ctx, logits, tokens, top_k, ignore_index, dev):
+        logp, entropy, top_logp, top_idx, bad, stats = _token_logprobs_fwd(dev, logits, tokens, top_k, ignore_index,
+                                                                           True)
         ctx.save_for_backward(logits, tokens, top_idx, stats)
-        ctx.meta = (top_k, ignore_index)
+        ctx.meta = dev, top_k, ignore_index
         ctx.set_materialize_grads(False)
-        ctx.mark_non_differentiable(*[t for t in (top_idx, bad) if t is not None])
+        if top_idx is None:
+            ctx.mark_non_differentiable(bad)
+        else:
+            ctx.mark_non_differentiable(top_idx, bad)
         return logp, entropy, top_logp, top_idx, bad
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g_logp, g_entropy, g_top, _g_idx, _g_bad):
         logits, tokens, top_idx, stats = ctx.saved_tensors
-        top_k, ignore_index = ctx.meta
-        dev = logits.device
+        dev, top_k, ignore_index = ctx.meta
         grad = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
         rows = tokens.numel()
         if rows:
-            gs = [None if g is None else g.contiguous() for g in (g_logp, g_entropy, g_top)]
+            g_logp, g_entropy, g_top = (None if g is None else g.contiguous() for g in (g_logp, g_entropy, g_top))
             x, st, sr = _logit_rows(logits)
             T, V = x.shape[0], x.shape[-1]
-            _call_on(dev, "spk_token_logprobs_bwd", x.data_ptr(), _FLOATS[x.dtype], T, rows, V, st, sr,
-                     tokens.data_ptr(), ignore_index, top_k, _lib.ptr(top_idx), stats.data_ptr(),
-                     *[_lib.ptr(g) for g in gs], grad.data_ptr(), tag="token_logprobs_bwd",
-                     work=dict(bytes=2 * T * rows * V * x.element_size()))
-        return grad, None, None, None
+            ptr = _lib.ptr
+            _lib.launch(dev, "spk_token_logprobs_bwd", "token_logprobs_bwd", 2 * T * rows * V * x.itemsize,
+                        x.data_ptr(), _FLOATS[x.dtype], T, rows, V, st, sr, tokens.data_ptr(), ignore_index, top_k,
+                        ptr(top_idx), stats.data_ptr(), ptr(g_logp), ptr(g_entropy), ptr(g_top), grad.data_ptr())
+        return grad, None, None, None, None
 
 
 def token_logprobs(logits, tokens, top_k=0, ignore_index=-100):
@@ -934,7 +986,7 @@ def token_logprobs(logits, tokens, top_k=0, ignore_index=-100):
     gradient; so do tokens outside ``[0, V)``, which set the device flag
     ``bad``.  A row of logits that are all -inf has no distribution: NaN
     (one that is all the type's lowest value is uniform)."""
-    _one_device(logits, tokens)
+    dev = _one_device(logits, tokens)
     _float_code(logits.dtype, "logits")
     if logits.dim() < 2 or logits.shape[0] < 1 or logits.shape[-1] < 1 or logits.shape[1:-1] != tokens.shape:
         raise RuntimeError("tokens %s do not match logits %s ([T, ..., V])"
@@ -942,9 +994,9 @@ def token_logprobs(logits, tokens, top_k=0, ignore_index=-100):
     if not 0 <= top_k <= min(MAX_TOP_K, logits.shape[-1]):
         raise ValueError("top_k must be between 0 and min(%d, V) (got %d)" % (MAX_TOP_K, top_k))
     tokens = _tokens_i64(tokens)
-    if not _needs_grad(logits):
-        return _token_logprobs_fwd(logits, tokens, int(top_k), int(ignore_index))[:5]
-    return _TokenLogprobs.apply(logits, tokens, int(top_k), int(ignore_index))
+    if torch.is_grad_enabled() and logits.requires_grad:
+        return _TokenLogprobs.apply(logits, tokens, int(top_k), int(ignore_index), dev)
+    return _token_logprobs_fwd(dev, logits, tokens, int(top_k), int(ignore_index), False)[:5]
 
 
 def device_error_check(device=None):

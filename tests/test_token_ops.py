@@ -60,16 +60,21 @@ def test_c_entries_reject_bad_arguments():
     assert lib.spk_layer_norm_fwd(p, 0, 8, None, 0, None, 0, 1e-5, 0, 8, p, 0, None, None) == 2   # no rows
     assert lib.spk_layer_norm_bwd(p, 0, p, 0, 8, None, p, 0, 2, 8, p, p, p, 0, p, 1 << 30, None) == 1
     assert lib.spk_layer_norm_bwd(p, 0, p, 0, 8, p, p, 0, 2, 8, p, p, p, 0, p, 4, None) == 1      # workspace
-    assert lib.spk_embedding_fwd(p, p, 0, 8, 1.0, 4, 10, 8, p, 0, None, None) == 1
-    assert lib.spk_embedding_fwd(p, p, 0, 7, 1.0, 4, 10, 8, p, 0, p, None) == 2
-    assert lib.spk_embedding_fwd(p, p, 5, 8, 1.0, 4, 10, 8, p, 0, p, None) == 1
-    assert lib.spk_embedding_bwd(p, p, 0, 1.0, -1, 4, 0, 8, p, 0, p, 1 << 30, None) == 2
-    assert lib.spk_embedding_bwd(p, p, 0, 1.0, -1, 4, 10, 8, p, 0, p, 0, None) == 1               # workspace
+    tail = (-1, None, 0, None)
+    assert lib.spk_embedding_fwd(p, p, 0, 8, 1.0, 4, 10, 8, p, 0, None, *tail) == 1
+    assert lib.spk_embedding_fwd(p, p, 0, 7, 1.0, 4, 10, 8, p, 0, p, *tail) == 2
+    assert lib.spk_embedding_fwd(p, p, 5, 8, 1.0, 4, 10, 8, p, 0, p, *tail) == 1
+    assert lib.spk_embedding_fwd(p, p, 0, 8, 1.0, 4, 10, 8, p, 0, p, -1, p, 63, None) == 1        # plan: 4 tokens
+    assert lib.spk_embedding_bwd(p, p, 0, 1.0, -1, 4, 0, 8, p, 0, p, 1 << 30, p, 1 << 30, None) == 2
+    assert lib.spk_embedding_bwd(p, p, 0, 1.0, -1, 4, 10, 8, p, 0, p, 63, p, 1 << 30, None) == 1  # plan
+    assert lib.spk_embedding_bwd(p, p, 0, 1.0, -1, 4, 10, 8, p, 0, p, 64, p, 0, None) == 1        # workspace
+    assert lib.spk_embedding_bwd(p, p, 0, 1.0, -1, 4, 10, 8, p, 0, None, 64, p, 1 << 30, None) == 1
     args = (p, p, p, p, p, p, p, 1 << 30, None)
     assert lib.spk_token_logprobs_fwd(None, 0, 1, 2, 8, 0, 8, p, -100, 0, *args) == 1
     assert lib.spk_token_logprobs_fwd(p, 3, 1, 2, 8, 0, 8, p, -100, 0, *args) == 1
     assert lib.spk_token_logprobs_fwd(p, 0, 1, 2, 8, 0, 8, p, -100, 9, *args) == 2                # top_k > V
     assert lib.spk_token_logprobs_fwd(p, 0, 1, 2, 99, 0, 99, p, -100, 33, *args) == 2             # top_k > 32
+    assert lib.spk_token_logprobs_fwd(p, 0, 1, 2, 99999, 0, 99999, p, -100, 0, *args[:-3], p, 16, None) == 1  # workspace
     assert lib.spk_token_logprobs_fwd(p, 0, 65, 2, 8, 0, 8, p, -100, 0, *args) == 2
     assert lib.spk_token_logprobs_fwd(p, 0, 1, 2, 8, 0, -8, p, -100, 0, *args) == 2
     assert lib.spk_token_logprobs_bwd(p, 0, 1, 2, 8, 0, 8, p, -100, 4, None, p, p, p, p, p, None) == 1  # no indices
