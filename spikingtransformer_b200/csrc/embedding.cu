@@ -32,18 +32,19 @@ constexpr int kDeep = 8;
 // A warp per (kDeep tokens, tile of 32 * VEC columns): the tokens are read
 // together, then their rows, then written.
 template <int WDT, int ODT, int VEC>
-__global__ void __launch_bounds__(256) gather_kernel(const int64_t* __restrict__ tokens,
+__global__ void __launch_bounds__(256, 4) gather_kernel(const int64_t* __restrict__ tokens,
                                                      const typename Elem<WDT>::T* __restrict__ w, int64_t ldw,
                                                      float scale, int64_t n, int64_t V, int D, int tiles,
                                                      typename Elem<ODT>::T* __restrict__ out, int* bad, int scan_bad,
                                                      int after_sort) {
-  // the sort before this kernel may still be running; whoever comes next finds it done
+  // The sort before this kernel may still be running: the last block does not end before it,
+  // so whoever comes after this kernel finds the sort done.
   struct AtEnd {
-    int on;
+    bool on;
     __device__ ~AtEnd() {
       if (on) pdl_wait();
     }
-  } at_end{after_sort};
+  } at_end{after_sort && blockIdx.x == gridDim.x - 1};
   if (scan_bad && blockIdx.x == 0) {  // the first block, so that it is not the last to end
     scan_tokens(tokens, n, V, 0, bad);
     return;
