@@ -48,7 +48,12 @@ class PositionalEncoding(nn.Module):
 
 
 class TokenEmbedding(nn.Module):
-    """``Seq2Seq.py:29-36``: ``embedding(tokens) * sqrt(emb_size)``."""
+    """``Seq2Seq.py:29-36``: ``embedding(tokens) * sqrt(emb_size)``, on CUDA through
+    ``ops.embedding`` (lookup and scaling in one kernel, the weight's gradient by
+    sorted tokens).  ``bad_tokens`` is then the device flag of the last call: 1 if
+    a token lay outside the vocabulary (its row is zeros)."""
+
+    bad_tokens = None
 
     def __init__(self, vocab_size: int, emb_size: int):
         super().__init__()
@@ -56,7 +61,13 @@ class TokenEmbedding(nn.Module):
         self.emb_size = emb_size
 
     def forward(self, tokens: Tensor):
-        return self.embedding(tokens.long()) * math.sqrt(self.emb_size)
+        e = self.embedding
+        if e.weight.is_cuda and e.weight.dtype in ops.EMBEDDING_DTYPES and e.max_norm is None \
+                and not e.scale_grad_by_freq and not e.sparse:
+            pad = e.padding_idx
+            out, self.bad_tokens = ops.embedding(tokens, e.weight, math.sqrt(self.emb_size), padding_idx=pad)
+            return out
+        return e(tokens.long()) * math.sqrt(self.emb_size)
 
 
 class Seq2Seq(nn.Module):
@@ -167,6 +178,16 @@ class Seq2Seq(nn.Module):
         out = self.output_layer(y)
         return out.view(T, out.shape[0] // T, out.shape[1], out.shape[2]), None
 
+    def score(self, src: Tensor, tgt: Tensor, targets: Tensor, look_ahead_mask: Tensor = None, top_k: int = 0,
+              ignore_index: int = -100):
+        """Teacher-forced scores of ``targets`` [B, N] given images ``src`` and the
+        decoder input ``tgt`` [B, N]: ``ops.token_logprobs`` of the forward's
+        logits, that is ``(logp [B, N], entropy [B, N], top_logp, top_idx [B, N,
+        top_k], bad)`` under the T-averaged logits.  Differentiable where
+        gradients are enabled."""
+        logits, _ = self.forward(src, tgt, look_ahead_mask)
+        return ops.token_logprobs(logits, targets, top_k=top_k, ignore_index=ignore_index)
+
     def create_padding_mask(self, seq: Tensor, pad_idx: int, device) -> Tensor:
         return torch.where(seq == pad_idx, 0.0, 1.0).unsqueeze(1).unsqueeze(1).to(device)
 
@@ -217,7 +238,7 @@ class Seq2Seq(nn.Module):
 
     @torch.no_grad()
     def greedy_decode_batch(self, src: Tensor, max_len: int, start_symbol: int, eos_idx: int, pad_idx: int,
-                            device: str = "cuda"):
+                            device: str = "cuda", return_logprobs: bool = False):
         """Greedy decoding of a batch of images ``src`` [B, C, H, W] in one
         pass per step.
 
@@ -226,7 +247,10 @@ class Seq2Seq(nn.Module):
         returns for image b alone.  Decoding continues until every row has
         produced ``eos_idx`` (or ``max_len`` tokens); positions after a row's
         eos are set to ``pad_idx``.  Returns ``(ys [B, L], lengths [B])``,
-        ``lengths`` counting the start symbol and the eos.
+        ``lengths`` counting the start symbol and the eos; with
+        ``return_logprobs`` also ``logp [B, L]``, the log probability of every
+        token under the T-averaged logits that chose it (0 for the start symbol
+        and behind a row's end).
         """
         if src.dim() == 3:
             src = src.unsqueeze(0)
@@ -241,6 +265,7 @@ class Seq2Seq(nn.Module):
         ys = torch.full((B, 1), fill_value=start_symbol, dtype=torch.long, device=device)
         done = torch.zeros(B, dtype=torch.bool, device=device)
         lengths = torch.full((B,), max_len, dtype=torch.long, device=device)
+        logps = [torch.zeros(B, device=device)]
         for n in range(1, max_len):
             tgt_mask = self.create_decoder_mask(ys, pad_idx, device)
             if fast:
@@ -248,6 +273,8 @@ class Seq2Seq(nn.Module):
             else:
                 out, _ = self.decode(ys, memory, tgt_mask)
             nxt = torch.argmax(out.mean(dim=0)[:, -1, :], dim=-1)
+            if return_logprobs:
+                logps.append(ops.token_logprobs(out[:, :, -1, :], nxt)[0])
             hit = (nxt == eos_idx) & ~done
             lengths = torch.where(hit, torch.full_like(lengths, n + 1), lengths)
             ys = torch.cat([ys, nxt.unsqueeze(1)], dim=1)
@@ -255,5 +282,9 @@ class Seq2Seq(nn.Module):
             if bool(done.all()):
                 break
         pos = torch.arange(ys.shape[1], device=device).unsqueeze(0)
-        ys = torch.where(pos < lengths.clamp(max=ys.shape[1]).unsqueeze(1), ys, torch.full_like(ys, pad_idx))
-        return ys, lengths.clamp(max=ys.shape[1])
+        inside = pos < lengths.clamp(max=ys.shape[1]).unsqueeze(1)
+        ys = torch.where(inside, ys, torch.full_like(ys, pad_idx))
+        lengths = lengths.clamp(max=ys.shape[1])
+        if return_logprobs:
+            return ys, lengths, torch.where(inside, torch.stack(logps, dim=1), 0.0)
+        return ys, lengths

@@ -648,6 +648,25 @@ def _one_device(first, *ts):
     return dev
 
 
+def _backward(fn):
+    """The backward of a Function with first derivatives only: as
+    ``once_differentiable``, whose work is skipped where no graph of the
+    gradient is being built."""
+    guarded = torch.autograd.function.once_differentiable(fn)
+
+    def backward(ctx, *grads):
+        return guarded(ctx, *grads) if torch.is_grad_enabled() else fn(ctx, *grads)
+
+    return staticmethod(backward)
+
+
+def _empty_as(x, dtype, device):
+    """A contiguous tensor of ``x``'s shape."""
+    if x.dtype is dtype and x.is_contiguous():
+        return torch.empty_like(x)
+    return torch.empty(x.shape, dtype=dtype, device=device)
+
+
 def _rows_of(x):
     """``(x, row stride)`` of ``x`` as ``[rows, x.shape[-1]]`` with unit column stride:
     in place where the layout allows (a column slice), else a contiguous copy."""
@@ -695,7 +714,7 @@ def _layer_norm_fwd(dev, x, weight, bias, eps, dt, want_stats):
     D = x.shape[-1]
     x, ld = _rows_of(x)
     rows = x.numel() // D
-    y = torch.empty(x.shape, dtype=dt, device=dev)
+    y = _empty_as(x, dt, dev)
     stats = torch.empty((rows, 2), dtype=torch.float32, device=dev) if want_stats else None
     if rows:
         wp = wc = bp = bc = 0
@@ -734,7 +753,7 @@ def _layer_norm_bwd(dev, g, x, stats, weight, need_x, need_weight, need_bias, wt
     D = x.shape[-1]
     x, ld = _rows_of(x)
     rows = x.numel() // D
-    gx = torch.empty(x.shape, dtype=x.dtype, device=dev) if need_x else None
+    gx = _empty_as(x, x.dtype, dev) if need_x else None
     gw = torch.empty(D, dtype=wt, device=dev) if need_weight else None
     gb = torch.empty(D, dtype=bt, device=dev) if need_bias else None
     if not rows:
@@ -763,8 +782,7 @@ class _LayerNorm(torch.autograd.Function):
         ctx.meta = dev, torch.float32 if weight is None else weight.dtype, torch.float32 if bias is None else bias.dtype
         return y
 
-    @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_backward
     def backward(ctx, g):
         x, stats, weight = ctx.saved_tensors
         dev, wt, bt = ctx.meta
@@ -794,6 +812,9 @@ def _tokens_i64(tokens):
     if tokens.dtype not in _INTS:
         raise TypeError("tokens must be integers (got %s)" % tokens.dtype)
     return tokens.to(torch.int64).contiguous()
+
+
+EMBEDDING_DTYPES = tuple(_FLOATS)  # weights that embedding takes
 
 
 def _check_embedding(tokens, weight, out_dtype):
@@ -877,8 +898,7 @@ class _Embedding(torch.autograd.Function):
         ctx.set_materialize_grads(False)
         return out, bad
 
-    @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_backward
     def backward(ctx, g, _g_bad):
         if g is None:
             return None, None, None, None, None, None
@@ -954,12 +974,11 @@ class _TokenLogprobs(torch.autograd.Function):
             ctx.mark_non_differentiable(top_idx, bad)
         return logp, entropy, top_logp, top_idx, bad
 
-    @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_backward
     def backward(ctx, g_logp, g_entropy, g_top, _g_idx, _g_bad):
         logits, tokens, top_idx, stats = ctx.saved_tensors
         dev, top_k, ignore_index = ctx.meta
-        grad = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
+        grad = _empty_as(logits, logits.dtype, dev)
         rows = tokens.numel()
         if rows:
             g_logp, g_entropy, g_top = (None if g is None else g.contiguous() for g in (g_logp, g_entropy, g_top))

@@ -743,6 +743,84 @@ def test_token_logprobs_gradient_against_differences(ops):
     assert abs((gx.cpu().double() * v).sum() - diff) <= bound
 
 
+# ------------------------------------------------------------------ in the model
+
+
+def small_model(dropout=0.0):
+    from spikingtransformer_b200.Seq2Seq import Seq2Seq
+    torch.manual_seed(3)
+    return Seq2Seq(patch_size=16, d_model=64, n_heads=4, ff_dim=128, num_encoder_layers=1, num_decoder_layers=1,
+                   dropout=dropout, tgt_vocab_size=64, n_steps=4, image_encoder="patch").to(DEV)
+
+
+@pytest.mark.gpu
+def test_token_embedding_module_matches_the_lookup(ops):
+    from spikingtransformer_b200.Seq2Seq import TokenEmbedding
+    torch.manual_seed(1)
+    m = TokenEmbedding(50, 96).to(DEV)
+    tok = torch.randint(0, 50, (4, 17), device=DEV)
+    g = torch.randint(-5, 6, (4, 17, 96), device=DEV).float()
+    out = m(tok)
+    (gw,) = torch.autograd.grad(out, m.embedding.weight, g)
+    ref = m.embedding(tok) * 96 ** 0.5
+    (rw,) = torch.autograd.grad(ref, m.embedding.weight, g)
+    assert torch.equal(out, ref) and int(m.bad_tokens) == 0   # the product is rounded once on both sides
+    # 68 tokens: each way sums a row's few terms (one scales before, one after) within (c + 2) u of their size
+    size = torch.zeros(50, 96, device=DEV).index_add_(0, tok.flatten(), g.abs().flatten(0, 1)) * 96 ** 0.5
+    assert ((gw - rw).abs() <= 2 * (68 + 2) * U * size).all()
+    assert torch.equal(m(tok.int()), ref) and torch.equal(m.half()(tok), (m.embedding.weight[tok].float() * 96 ** 0.5).half())
+    m.float().embedding.padding_idx = 3
+    (gw,) = torch.autograd.grad(m(tok), m.embedding.weight, g)
+    assert not gw[3].any()
+    assert list(m.state_dict()) == ["embedding.weight"]
+    m(tok + 50)
+    assert int(m.bad_tokens) == 1
+
+
+@pytest.mark.gpu
+def test_score_is_the_log_softmax_of_the_mean_logits(ops):
+    model = small_model().eval()
+    g = gen(2)
+    src = (torch.rand(3, 1, 32, 128, generator=g) * 0.2).to(DEV)
+    tgt = torch.randint(1, 64, (3, 9), generator=g).to(DEV)
+    targets = torch.randint(1, 64, (3, 9), generator=g)
+    targets[1, 4:] = 0
+    mask = model.create_decoder_mask(tgt, 0, DEV)
+    with torch.no_grad():
+        logits, _ = model(src, tgt, mask)
+        logp, H, top, idx, bad = model.score(src, tgt, targets.to(DEV), mask, top_k=4, ignore_index=0)
+    o = lp_exact(logits.cpu(), targets, 4, ignore=0)
+    assert int(bad) == 0 and torch.equal(idx.cpu(), o["top_idx"])
+    assert_within(logp, o["logp"], o["e_logp"], "logp")
+    assert_within(H, o["entropy"], o["e_H"], "entropy")
+    model.train()
+    loss = -model.score(src, tgt, targets.to(DEV), mask, ignore_index=0)[0].sum()
+    loss.backward()
+    for name in ("output_layer.weight", "tgt_tok_emb.embedding.weight"):
+        grad = dict(model.named_parameters())[name].grad
+        assert grad is not None and torch.isfinite(grad).all() and grad.any(), name
+
+
+@pytest.mark.gpu
+def test_greedy_decoding_returns_its_tokens_log_probabilities(ops):
+    model = small_model().eval()
+    src = (torch.rand(4, 1, 32, 128, generator=gen(5)) * 0.2).to(DEV)
+    ys, lengths = model.greedy_decode_batch(src, 8, 1, 2, 0)
+    ys2, lengths2, logp = model.greedy_decode_batch(src, 8, 1, 2, 0, return_logprobs=True)
+    assert torch.equal(ys, ys2) and torch.equal(lengths, lengths2) and logp.shape == ys.shape
+    assert not logp[:, 0].any()
+    for b in range(4):
+        n = int(lengths[b])
+        assert not logp[b, n:].any()
+        # the last token again, from the whole prefix before it
+        pre = ys[b:b + 1, :n - 1]
+        with torch.no_grad():
+            enc, _ = model.encode(src[b:b + 1])
+            out, _ = model.decode(pre, enc, model.create_decoder_mask(pre, 0, DEV))
+        o = lp_exact(out[:, :, -1].cpu(), ys[b, n - 1:n].cpu(), 0)
+        assert_within(logp[b, n - 1:n], o["logp"], o["e_logp"] + 1e-5, "logp")
+
+
 # ------------------------------------------------------------------ together, streams, graphs
 
 
