@@ -62,10 +62,11 @@ class TokenEmbedding(nn.Module):
 
     def forward(self, tokens: Tensor):
         e = self.embedding
-        if e.weight.is_cuda and e.weight.dtype in ops.EMBEDDING_DTYPES and e.max_norm is None \
-                and not e.scale_grad_by_freq and not e.sparse:
-            pad = e.padding_idx
-            out, self.bad_tokens = ops.embedding(tokens, e.weight, math.sqrt(self.emb_size), padding_idx=pad)
+        plain = e.max_norm is None and not (e.scale_grad_by_freq or e.sparse or e._forward_hooks
+                                            or e._forward_pre_hooks or e._backward_hooks)
+        if plain and e.weight.is_cuda and e.weight.dtype in ops.EMBEDDING_DTYPES:
+            out, self.bad_tokens = ops.embedding(tokens.long(), e.weight, math.sqrt(self.emb_size),
+                                                 padding_idx=e.padding_idx)
             return out
         return e(tokens.long()) * math.sqrt(self.emb_size)
 

@@ -203,10 +203,10 @@ def _raise(name, rc):
     raise RuntimeError("%s failed (%s): %s" % (name, status, msg))
 
 
-def launch(device, name, tag, nbytes, *args):
+def launch(device, name, tag, kernels, nbytes, *args):
     """``call`` of an entry point whose last argument is the stream, on ``device`` (made
-    current for the call where it is not) and its current stream.  Kept short:
-    the smallest calls are bound by the host."""
+    current for the call where it is not) and its current stream; ``kernels``: how
+    many it launches.  Kept short: the smallest calls are bound by the host."""
     index = device.index
     if _counter is None and _recorder is None and torch.cuda.current_device() == index:
         rc = getattr(_lib or load(), name)(*args, torch._C._cuda_getCurrentRawStream(index))
@@ -214,7 +214,8 @@ def launch(device, name, tag, nbytes, *args):
             _raise(name, rc)
         return
     with torch.cuda.device(device):
-        call(name, *args, torch.cuda.current_stream(device).cuda_stream, tag=tag, work=dict(bytes=nbytes))
+        call(name, *args, torch.cuda.current_stream(device).cuda_stream, tag=tag,
+             work=dict(bytes=nbytes, launches=kernels))
 
 
 def stream_ptr(device=None):

@@ -929,7 +929,7 @@ int dispatch_bwd(bool wide, const Logits& x, const int64_t* tokens, int64_t igno
 
 #define SPK_LP_SIZES()                                                                                              \
   SPK_REQUIRE(float_type(dtype), SPK_ERR_INVALID, "logits must be fp32, fp16 or bf16");                            \
-  SPK_REQUIRE(T >= 1 && T <= 64 && rows >= 1 && rows < (1ll << 25) && V >= 1 && V < (1ll << 30), SPK_ERR_SHAPE,     \
+  SPK_REQUIRE(T >= 1 && T <= 64 && rows >= 1 && rows < (1ll << 31) - 8 && V >= 1 && V < (1ll << 30), SPK_ERR_SHAPE,     \
               "unsupported sizes T=%lld rows=%lld V=%lld", (long long)T, (long long)rows, (long long)V);            \
   SPK_REQUIRE((T == 1 || step_stride >= 0) && (rows == 1 || row_stride >= 0), SPK_ERR_SHAPE, "negative stride");    \
   SPK_REQUIRE(top_k >= 0 && top_k <= kMaxTop && top_k <= V, SPK_ERR_SHAPE, "top_k=%lld: at most %d and V",          \

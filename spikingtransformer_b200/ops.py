@@ -724,7 +724,7 @@ def _layer_norm_fwd(dev, x, weight, bias, eps, dt, want_stats):
         if bias is not None:
             bias = bias.contiguous()
             bp, bc = bias.data_ptr(), _FLOATS[bias.dtype]
-        _lib.launch(dev, "spk_layer_norm_fwd", "layer_norm_fwd", rows * D * (x.itemsize + y.itemsize), x.data_ptr(),
+        _lib.launch(dev, "spk_layer_norm_fwd", "layer_norm_fwd", 1, rows * D * (x.itemsize + y.itemsize), x.data_ptr(),
                     _FLOATS[x.dtype], ld, wp, wc, bp, bc, float(eps), rows, D, y.data_ptr(), _FLOATS[dt],
                     stats.data_ptr() if want_stats else None)
     return y, stats
@@ -768,7 +768,7 @@ def _layer_norm_bwd(dev, g, x, stats, weight, need_x, need_weight, need_bias, wt
     if weight is not None:
         weight = weight.contiguous()
     ptr = _lib.ptr
-    _lib.launch(dev, "spk_layer_norm_bwd", "layer_norm_bwd", rows * D * (g.itemsize + 2 * x.itemsize), g.data_ptr(),
+    _lib.launch(dev, "spk_layer_norm_bwd", "layer_norm_bwd", 1 if ws is None else 2, rows * D * (g.itemsize + 2 * x.itemsize), g.data_ptr(),
                 _FLOATS[g.dtype], x.data_ptr(), _FLOATS[x.dtype], ld, stats.data_ptr(), ptr(weight), _FLOATS[wt], rows,
                 D, ptr(gx), ptr(gw), ptr(gb), _FLOATS[bt], ptr(ws), wsb)
     return gx, gw, gb
@@ -794,8 +794,9 @@ class _LayerNorm(torch.autograd.Function):
 def layer_norm(x, weight=None, bias=None, eps=1e-5, out_dtype=None):
     """Differentiable LayerNorm over the last dimension (``torch.nn.LayerNorm``
     without a LIF behind it, for the shapes and uses ``ln_lif_fwd`` does not
-    cover): ``layer_norm_fwd`` with gradients of ``x``, ``weight`` and
-    ``bias``."""
+    cover): ``layer_norm_fwd`` with gradients of ``x``, ``weight`` and ``bias``
+    (first derivatives only).  Autocast does not change the types: a bf16 ``x``
+    gives a bf16 result unless ``out_dtype`` says otherwise."""
     dev, dt = _check_layer_norm_fwd(x, weight, bias, out_dtype)
     if torch.is_grad_enabled() and (x.requires_grad or weight is not None and weight.requires_grad
                                     or bias is not None and bias.requires_grad):
@@ -844,7 +845,7 @@ def _embedding_fwd(dev, tokens, weight, scale, dt, plan, padding_idx):
     if n == 0:
         return out, torch.zeros(1, dtype=torch.int32, device=dev)
     bad = torch.empty(1, dtype=torch.int32, device=dev)
-    _lib.launch(dev, "spk_embedding_fwd", "embedding_fwd", n * (8 + D * (weight.itemsize + out.itemsize)),
+    _lib.launch(dev, "spk_embedding_fwd", "embedding_fwd", 1 if plan is None else 2, n * (8 + D * (weight.itemsize + out.itemsize)),
                 tokens.data_ptr(), weight.data_ptr(), _FLOATS[weight.dtype], ld, float(scale), n, V, D, out.data_ptr(),
                 _FLOATS[dt], bad.data_ptr(), padding_idx, None if plan is None else plan.data_ptr(),
                 0 if plan is None else plan.numel())
@@ -881,7 +882,7 @@ def _embedding_bwd(dev, g, tokens, plan, V, scale, padding_idx, dtype):
     gw = torch.empty((V, D), dtype=dtype, device=dev)
     wsb = _lib.load().spk_embedding_bwd_workspace_bytes(n, V, D)
     ws = torch.empty(wsb, dtype=torch.uint8, device=dev)
-    _lib.launch(dev, "spk_embedding_bwd", "embedding_bwd", n * (8 + D * g.itemsize) + V * D * gw.itemsize,
+    _lib.launch(dev, "spk_embedding_bwd", "embedding_bwd", 2 if tokens is None else 3, n * (8 + D * g.itemsize) + V * D * gw.itemsize,
                 None if tokens is None else tokens.data_ptr(), g.data_ptr(), _FLOATS[g.dtype], float(scale),
                 padding_idx, n, V, D, gw.data_ptr(), _FLOATS[dtype], plan.data_ptr(), plan.numel(), ws.data_ptr(), wsb)
     return gw
@@ -892,18 +893,41 @@ class _Embedding(torch.autograd.Function):
     def forward(ctx, weight, tokens, scale, padding_idx, dev, dt):
         plan = _embedding_plan(dev, tokens)
         out, bad = _embedding_fwd(dev, tokens, weight, scale, dt, plan, padding_idx)
-        ctx.save_for_backward(plan)
+        ctx.save_for_backward(plan, tokens)
         ctx.meta = dev, weight.shape[0], scale, padding_idx, weight.dtype
         ctx.mark_non_differentiable(bad)
         ctx.set_materialize_grads(False)
         return out, bad
 
-    @_backward
+    @staticmethod
     def backward(ctx, g, _g_bad):
         if g is None:
             return None, None, None, None, None, None
+        plan, tokens = ctx.saved_tensors
+        if torch.is_grad_enabled():
+            return _EmbeddingGrad.apply(g, plan, tokens, ctx.meta), None, None, None, None, None
         dev, V, scale, padding_idx, dtype = ctx.meta
-        return _embedding_bwd(dev, g, None, ctx.saved_tensors[0], V, scale, padding_idx, dtype), None, None, None, None, None
+        return _embedding_bwd(dev, g, None, plan, V, scale, padding_idx, dtype), None, None, None, None, None
+
+
+class _EmbeddingGrad(torch.autograd.Function):
+    """The weight's gradient as a function of ``g``; it is linear, and its own gradient
+    is the lookup (zeros for padding_idx)."""
+
+    @staticmethod
+    def forward(ctx, g, plan, tokens, meta):
+        dev, V, scale, padding_idx, dtype = meta
+        ctx.save_for_backward(tokens)
+        ctx.meta = scale, padding_idx, g.dtype
+        return _embedding_bwd(dev, g, None, plan, V, scale, padding_idx, dtype)
+
+    @staticmethod
+    def backward(ctx, gg):
+        scale, padding_idx, dtype = ctx.meta
+        tokens = ctx.saved_tensors[0]
+        if padding_idx >= 0:
+            tokens = torch.where(tokens == padding_idx, -1, tokens)
+        return embedding(tokens, gg, scale, out_dtype=dtype)[0], None, None, None
 
 
 def embedding(tokens, weight, scale=1.0, padding_idx=None, out_dtype=None):
@@ -953,7 +977,7 @@ def _token_logprobs_fwd(dev, logits, tokens, top_k, ignore_index, want_stats):
     wsb = _lib.load().spk_token_logprobs_workspace_bytes(T, rows, V, top_k)
     ws = torch.empty(wsb, dtype=torch.uint8, device=dev) if wsb else None
     ptr = _lib.ptr
-    _lib.launch(dev, "spk_token_logprobs_fwd", "token_logprobs_fwd", T * rows * V * logits.itemsize,
+    _lib.launch(dev, "spk_token_logprobs_fwd", "token_logprobs_fwd", 2 if wsb else 1, T * rows * V * logits.itemsize,
                 logits.data_ptr(), _FLOATS[logits.dtype], T, rows, V, st, sr, tokens.data_ptr(), ignore_index, top_k,
                 logp.data_ptr(), entropy.data_ptr(), ptr(top_logp), ptr(top_idx), ptr(stats), bad.data_ptr(), ptr(ws),
                 wsb)
@@ -985,7 +1009,7 @@ class _TokenLogprobs(torch.autograd.Function):
             x, st, sr = _logit_rows(logits)
             T, V = x.shape[0], x.shape[-1]
             ptr = _lib.ptr
-            _lib.launch(dev, "spk_token_logprobs_bwd", "token_logprobs_bwd", 2 * T * rows * V * x.itemsize,
+            _lib.launch(dev, "spk_token_logprobs_bwd", "token_logprobs_bwd", 1, 2 * T * rows * V * x.itemsize,
                         x.data_ptr(), _FLOATS[x.dtype], T, rows, V, st, sr, tokens.data_ptr(), ignore_index, top_k,
                         ptr(top_idx), stats.data_ptr(), ptr(g_logp), ptr(g_entropy), ptr(g_top), grad.data_ptr())
         return grad, None, None, None, None
@@ -1000,7 +1024,8 @@ def token_logprobs(logits, tokens, top_k=0, ignore_index=-100):
     top_logp [..., top_k], top_idx [..., top_k], bad)``, fp32 and int64,
     ``top_*`` None with ``top_k`` 0 (at most 32).  Alternatives come in falling
     order, ties to the lower index; a NaN counts as the smallest.  ``logp``,
-    ``entropy`` and ``top_logp`` are differentiable in the logits.  Positions
+    ``entropy`` and ``top_logp`` are differentiable in the logits (first
+    derivatives only).  Positions
     whose token is ``ignore_index`` give zeros (``top_idx`` -1) and take no
     gradient; so do tokens outside ``[0, V)``, which set the device flag
     ``bad``.  A row of logits that are all -inf has no distribution: NaN

@@ -118,7 +118,7 @@ def test_ops_refuse_what_they_do_not_take(ops):
 def test_second_derivatives_are_refused(ops):
     x = torch.randn(4, 8, device=DEV, requires_grad=True)
     t = torch.zeros(4, dtype=torch.int64, device=DEV)
-    for y in (ops.layer_norm(x), ops.embedding(t, x)[0], ops.token_logprobs(x[None], t)[0]):
+    for y in (ops.layer_norm(x), ops.token_logprobs(x[None], t)[0]):
         (g,) = torch.autograd.grad(y.square().sum(), x, create_graph=True)
         with pytest.raises(RuntimeError):
             g.sum().backward()
@@ -397,6 +397,22 @@ def test_embedding_gradient_against_differences(ops):
         step = torch.zeros_like(w)
         step[v, d] = 1.0
         assert float(got[v, d]) == float(f(w + step) - f(w))
+
+
+@pytest.mark.gpu
+def test_embedding_second_derivatives(ops):
+    """The gradient is linear in g: its own gradient is the lookup, without the padding
+    row (integers: equality with torch's)."""
+    tok = torch.randint(0, 7, (5, 6), generator=gen(1)).to(DEV)
+    w = torch.randint(-4, 5, (7, 12), generator=gen(2)).float().to(DEV).requires_grad_(True)
+    v = torch.randint(-4, 5, (7, 12), generator=gen(3)).float().to(DEV)
+    res = []
+    for f in (lambda: ops.embedding(tok, w, 2.0, padding_idx=3)[0],
+              lambda: torch.nn.functional.embedding(tok, w, padding_idx=3) * 2.0):
+        (gw,) = torch.autograd.grad(f().pow(2).sum(), w, create_graph=True)
+        (gg,) = torch.autograd.grad((gw * v).sum(), w)
+        res.append((gw.detach(), gg))
+    assert torch.equal(res[0][0], res[1][0]) and torch.equal(res[0][1], res[1][1])
 
 
 @pytest.mark.gpu
@@ -768,7 +784,12 @@ def test_token_embedding_module_matches_the_lookup(ops):
     # 68 tokens: each way sums a row's few terms (one scales before, one after) within (c + 2) u of their size
     size = torch.zeros(50, 96, device=DEV).index_add_(0, tok.flatten(), g.abs().flatten(0, 1)) * 96 ** 0.5
     assert ((gw - rw).abs() <= 2 * (68 + 2) * U * size).all()
-    assert torch.equal(m(tok.int()), ref) and torch.equal(m.half()(tok), (m.embedding.weight[tok].float() * 96 ** 0.5).half())
+    assert torch.equal(m(tok.int()), ref) and torch.equal(m(tok.float()), ref)
+    seen = []
+    hook = m.embedding.register_forward_hook(lambda *a: seen.append(1))
+    assert torch.equal(m(tok), ref) and seen
+    hook.remove()
+    assert torch.equal(m.half()(tok), (m.embedding.weight[tok].float() * 96 ** 0.5).half())
     m.float().embedding.padding_idx = 3
     (gw,) = torch.autograd.grad(m(tok), m.embedding.weight, g)
     assert not gw[3].any()
@@ -913,6 +934,64 @@ def test_operators_in_two_cuda_graphs(ops):
     for s, graph, outs in made:
         for a, b in zip(outs, step(s)):
             assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_offsets_beyond_32_bits(ops):
+    """Tensors of more than 2^31 elements: the last rows equal those of a small call."""
+    D, rows = 2048, (1 << 20) + 4096
+    x = torch.empty(rows, D, dtype=torch.bfloat16, device=DEV).normal_()
+    w = torch.randn(D, device=DEV)
+    y, stats = ops.layer_norm_fwd(x, w)
+    assert torch.equal(y[-64:], ops.layer_norm(x[-64:], w))
+    gx, _, _ = ops.layer_norm_bwd(x, x, stats, w, need_weight=False, need_bias=False)
+    assert torch.equal(gx[-64:], ops.layer_norm_bwd(x[-64:], x[-64:], stats[-64:], w)[0])
+    del y, gx
+    tok = torch.tensor([0, rows - 1, rows - 1, 1 << 20, 7], device=DEV)
+    out, bad = ops.embedding(tok, x)
+    assert int(bad) == 0 and torch.equal(out, x[tok])
+    g = torch.randint(-9, 10, (5, D), device=DEV).to(torch.bfloat16)
+    gw = ops.embedding_bwd(g, tok, rows, dtype=torch.bfloat16)
+    assert torch.equal(gw[rows - 1], g[1] + g[2]) and torch.equal(gw[0], g[0]) and torch.equal(gw[1 << 20], g[3])
+    assert not gw[rows - 2].any() and float(gw[-4000:].float().abs().sum()) == float((g[1] + g[2]).float().abs().sum())
+    del gw
+    big = torch.randint(0, rows, (rows,), device=DEV)
+    out, _ = ops.embedding(big, x[:, :D])
+    assert torch.equal(out[-1000:], x[big[-1000:]])
+    del out, big
+    V = 65536
+    z = x.flatten()[: (1 << 15) * V + 64 * V].view(1, -1, V)
+    t = torch.randint(0, V, (z.shape[1],), device=DEV)
+    logp, H, top, idx, _ = ops.token_logprobs(z, t, top_k=2)
+    last = ops.token_logprobs(z[:, -64:], t[-64:], top_k=2)
+    # 64 rows are cut over several blocks and join their sums in another order
+    for a, b in zip((logp, H, top), last):
+        assert torch.allclose(a[-64:], b, rtol=0, atol=2e-5)
+    assert torch.equal(idx[-64:], last[3])
+    zl = z.detach().requires_grad_(True)
+    (gz,) = torch.autograd.grad(ops.token_logprobs(zl, t)[0].sum(), zl)
+    p = z[0, -1].float().softmax(-1)
+    p[t[-1]] -= 1.0
+    assert torch.allclose(gz[0, -1].float(), -p, rtol=2 ** -7, atol=1e-8)
+
+
+@pytest.mark.gpu
+def test_operators_run_beside_each_other(ops):
+    """The same calls at once on two streams, each with its own buffers."""
+    a, b = chain_inputs(21), chain_inputs(22)
+    want = [torch.autograd.grad(chain(ops, s[0], s[1], *s[2])[0].sum(), s[2]) for s in (a, b)]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(5):
+        for i, s in enumerate((a, b)):
+            with torch.cuda.stream(streams[i]):
+                ps = [p.detach().requires_grad_(True) for p in s[2]]
+                got[i].append(torch.autograd.grad(chain(ops, s[0], s[1], *ps)[0].sum(), ps))
+    torch.cuda.synchronize()
+    for w, runs in zip(want, got):
+        for r in runs:
+            assert all(torch.equal(u, v) for u, v in zip(w, r))
 
 
 @pytest.mark.gpu
