@@ -29,8 +29,59 @@ namespace embg {
 // rows that a warp has in flight
 constexpr int kDeep = 8;
 
-// A warp per (kDeep tokens, tile of 32 * VEC columns): the tokens are read
-// together, then their rows, then written.
+// Columns of a lane in a tile: one vector, or kSingle single elements 32 apart.
+constexpr int kSingle = 4;
+constexpr int cols_of(int vec) { return vec > 1 ? vec : kSingle; }
+template <int VEC>
+struct Columns {
+  static constexpr int N = cols_of(VEC);
+  int base, D;
+  __device__ __forceinline__ Columns(int64_t tile, int lane, int d)
+      : base((int)tile * 32 * N + lane * (VEC > 1 ? VEC : 1)), D(d) {}
+  __device__ __forceinline__ int at(int i) const { return VEC > 1 ? base + i : base + 32 * i; }
+  __device__ __forceinline__ bool any() const { return base < D; }
+  __device__ __forceinline__ bool on(int i) const { return VEC > 1 ? base < D : at(i) < D; }
+};
+// a lane's values of a row as they lie in memory
+template <int DT, int VEC>
+struct Raw {
+  using E = typename Elem<DT>::T;
+  using C = Columns<VEC>;
+  typename Vec<DT, VEC>::W w[VEC > 1 ? 1 : kSingle];
+  __device__ __forceinline__ void load(const E* row, const C& c) {
+    if constexpr (VEC > 1) {
+      w[0] = Vec<DT, VEC>::raw(row + c.base);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kSingle; ++i)
+        if (c.on(i)) w[i] = Vec<DT, 1>::raw(row + c.at(i));
+    }
+  }
+  __device__ __forceinline__ void unpack(float (&v)[C::N]) const {
+    if constexpr (VEC > 1) {
+      Vec<DT, VEC>::unpack(w[0], v);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kSingle; ++i) {
+        float one[1];
+        Vec<DT, 1>::unpack(w[i], one);
+        v[i] = one[0];
+      }
+    }
+  }
+  __device__ __forceinline__ static void store(E* row, const C& c, const float (&v)[C::N]) {
+    if constexpr (VEC > 1) {
+      Vec<DT, VEC>::store(row + c.base, v);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kSingle; ++i)
+        if (c.on(i)) row[c.at(i)] = Elem<DT>::make(v[i]);
+    }
+  }
+};
+
+// A warp per (kDeep tokens, tile of columns): the tokens are read together, then
+// their rows, then written.
 template <int WDT, int ODT, int VEC>
 __global__ void __launch_bounds__(256, 4) gather_kernel(const int64_t* __restrict__ tokens,
                                                      const typename Elem<WDT>::T* __restrict__ w, int64_t ldw,
@@ -52,7 +103,7 @@ __global__ void __launch_bounds__(256, 4) gather_kernel(const int64_t* __restric
   const int lane = threadIdx.x & 31;
   const int64_t item = ((int64_t)blockIdx.x - scan_bad) * 8 + (threadIdx.x >> 5);
   const int64_t group = item / tiles;
-  const int col = (int)(item - group * tiles) * 32 * VEC + lane * VEC;
+  const Columns<VEC> col(item - group * tiles, lane, D);
   const int64_t i0 = group * kDeep;
   if (i0 >= n) return;
   int64_t tok = -1;
@@ -63,25 +114,25 @@ __global__ void __launch_bounds__(256, 4) gather_kernel(const int64_t* __restric
       if (!scan_bad) atomicExch(bad, 1);
     }
   }
-  typename Vec<WDT, VEC>::W x[kDeep];
+  Raw<WDT, VEC> x[kDeep];
   unsigned in = 0;  // rows that are inside the vocabulary
 #pragma unroll
   for (int k = 0; k < kDeep; ++k) {
     const int64_t t = __shfl_sync(0xffffffffu, tok, k);
-    if (t >= 0 && col < D) {
+    if (t >= 0 && col.any()) {
       in |= 1u << k;
-      x[k] = Vec<WDT, VEC>::raw(w + t * ldw + col);
+      x[k].load(w + t * ldw, col);
     }
   }
-  if (col >= D) return;
+  if (!col.any()) return;
 #pragma unroll
   for (int k = 0; k < kDeep; ++k) {
     if (i0 + k >= n) break;
-    float v[VEC];
-    Vec<WDT, VEC>::unpack(x[k], v);
+    float v[Columns<VEC>::N];
+    x[k].unpack(v);
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) v[j] = (in >> k) & 1u ? v[j] * scale : 0.0f;
-    Vec<ODT, VEC>::store(out + (i0 + k) * D + col, v);
+    for (int j = 0; j < Columns<VEC>::N; ++j) v[j] = (in >> k) & 1u ? v[j] * scale : 0.0f;
+    Raw<ODT, VEC>::store(out + (i0 + k) * D, col, v);
   }
 }
 
@@ -254,7 +305,7 @@ __device__ __forceinline__ void clear_rows(const uint2* __restrict__ items, int6
   }
 }
 
-// A warp per (chunk of sorted positions, tile of 32 * VEC columns).  With
+// A warp per (chunk of sorted positions, tile of columns).  With
 // VEC > 1 a lane's vectors of the next kRing rows are on their way into a
 // ring of its own in shared memory (a lane reads back only what it copied
 // itself, so the ring needs no barrier); single elements, which asynchronous
@@ -279,17 +330,18 @@ __global__ void __launch_bounds__(256) sum_kernel(const uint2* __restrict__ item
   const int64_t item = blockIdx.x * (int64_t)8 + (threadIdx.x >> 5);
   if (item >= chunks * tiles) return;
   const int64_t c = item / tiles;
-  const int col = (int)(item - c * tiles) * 32 * VEC + lane * VEC;
-  const bool on = col < D;
+  constexpr int N = Columns<VEC>::N;
+  const Columns<VEC> col(item - c * tiles, lane, D);
+  const bool on = col.any();
   const int64_t lo = c * chunk, hi = lo + chunk < n ? lo + chunk : n;
   const int m = (int)(hi - lo);
   const uint32_t before = lo > 0 ? items[lo - 1].x : 0xffffffffu;
   const uint32_t after = hi < n ? items[hi].x : 0xffffffffu;
   uint32_t cur = items[lo].x;
   bool first = true;  // the chunk's first token is being added
-  float acc[VEC];
+  float acc[N];
 #pragma unroll
-  for (int j = 0; j < VEC; ++j) acc[j] = 0.0f;
+  for (int j = 0; j < N; ++j) acc[j] = 0.0f;
   // the sum so far belongs to token `cur`: to the gradient, or to the parts
   auto flush = [&](bool last) {
     if (cur >= V || !on) return;
@@ -298,29 +350,30 @@ __global__ void __launch_bounds__(256) sum_kernel(const uint2* __restrict__ item
     if (head || tail) {
       // [chunk][0]: the part of a token that comes from the chunk before (and may go on),
       // [chunk][1]: of one that begins here and goes on
-      float* q = part + (c * 2 + (head ? 0 : 1)) * D + col;
+      float* q = part + (c * 2 + (head ? 0 : 1)) * D;
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) q[j] = acc[j];
+      for (int j = 0; j < N; ++j)
+        if (col.on(j)) q[col.at(j)] = acc[j];
     } else {
-      float v[VEC];
+      float v[N];
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) v[j] = acc[j] * scale;
-      Vec<WDT, VEC>::store(gw + (int64_t)cur * D + col, v);
+      for (int j = 0; j < N; ++j) v[j] = acc[j] * scale;
+      Raw<WDT, VEC>::store(gw + (int64_t)cur * D, col, v);
     }
   };
-  auto take = [&](uint32_t k, const W& x) {
+  auto take = [&](uint32_t k, const Raw<GDT, VEC>& x) {
     if (k != cur) {
       flush(false);
       cur = k;
       first = false;
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) acc[i] = 0.0f;
+      for (int i = 0; i < N; ++i) acc[i] = 0.0f;
     }
     if (k < V) {
-      float v[VEC];
-      Vec<GDT, VEC>::unpack(x, v);
+      float v[N];
+      x.unpack(v);
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) acc[i] += v[i];
+      for (int i = 0; i < N; ++i) acc[i] += v[i];
     }
   };
   // the items of the group of 32 that is added, and of the next one
@@ -338,7 +391,7 @@ __global__ void __launch_bounds__(256) sum_kernel(const uint2* __restrict__ item
         const uint32_t k = __shfl_sync(0xffffffffu, in_b ? b.x : a.x, r);
         const uint32_t q = __shfl_sync(0xffffffffu, in_b ? b.y : a.y, r);
         if (on && k < V)
-          copy_async(ring_at + ((j + i) & (kRing - 1)) * 32 * (int)sizeof(W), g + (int64_t)q * D + col,
+          copy_async(ring_at + ((j + i) & (kRing - 1)) * 32 * (int)sizeof(W), g + (int64_t)q * D + col.base,
                      sizeof(W) == 16);
       }
       asm volatile("cp.async.commit_group;" ::: "memory");
@@ -352,7 +405,11 @@ __global__ void __launch_bounds__(256) sum_kernel(const uint2* __restrict__ item
 #pragma unroll
         for (int i = 0; i < kStep; ++i) {
           const uint32_t k = __shfl_sync(0xffffffffu, a.x, j + i);
-          if (j0 + j + i < m) take(k, ring[((j + i) & (kRing - 1)) * 32]);
+          if (j0 + j + i < m) {
+            Raw<GDT, VEC> x;
+            x.w[0] = ring[((j + i) & (kRing - 1)) * 32];
+            take(k, x);
+          }
         }
         issue(j + kRing);
       }
@@ -363,11 +420,11 @@ __global__ void __launch_bounds__(256) sum_kernel(const uint2* __restrict__ item
   } else {
     for (int j0 = 0; j0 < m; j0 += 32) {
       for (int j = 0; j < 32 && j0 + j < m; j += kDeep) {
-        W x[kDeep];
+        Raw<GDT, VEC> x[kDeep];
 #pragma unroll
         for (int i = 0; i < kDeep; ++i) {
           const uint32_t k = __shfl_sync(0xffffffffu, a.x, j + i), q = __shfl_sync(0xffffffffu, a.y, j + i);
-          if (on && k < V) x[i] = Vec<GDT, VEC>::raw(g + (int64_t)q * D + col);
+          if (on && k < V) x[i].load(g + (int64_t)q * D, col);
         }
 #pragma unroll
         for (int i = 0; i < kDeep; ++i) {
@@ -460,12 +517,12 @@ inline int64_t align16(int64_t b) { return (b + 15) / 16 * 16; }
 struct Plan {
   int bits, passes, chunk, tiles;
   int64_t chunks, items;  // items: bytes of one of the two arrays of (key, position)
-  Plan(int64_t n, int64_t V, int64_t D, int vec) {
+  Plan(int64_t n, int64_t V, int64_t D, int cols) {  // cols: columns of a lane in a tile
     int b = 1;
     while ((V >> b) != 0) ++b;  // keys 0 .. V
     passes = (b + kMaxDigit - 1) / kMaxDigit;
     bits = (b + passes - 1) / passes;
-    tiles = (int)((D + 32 * vec - 1) / (32 * vec));
+    tiles = (int)((D + 32 * cols - 1) / (32 * cols));
     const int64_t warps = (int64_t)num_sms() * 24;
     int64_t ch = ((n * tiles + warps - 1) / warps + 15) / 16 * 16;
     chunk = (int)(ch < 16 ? 16 : ch > 1024 ? 1024 : ch);
@@ -504,7 +561,7 @@ int launch_bwd(const Plan& pl, const uint2* items, const void* g, float scale, i
   return check_launch("embedding_bwd");
 }
 
-// elements of an access: 16 bytes of the wider type where the layout allows
+// elements of an access: 16 bytes of the wider type where the layout allows, else one
 inline int bwd_vec(const void* g, int g_dtype, const void* gw, int w_dtype, int64_t D) {
   const int v = g_dtype == SPK_F32 || w_dtype == SPK_F32 ? 4 : 8;
   return D % v == 0 && aligned(g, v * dtype_size(g_dtype)) && aligned(gw, v * dtype_size(w_dtype)) ? v : 1;
@@ -544,7 +601,7 @@ int launch_gather(const int64_t* tokens, const void* w, int64_t ldw, float scale
   constexpr int kWide = WDT == SPK_F32 || ODT == SPK_F32 ? 4 : 8;
   const bool wide = D % kWide == 0 && ldw % kWide == 0 && aligned(w, kWide * dtype_size(WDT)) &&
                     aligned(out, kWide * dtype_size(ODT));
-  const int tiles = (D + 32 * (wide ? kWide : 1) - 1) / (32 * (wide ? kWide : 1));
+  const int cols = 32 * cols_of(wide ? kWide : 1), tiles = (D + cols - 1) / cols;
   const int scan = n <= kScanTokens ? 1 : 0;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(((n + kDeep - 1) / kDeep * tiles + 7) / 8 + scan));
@@ -630,7 +687,7 @@ int spk_embedding_bwd(const int64_t* tokens, const void* g, int g_dtype, float s
   if (rc != SPK_OK) return rc;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const int vec = bwd_vec(g, g_dtype, gw, w_dtype, D);
-  const Plan pl(n, V, D, vec);
+  const Plan pl(n, V, D, cols_of(vec));
   if (tokens) {
     rc = launch_sort(pl, tokens, n, V, padding_idx, plan, st);
     if (rc != SPK_OK) return rc;

@@ -615,8 +615,9 @@ __device__ __forceinline__ void write_unused(int64_t r, int K, int lane, const O
   }
 }
 
-// Values of a row that one warp takes, where there are rows for 16 warps on every SM.
-constexpr int kWarpRow = 1024;
+// Values of a row that one warp takes, where there are rows for 16 warps on every
+// SM, and for 64.
+constexpr int kWarpRow = 1024, kManyRow = 8192;
 
 // GT = 32: a warp a row.  GT = 256: a block a (row, split); with several splits
 // the state and list go to part / keys.
@@ -851,13 +852,16 @@ __global__ void __launch_bounds__(256) bwd_kernel(Logits x, const int64_t* __res
 
 // blocks that a row is cut over, so that there are two for every SM
 inline int splits_of(int64_t rows, int64_t V) {
-  if (V <= kWarpRow * 4) return 1;
+  if (V <= kWarpRow * 4 || rows >= 2 * (int64_t)num_sms()) return 1;
   int64_t s = (2 * (int64_t)num_sms() + rows - 1) / rows;
   const int64_t most = V / 2048;
   if (s > most) s = most;
   return (int)(s > 32 ? 32 : s < 1 ? 1 : s);
 }
-inline bool warp_rows(int64_t rows, int64_t V) { return V <= kWarpRow && (V <= 256 || rows >= 16 * (int64_t)num_sms()); }
+inline bool warp_rows(int64_t rows, int64_t V) {
+  return V <= 256 || (V <= kWarpRow && rows >= 16 * (int64_t)num_sms()) ||
+         (V <= kManyRow && rows >= 64 * (int64_t)num_sms());
+}
 
 // 48 KB of dynamic shared memory without asking, the kernel's static arrays included
 template <typename K>
