@@ -86,22 +86,17 @@ template <int WDT, int ODT, int VEC>
 __global__ void __launch_bounds__(256, 4) gather_kernel(const int64_t* __restrict__ tokens,
                                                      const typename Elem<WDT>::T* __restrict__ w, int64_t ldw,
                                                      float scale, int64_t n, int64_t V, int D, int tiles,
-                                                     typename Elem<ODT>::T* __restrict__ out, int* bad, int scan_bad,
-                                                     int after_sort) {
-  // The sort before this kernel may still be running: the last block does not end before it,
-  // so whoever comes after this kernel finds the sort done.
-  struct AtEnd {
-    bool on;
-    __device__ ~AtEnd() {
-      if (on) pdl_wait();
-    }
-  } at_end{after_sort && blockIdx.x == gridDim.x - 1};
-  if (scan_bad && blockIdx.x == 0) {  // the first block, so that it is not the last to end
-    scan_tokens(tokens, n, V, 0, bad);
+                                                     typename Elem<ODT>::T* __restrict__ out, int* bad, int extra,
+                                                     int scan_bad, int after_sort) {
+  if (extra && blockIdx.x == 0) {  // the first block, so that it is not the last to end
+    if (scan_bad) scan_tokens(tokens, n, V, 0, bad);
+    // The sort before this kernel may still be running: this block does not end before it, so
+    // whoever comes after this kernel finds the sort done.
+    if (after_sort) pdl_wait();
     return;
   }
   const int lane = threadIdx.x & 31;
-  const int64_t item = ((int64_t)blockIdx.x - scan_bad) * 8 + (threadIdx.x >> 5);
+  const int64_t item = ((int64_t)blockIdx.x - extra) * 8 + (threadIdx.x >> 5);
   const int64_t group = item / tiles;
   const Columns<VEC> col(item - group * tiles, lane, D);
   const int64_t i0 = group * kDeep;
@@ -602,9 +597,9 @@ int launch_gather(const int64_t* tokens, const void* w, int64_t ldw, float scale
   const bool wide = D % kWide == 0 && ldw % kWide == 0 && aligned(w, kWide * dtype_size(WDT)) &&
                     aligned(out, kWide * dtype_size(ODT));
   const int cols = 32 * cols_of(wide ? kWide : 1), tiles = (D + cols - 1) / cols;
-  const int scan = n <= kScanTokens ? 1 : 0;
+  const int scan = n <= kScanTokens ? 1 : 0, extra = scan || after_sort ? 1 : 0;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(((n + kDeep - 1) / kDeep * tiles + 7) / 8 + scan));
+  cfg.gridDim = dim3((unsigned)(((n + kDeep - 1) / kDeep * tiles + 7) / 8 + extra));
   cfg.blockDim = dim3(256);
   cfg.stream = st;
   cudaLaunchAttribute at[1];
@@ -612,7 +607,7 @@ int launch_gather(const int64_t* tokens, const void* w, int64_t ldw, float scale
   const cudaError_t e = cudaLaunchKernelEx(
       &cfg, wide ? gather_kernel<WDT, ODT, kWide> : gather_kernel<WDT, ODT, 1>, tokens,
       reinterpret_cast<const typename Elem<WDT>::T*>(w), ldw, scale, n, V, D, tiles,
-      reinterpret_cast<typename Elem<ODT>::T*>(out), bad, scan, after_sort ? 1 : 0);
+      reinterpret_cast<typename Elem<ODT>::T*>(out), bad, extra, scan, after_sort ? 1 : 0);
   return e == cudaSuccess ? check_launch("embedding_fwd") : fail(SPK_ERR_LAUNCH, "embedding_fwd: %s", cudaGetErrorString(e));
 }
 
