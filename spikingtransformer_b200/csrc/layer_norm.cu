@@ -273,7 +273,7 @@ struct Bwd {
 };
 
 template <int XDT, int VEC, int NV>
-__global__ void __launch_bounds__(32 * kMaxGroup) fwd_kernel(const typename Elem<XDT>::T* __restrict__ x, int64_t ld,
+__global__ void __launch_bounds__(NV == 8 ? 32 * kWarps : 32 * kMaxGroup) fwd_kernel(const typename Elem<XDT>::T* __restrict__ x, int64_t ld,
                                                              const void* w, int wdt, const void* b, int bdt, float eps,
                                                              int64_t rows, int D, int wpr, int lpr, void* __restrict__ y,
                                                              int ydt, float2* __restrict__ stats) {
@@ -528,19 +528,23 @@ __global__ void __launch_bounds__(kLong) long_bwd_w_kernel(const void* g, int gd
 
 // ---------------------------------------------------------------- which kernel, how many blocks
 
-// vectors a lane holds at most, forward and backward; single elements: the second
-// number only where 16 warps of the first do not hold the row (it spills)
-constexpr int kNvFwd = 6, kNvBwd = 4, kNv1Fwd = 12, kNv1Bwd = 10, kNv1FwdLast = 24, kNv1BwdLast = 16;
+// Vectors (single elements) that a lane holds at most, forward and backward: the
+// more, the fewer warps meet for a row (65536 x 1536 bf16 forward: 80 us with 6
+// vectors and 2 warps, 94 us with 3 and 4; 65536 x 1024: 57 us with 8 and one
+// warp, 68 us with 4 and 2; backward 80 us with 4 and 2, 107 us with 2 and 4).
+// The `Last` number where 16 warps are needed.
+constexpr int kNvFwd = 8, kNvFwdLast = 6, kNvBwd = 4, kNvBwdLast = 4;
+constexpr int kNv1Fwd = 12, kNv1FwdLast = 24, kNv1Bwd = 10, kNv1BwdLast = 16;
 
 struct Shape {
   int vec, nv, wpr, lpr = 32;  // nv = 0: the row does not fit the registers
-  Shape(int64_t D, bool wide, int most4, int most1, int last1) {
+  Shape(int64_t D, bool wide, int most4, int last4, int most1, int last1) {
     vec = wide ? 4 : 1;
     const int most = wide ? most4 : most1;
     const int64_t vecs = (D + vec - 1) / vec;
     for (wpr = 1; wpr < kMaxGroup && vecs > 32ll * wpr * most; wpr *= 2) {}
     const int64_t n = (vecs + 32 * wpr - 1) / (32 * wpr);
-    nv = n > (wide ? most4 : last1) ? 0 : (int)n;
+    nv = n > (wide ? (wpr > kWarps ? last4 : most4) : last1) ? 0 : (int)n;
     if (wide && vecs <= 16) lpr = vecs <= 8 ? 8 : 16;
   }
   int threads() const { return 32 * (wpr > kWarps ? wpr : kWarps); }
@@ -620,7 +624,9 @@ bool dispatch_fwd(const void* x, int64_t ld, const void* w, int wdt, const void*
       case 2: return GO(4, 2);
       case 3: return GO(4, 3);
       case 4: return GO(4, 4);
-      default: return GO(4, 6);
+      case 5:
+      case 6: return GO(4, 6);
+      default: return GO(4, 8);
     }
   }
   return s.nv <= 4 ? GO(1, 4) : s.nv <= 6 ? GO(1, 6) : s.nv <= 10 ? GO(1, 10) : s.nv <= 12 ? GO(1, 12) : GO(1, 24);
@@ -662,7 +668,7 @@ int spk_layer_norm_fwd(const void* x, int x_dtype, int64_t ld, const void* w, in
   if (rc != SPK_OK) return rc;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const bool wide = D % 4 == 0 && ld % 4 == 0 && aligned(x, 4 * dtype_size(x_dtype)) && aligned(y, 4 * dtype_size(y_dtype));
-  const Shape s(D, wide, kNvFwd, kNv1Fwd, kNv1FwdLast);
+  const Shape s(D, wide, kNvFwd, kNvFwdLast, kNv1Fwd, kNv1FwdLast);
   auto go = x_dtype == SPK_F32 ? dispatch_fwd<SPK_F32> : x_dtype == SPK_F16 ? dispatch_fwd<SPK_F16> : dispatch_fwd<SPK_BF16>;
   if (!go(x, ld, w, w_dtype, b, b_dtype, eps, rows, D, s, y, y_dtype, stats, st)) {
     const int64_t cap = (int64_t)num_sms() * 4;
@@ -698,7 +704,7 @@ int spk_layer_norm_bwd(const void* g, int g_dtype, const void* x, int x_dtype, i
   float* part = gw || gb ? reinterpret_cast<float*>(workspace) : nullptr;
   const bool wide = D % 4 == 0 && ld % 4 == 0 && aligned(x, 4 * dtype_size(x_dtype)) &&
                     aligned(g, 4 * dtype_size(g_dtype)) && aligned(gx, 4 * dtype_size(x_dtype));
-  const Shape s(D, wide, kNvBwd, kNv1Bwd, kNv1BwdLast);
+  const Shape s(D, wide, kNvBwd, kNvBwdLast, kNv1Bwd, kNv1BwdLast);
   int parts;
   if (s.nv > 0) {
 #define GO(G, X) dispatch_bwd<G, X>(g, x, ld, stats, w, w_dtype, rows, D, s, gx, part, st)
