@@ -49,6 +49,16 @@
  *   spk_attn_masked_train_fwd / _bwd
  *                          the decoder's masked self-attention core in
  *                          training, SSA.py:234-242 and its autograd
+ *   spk_layer_norm_fwd / _bwd
+ *                          nn.LayerNorm on its own (SSA.py:218-249,
+ *                          SpikingMLP.py:31-36) and its autograd
+ *   spk_embedding_fwd / _bwd
+ *                          TokenEmbedding, Seq2Seq.py:29-36, and the gradient
+ *                          of its weight
+ *   spk_token_logprobs_fwd / _bwd
+ *                          scores of the distribution that greedy_decode takes
+ *                          its argmax of (T-averaged logits, Seq2Seq.py:136-162);
+ *                          no reference counterpart of its own
  *   spk_ce_over_t          the training loss and token accuracy,
  *                          train_spikeformer.py:309-323 (step_loss with
  *                          CrossEntropyLoss(ignore_index, label_smoothing),

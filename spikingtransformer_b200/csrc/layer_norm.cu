@@ -272,6 +272,7 @@ struct Bwd {
   using G = Rows<GDT, VEC, NV, S>;
 };
 
+// 262144 x 384 bf16: 76 us, 5.3 TB/s (0.82 of a plain copy); 65536 x 1536: 77 us.
 template <int XDT, int VEC, int NV>
 __global__ void __launch_bounds__(NV == 8 ? 32 * kWarps : 32 * kMaxGroup) fwd_kernel(const typename Elem<XDT>::T* __restrict__ x, int64_t ld,
                                                              const void* w, int wdt, const void* b, int bdt, float eps,
@@ -333,7 +334,8 @@ __global__ void __launch_bounds__(NV == 8 ? 32 * kWarps : 32 * kMaxGroup) fwd_ke
   wait_copies<0>();
 }
 
-// part[block][2][D]: (sum g * h, sum g) over the block's rows
+// part[block][2][D]: (sum g * h, sum g) over the block's rows.  65536 x 1536 bf16:
+// 107 us, 5.6 TB/s.
 template <int GDT, int XDT, int VEC, int NV>
 __global__ void __launch_bounds__(32 * kMaxGroup) bwd_kernel(const typename Elem<GDT>::T* __restrict__ g,
                                                              const typename Elem<XDT>::T* __restrict__ x, int64_t ld,

@@ -619,6 +619,10 @@ __device__ __forceinline__ void write_unused(int64_t r, int K, int lane, const O
 // SM, and for 64.
 constexpr int kWarpRow = 1024, kManyRow = 8192;
 
+// Without alternatives bound by instructions more than by HBM: 8192 x 65536 bf16
+// (1.07 GB) take 213 us, 0.78 of a plain copy's rate, at 80 % of the issue slots;
+// with 5 alternatives 389 us, with 32 537 us.  16384 x 256 fp32 of 4 steps: 27 us,
+// with 5 alternatives 37 us, where a row's reductions cost more than its values.
 // GT = 32: a warp a row.  GT = 256: a block a (row, split); with several splits
 // the state and list go to part / keys.
 template <int DT, int VEC, int U, int GT, bool TOP>
@@ -748,7 +752,8 @@ struct Grads {
   const float4* stats;
 };
 
-// dz_j = 2^t_j (a t_j + b), and g_logp, g_top added at their symbols
+// dz_j = 2^t_j (a t_j + b), and g_logp, g_top added at their symbols.  Bound by
+// HBM: 8192 x 65536 bf16, read and written, take 320 us, 6.7 TB/s.
 template <int DT, int VEC, int U, int GT>
 __global__ void __launch_bounds__(256) bwd_kernel(Logits x, const int64_t* __restrict__ tokens, int64_t ignore, int K,
                                                   int splits, Grads g, typename Elem<DT>::T* __restrict__ grad) {

@@ -1,6 +1,6 @@
 """Kernel micro-benchmarks at the benchmark shapes (CUDA events, device time).
 
-    python -m spikingtransformer_b200.kbench [--only lif|gemm|ssa|ssa_model|data|shapes|lnlif] [--iters N]
+    python -m spikingtransformer_b200.kbench [--only lif|gemm|ssa|ssa_model|data|shapes|lnlif|token] [--iters N]
 
   lif   LIF forward on [T=4, 64*256, 1536] fp32 input -> bf16 and packed-bit
         spikes (the MLP expansion LIF of a 64-image batch), and the backward
@@ -21,6 +21,11 @@
   ssa_model  the forward's three attention calls at the bench batch (256
         images): encoder self 256 x 256, decoder cross 64 x 256, decoder
         self 64 x 64 with the dense look-ahead mask; bound: HBM bytes.
+  token the token-side operators: LayerNorm forward and backward [65536, 1536]
+        bf16, the embedding of 131072 long-tailed tokens (V 65536, D 1024, bf16)
+        with its gradient, token log probabilities of [1, 8192, 65536] bf16
+        (plain, with 5 alternatives, with the gradient) and of the scoring shape
+        [4, 16384, 256] fp32; bound: HBM bytes.
 Inputs are regenerated per configuration; each timed iteration rotates over
 input copies whose total exceeds the 126 MB L2.  Prints one JSON line.
 """
@@ -339,11 +344,60 @@ def bench_lnlif(iters, R=16384, T=4):
     return res
 
 
+def bench_token(iters):
+    """The token-side operators (LayerNorm, embedding, token log probabilities);
+    bytes: each input read once, each output written once."""
+    out, bf16 = [], torch.bfloat16
+
+    def add(kernel, shape, ms, nbytes):
+        out.append({"kernel": kernel, "shape": list(shape), "ms": ms, "GB/s": nbytes / ms / 1e6, "bytes": nbytes})
+
+    rows, D = 65536, 1536  # 201 MB: larger than L2
+    x, g = (torch.randn(rows, D, device="cuda").to(bf16) for _ in range(2))
+    w, b = torch.randn(D, device="cuda"), torch.randn(D, device="cuda")
+    _, stats = ops.layer_norm_fwd(x, w, b)
+    n = rows * D * 2
+    add("layer_norm_fwd", (rows, D), _time(lambda i: ops.layer_norm(x, w, b), iters), 2 * n)
+    add("layer_norm_bwd", (rows, D), _time(lambda i: ops.layer_norm_bwd(g, x, stats, w), iters), 3 * n)
+    del x, g
+    n, V, D = 131072, 65536, 1024
+    tok = torch.randperm(V, device="cuda")[(torch.rand(n, device="cuda") ** 4 * V).long().clamp(max=V - 1)]
+    weight = torch.randn(V, D, device="cuda").to(bf16)
+    g = torch.randn(n, D, device="cuda").to(bf16)
+    used = int(torch.unique(tok).numel())
+    add("embedding_fwd", (n, V, D), _time(lambda i: ops.embedding(tok, weight, 32.0), iters), 8 * n + 2 * D * (n + used))
+    add("embedding_bwd", (n, V, D), _time(lambda i: ops.embedding_bwd(g, tok, V, 32.0, dtype=bf16), iters),
+        8 * n + 2 * D * (n + V))
+    weight.requires_grad_(True)
+
+    def train(i):
+        torch.autograd.grad(ops.embedding(tok, weight, 32.0)[0], weight, g)
+    add("embedding (+backward)", (n, V, D), _time(train, iters), 8 * n + 2 * D * (2 * n + used + V))
+    del weight, g
+    logits = torch.randn(1, 8192, 65536, device="cuda", dtype=bf16).mul_(3.0)
+    tgt = torch.randint(0, 65536, (8192,), device="cuda")
+    n = logits.numel() * 2
+    for k in (0, 5):
+        add("token_logprobs top_k=%d" % k, logits.shape, _time(lambda i: ops.token_logprobs(logits, tgt, top_k=k), iters), n)
+    logits.requires_grad_(True)
+
+    def step(i):
+        logp, entropy = ops.token_logprobs(logits, tgt)[:2]
+        torch.autograd.grad((logp.sum(), entropy.sum()), logits)
+    add("token_logprobs (+backward)", logits.shape, _time(step, iters), 3 * n)
+    del logits
+    logits = [torch.randn(4, 16384, 256, device="cuda") for _ in range(3)]  # 3 x 67 MB
+    tgt = torch.randint(0, 256, (16384,), device="cuda")
+    add("token_logprobs top_k=5", logits[0].shape,
+        _time(lambda i: ops.token_logprobs(logits[i % 3], tgt, top_k=5), iters), logits[0].numel() * 4)
+    return out
+
+
 def main():
     ap = argparse.ArgumentParser()
     ap.add_argument("--only", default=None,
                     choices=["lif", "gemm", "ssa", "ssa_model", "train_gemm", "cnn", "attn_train", "data", "shapes",
-                             "lnlif"])
+                             "lnlif", "token"])
     ap.add_argument("--ssa-batch", type=int, default=256, help="images for --only ssa_model")
     ap.add_argument("--iters", type=int, default=20)
     ap.add_argument("--tokens", type=int, default=32 * 256, help="tokens per step for the gemm shapes")
@@ -392,6 +446,10 @@ def main():
             out["results"].append(r)
     if a.only in (None, "lnlif"):
         for r in bench_lnlif(a.iters):
+            r["frac_hbm"] = r["GB/s"] / peaks["hbm_gbs"]
+            out["results"].append(r)
+    if a.only in (None, "token"):
+        for r in bench_token(a.iters):
             r["frac_hbm"] = r["GB/s"] / peaks["hbm_gbs"]
             out["results"].append(r)
     if a.only in (None, "data"):
