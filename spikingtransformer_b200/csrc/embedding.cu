@@ -582,8 +582,9 @@ int launch_sort(const Plan& pl, const int64_t* tokens, int64_t n, int64_t V, int
   cfg.attrs = at;
   cfg.numAttrs = 1;
   cudaError_t e = cudaSuccess;
-  if (cfg.dynamicSmemBytes > (40u << 10))
-    e = cudaFuncSetAttribute(sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)cfg.dynamicSmemBytes);
+  if (cfg.dynamicSmemBytes > (40u << 10))  // the most of any call: another thread may be setting it too
+    e = cudaFuncSetAttribute(sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             (int)((kSortWarps + 2) << kMaxDigit) * 4);
   if (e == cudaSuccess && csize > 8) e = cudaFuncSetAttribute(sort_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
   if (e == cudaSuccess)
     e = cudaLaunchKernelEx(&cfg, sort_kernel, tokens, n, V, padding_idx, pl.bits, pl.passes, item0, item1);

@@ -568,8 +568,9 @@ unsigned blocks_of(K kernel, Resident& last, int64_t rows, const Shape& s, size_
   cudaGetDevice(&dev);
   if (last.dev != dev || last.threads != s.threads() || last.smem != smem) {
     int per_sm = 1;
-    if (smem > (40u << 10))  // 48 KB without asking, the kernel's static arrays included
-      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    // 48 KB without asking, the kernel's static arrays included; the same limit in every call,
+    // since another thread may be asking for another size
+    if (smem > (40u << 10)) cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 << 10);
     if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, s.threads(), smem) != cudaSuccess || per_sm < 1)
       per_sm = 1;
     last.dev = dev;

@@ -995,5 +995,45 @@ def test_operators_run_beside_each_other(ops):
 
 
 @pytest.mark.gpu
+def test_operators_from_several_threads(ops):
+    """Calls of different sizes (and so of different shared memory) from four host
+    threads at once give what they give one after the other."""
+    import threading
+    sizes = [(64, 512, torch.float32), (300, 768, torch.float32), (33, 8192, torch.float32), (50, 96, torch.bfloat16)]
+
+    def work(rows, D, dtype, seed):
+        x, w, b, gy = (t.to(DEV) for t in ln_case(rows, D, dtype, seed))
+        res = []
+        for _ in range(20):
+            y, stats = ops.layer_norm_fwd(x, w, b)
+            res = [y, *ops.layer_norm_bwd(gy, x, stats, w)]
+            tok = torch.arange(rows, device=DEV) * 7919 % (1 << (8 + seed))
+            res.append(ops.embedding_bwd(gy, tok, 1 << (8 + seed)))
+            res += ops.token_logprobs(x[None], tok % D, top_k=min(seed + 1, D))[:4]
+        torch.cuda.current_stream().synchronize()
+        return res
+
+    want = [work(*s, i) for i, s in enumerate(sizes)]
+    got, errors = [None] * len(sizes), []
+
+    def run(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                got[i] = work(*sizes[i], i)
+        except Exception as e:  # noqa: BLE001
+            errors.append(e)
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(len(sizes))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors
+    torch.cuda.synchronize()
+    for a, b in zip(want, got):
+        assert all(torch.equal(u, v) for u, v in zip(a, b))
+
+
+@pytest.mark.gpu
 def test_no_device_timeouts(ops):
     ops.device_error_check()
