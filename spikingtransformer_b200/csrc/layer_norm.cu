@@ -472,60 +472,111 @@ __device__ __forceinline__ float block_sum(float v) {
   return s;
 }
 
+// VEC = 4 or 1 elements of a type known at run time (aligned to themselves)
+template <int VEC>
+__device__ __forceinline__ void ld_long(const void* p, int dt, int64_t i, float (&v)[VEC]) {
+  if (dt == SPK_F32) Vec<SPK_F32, VEC>::load(reinterpret_cast<const float*>(p) + i, v);
+  else if (dt == SPK_F16) Vec<SPK_F16, VEC>::load(reinterpret_cast<const __half*>(p) + i, v);
+  else Vec<SPK_BF16, VEC>::load(reinterpret_cast<const __nv_bfloat16*>(p) + i, v);
+}
+template <int VEC>
+__device__ __forceinline__ void st_long(void* p, int dt, int64_t i, const float (&v)[VEC]) {
+  if (dt == SPK_F32) Vec<SPK_F32, VEC>::store(reinterpret_cast<float*>(p) + i, v);
+  else if (dt == SPK_F16) Vec<SPK_F16, VEC>::store(reinterpret_cast<__half*>(p) + i, v);
+  else Vec<SPK_BF16, VEC>::store(reinterpret_cast<__nv_bfloat16*>(p) + i, v);
+}
+
+// 1024 x 20000 bf16: 51 us (74 us by single elements); the backward 119 us (242).
+template <int VEC>
 __global__ void __launch_bounds__(kLong) long_fwd_kernel(const void* x, int xdt, int64_t ld, const void* w, int wdt,
                                                          const void* b, int bdt, float eps, int64_t rows, int D,
                                                          void* y, int ydt, float2* stats) {
   for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
-    float s = 0.0f;
-    for (int i = threadIdx.x; i < D; i += kLong) s += ld_any(x, xdt, r * ld + i);
+    float v[VEC], s = 0.0f;
+#pragma unroll 4
+    for (int i = threadIdx.x * VEC; i < D; i += kLong * VEC) {
+      ld_long<VEC>(x, xdt, r * ld + i, v);
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) s += v[j];
+    }
     const float mean = block_sum(s) / (float)D;
     float q = 0.0f;
-    for (int i = threadIdx.x; i < D; i += kLong) {
-      const float c = ld_any(x, xdt, r * ld + i) - mean;
-      q = fmaf(c, c, q);
+#pragma unroll 4
+    for (int i = threadIdx.x * VEC; i < D; i += kLong * VEC) {
+      ld_long<VEC>(x, xdt, r * ld + i, v);
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) q = fmaf(v[j] - mean, v[j] - mean, q);
     }
     const float rstd = 1.0f / sqrtf(block_sum(q) / (float)D + eps);
-    for (int i = threadIdx.x; i < D; i += kLong) {
-      const float h = (ld_any(x, xdt, r * ld + i) - mean) * rstd;
-      st_any(y, ydt, r * D + i, fmaf(h, w ? ld_any(w, wdt, i) : 1.0f, b ? ld_any(b, bdt, i) : 0.0f));
+#pragma unroll 2
+    for (int i = threadIdx.x * VEC; i < D; i += kLong * VEC) {
+      ld_long<VEC>(x, xdt, r * ld + i, v);
+#pragma unroll
+      for (int j = 0; j < VEC; ++j)
+        v[j] = fmaf((v[j] - mean) * rstd, w ? ld_any(w, wdt, i + j) : 1.0f, b ? ld_any(b, bdt, i + j) : 0.0f);
+      st_long<VEC>(y, ydt, r * D + i, v);
     }
     if (stats && threadIdx.x == 0) stats[r] = make_float2(mean, rstd);
   }
 }
 
+template <int VEC>
 __global__ void __launch_bounds__(kLong) long_bwd_x_kernel(const void* g, int gdt, const void* x, int xdt, int64_t ld,
                                                            const float2* stats, const void* w, int wdt, int64_t rows,
                                                            int D, void* gx) {
   for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
     const float mean = stats[r].x, rstd = stats[r].y;
-    float sa = 0.0f, sh = 0.0f;
-    for (int i = threadIdx.x; i < D; i += kLong) {
-      const float a = ld_any(g, gdt, r * D + i) * (w ? ld_any(w, wdt, i) : 1.0f);
-      sa += a;
-      sh = fmaf(a, (ld_any(x, xdt, r * ld + i) - mean) * rstd, sh);
+    float v[VEC], a[VEC], sa = 0.0f, sh = 0.0f;
+#pragma unroll 2
+    for (int i = threadIdx.x * VEC; i < D; i += kLong * VEC) {
+      ld_long<VEC>(g, gdt, r * D + i, a);
+      ld_long<VEC>(x, xdt, r * ld + i, v);
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        const float t = a[j] * (w ? ld_any(w, wdt, i + j) : 1.0f);
+        sa += t;
+        sh = fmaf(t, (v[j] - mean) * rstd, sh);
+      }
     }
     const float ma = block_sum(sa) / (float)D, mh = block_sum(sh) / (float)D;
-    for (int i = threadIdx.x; i < D; i += kLong) {
-      const float a = ld_any(g, gdt, r * D + i) * (w ? ld_any(w, wdt, i) : 1.0f);
-      const float h = (ld_any(x, xdt, r * ld + i) - mean) * rstd;
-      st_any(gx, xdt, r * D + i, rstd * (a - ma - h * mh));
+#pragma unroll 2
+    for (int i = threadIdx.x * VEC; i < D; i += kLong * VEC) {
+      ld_long<VEC>(g, gdt, r * D + i, a);
+      ld_long<VEC>(x, xdt, r * ld + i, v);
+#pragma unroll
+      for (int j = 0; j < VEC; ++j)
+        a[j] = rstd * (a[j] * (w ? ld_any(w, wdt, i + j) : 1.0f) - ma - (v[j] - mean) * rstd * mh);
+      st_long<VEC>(gx, xdt, r * D + i, a);
     }
   }
 }
 
+template <int VEC>
 __global__ void __launch_bounds__(kLong) long_bwd_w_kernel(const void* g, int gdt, const void* x, int xdt, int64_t ld,
                                                            const float2* stats, int64_t rows, int D, float* part) {
   pdl_trigger();
-  const int i = blockIdx.x * kLong + threadIdx.x;
+  const int i = (blockIdx.x * kLong + threadIdx.x) * VEC;
   if (i >= D) return;
-  float sw = 0.0f, sb = 0.0f;
+  float sw[VEC], sb[VEC], v[VEC], a[VEC];
+#pragma unroll
+  for (int j = 0; j < VEC; ++j) sw[j] = sb[j] = 0.0f;
+#pragma unroll 4
   for (int64_t r = blockIdx.y; r < rows; r += gridDim.y) {
-    const float gv = ld_any(g, gdt, r * D + i);
-    sw = fmaf(gv, (ld_any(x, xdt, r * ld + i) - stats[r].x) * stats[r].y, sw);
-    sb += gv;
+    ld_long<VEC>(g, gdt, r * D + i, a);
+    ld_long<VEC>(x, xdt, r * ld + i, v);
+    const float2 st = stats[r];
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+      sw[j] = fmaf(a[j], (v[j] - st.x) * st.y, sw[j]);
+      sb[j] += a[j];
+    }
   }
-  part[(int64_t)blockIdx.y * 2 * D + i] = sw;
-  part[((int64_t)blockIdx.y * 2 + 1) * D + i] = sb;
+  float* to = part + (int64_t)blockIdx.y * 2 * D + i;
+#pragma unroll
+  for (int j = 0; j < VEC; ++j) {
+    to[j] = sw[j];
+    to[D + j] = sb[j];
+  }
 }
 
 // ---------------------------------------------------------------- which kernel, how many blocks
@@ -675,9 +726,9 @@ int spk_layer_norm_fwd(const void* x, int x_dtype, int64_t ld, const void* w, in
   auto go = x_dtype == SPK_F32 ? dispatch_fwd<SPK_F32> : x_dtype == SPK_F16 ? dispatch_fwd<SPK_F16> : dispatch_fwd<SPK_BF16>;
   if (!go(x, ld, w, w_dtype, b, b_dtype, eps, rows, D, s, y, y_dtype, stats, st)) {
     const int64_t cap = (int64_t)num_sms() * 4;
-    long_fwd_kernel<<<(unsigned)(rows < cap ? rows : cap), kLong, 0, st>>>(x, x_dtype, ld, w, w_dtype, b, b_dtype, eps,
-                                                                          rows, (int)D, y, y_dtype,
-                                                                          reinterpret_cast<float2*>(stats));
+    auto kernel = wide ? long_fwd_kernel<4> : long_fwd_kernel<1>;
+    kernel<<<(unsigned)(rows < cap ? rows : cap), kLong, 0, st>>>(x, x_dtype, ld, w, w_dtype, b, b_dtype, eps, rows,
+                                                                 (int)D, y, y_dtype, reinterpret_cast<float2*>(stats));
   }
   return check_launch("layer_norm_fwd");
 }
@@ -718,12 +769,14 @@ int spk_layer_norm_bwd(const void* g, int g_dtype, const void* x, int x_dtype, i
   } else {
     const float2* sv = reinterpret_cast<const float2*>(stats);
     const int64_t cap = (int64_t)num_sms() * 4;
+    auto of_x = wide ? long_bwd_x_kernel<4> : long_bwd_x_kernel<1>;
+    auto of_w = wide ? long_bwd_w_kernel<4> : long_bwd_w_kernel<1>;
     if (gx)
-      long_bwd_x_kernel<<<(unsigned)(rows < cap ? rows : cap), kLong, 0, st>>>(g, g_dtype, x, x_dtype, ld, sv, w, w_dtype,
-                                                                              rows, (int)D, gx);
+      of_x<<<(unsigned)(rows < cap ? rows : cap), kLong, 0, st>>>(g, g_dtype, x, x_dtype, ld, sv, w, w_dtype, rows,
+                                                                 (int)D, gx);
     parts = (int)(rows < kLongChunks ? rows : kLongChunks);
     if (part)
-      long_bwd_w_kernel<<<dim3((unsigned)((D + kLong - 1) / kLong), (unsigned)parts), kLong, 0, st>>>(
+      of_w<<<dim3((unsigned)((D + kLong * s.vec - 1) / (kLong * s.vec)), (unsigned)parts), kLong, 0, st>>>(
           g, g_dtype, x, x_dtype, ld, sv, rows, (int)D, part);
   }
   if (part) {

@@ -172,7 +172,7 @@ def ln_exact(x, w, b, gy, eps, out_dtype):
 
 
 LN_SHAPES = [(1, 1), (3, 2), (5, 7), (2, 32), (9, 33), (64, 384), (33, 512), (7, 515), (130, 1000), (17, 1024),
-             (6, 1536), (5, 2047), (4, 4096), (3, 5001), (2, 8192), (2, 20000), (1500, 96), (777, 130), (1, 384)]
+             (6, 1536), (5, 2047), (4, 4096), (3, 5001), (2, 8192), (2, 20000), (3, 13001), (1500, 96), (777, 130), (1, 384)]
 
 
 @pytest.mark.gpu
@@ -236,7 +236,7 @@ def test_layer_norm_reads_column_slices(ops, start, D, pitch, dtype):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("rows,D", [(1, 8), (2, 384), (147, 96), (148, 384), (149, 515), (1184, 64), (1185, 1000),
-                                    (5000, 384), (3001, 2048), (700, 8192)])
+                                    (5000, 384), (3001, 2048), (700, 8192), (150, 20000), (70, 12801)])
 @pytest.mark.parametrize("dtype", FLOATS)
 def test_layer_norm_parameter_gradients_are_exact_on_integers(ops, rows, D, dtype):
     """With mean 0, 1/std 1 and small integers g_w = sum g x and g_b = sum g are
