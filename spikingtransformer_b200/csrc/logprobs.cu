@@ -127,13 +127,31 @@ __device__ __noinline__ float mean_of_extremes(const typename Elem<DT>::T* x, in
 }
 
 // (s + err) / T rounded once: the quotient's remainder takes the errors in, so
-// that near ties keep the order that the exact means have.  x: the value's first step.
+// that near ties keep the order that the exact means have.  With a T that is no
+// power of two 1 / T is rounded, which may push a quotient that lies half way
+// between two numbers to the odd one: the remainder of the result then is half a
+// step of it, exactly, and the even neighbour is taken.
+__device__ __forceinline__ bool power_of_two(int T) { return (T & (T - 1)) == 0; }
+__device__ __forceinline__ float quotient(float s, float err, int T, float inv_t) {
+  const float steps = (float)T, q = __fmul_rn(s, inv_t);
+  float z = fmaf(__fadd_rn(fmaf(-q, steps, s), err), inv_t, q);
+  if (!power_of_two(T)) {
+    const float rest = __fadd_rn(fmaf(-z, steps, s), err);
+    const uint32_t bits = __float_as_uint(z), exponent = bits & 0x7f800000u;
+    // half a step of z, T times; 0 where a step is below the normal numbers
+    const float half = exponent > (24u << 23) ? __uint_as_float(exponent - (24u << 23)) * steps : 0.0f;
+    if ((bits & 1u) && fabsf(rest) == half && half > 0.0f)
+      z = __uint_as_float((rest > 0.0f) == (z > 0.0f) ? bits + 1u : bits - 1u);
+  }
+  return z;
+}
+
+// x: the value's first step
 template <int DT>
 __device__ __forceinline__ float mean_of(float s, float err, const typename Elem<DT>::T* x, int64_t st, int T,
                                          float inv_t) {
   if (!(fabsf(s) < INFINITY)) return mean_of_extremes<DT>(x, st, T);
-  const float q = __fmul_rn(s, inv_t);
-  return fmaf(__fadd_rn(fmaf(-q, (float)T, s), err), inv_t, q);
+  return quotient(s, err, T, inv_t);
 }
 
 // z_j of one value
@@ -294,11 +312,14 @@ struct Tiles {
 #pragma unroll
     for (int i = 0; i < N / 2; ++i) odd = fma2(z[i], odd, odd);
     if (odd.x + odd.y == 0.0f) {
-      const float2 r2 = make_float2(inv_t, inv_t), t2 = make_float2(-(float)T, -(float)T);
+      if (power_of_two(T)) {  // s / T is exact
+        const float2 r2 = make_float2(inv_t, inv_t);
 #pragma unroll
-      for (int i = 0; i < N / 2; ++i) {
-        const float2 q = mul2(z[i], r2);
-        z[i] = fma2(add2(fma2(q, t2, z[i]), err[i]), r2, q);
+        for (int i = 0; i < N / 2; ++i) z[i] = fma2(err[i], r2, mul2(z[i], r2));
+      } else {
+#pragma unroll
+        for (int i = 0; i < N / 2; ++i)
+          z[i] = make_float2(quotient(z[i].x, err[i].x, T, inv_t), quotient(z[i].y, err[i].y, T, inv_t));
       }
     } else {
 #pragma unroll

@@ -607,6 +607,31 @@ def test_near_ties_of_the_step_mean_keep_the_exact_order(ops):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("T", [3, 4, 5, 6, 7, 10, 12, 31])
+def test_means_half_way_between_two_numbers_go_to_the_even_one(ops, T):
+    """Sums of T steps whose quotient lies exactly half way (integers N = T (2 k + 1), k
+    near 2^23 so that fp32 holds only every second of the quotients): with 1 / T
+    rounded, an unguarded quotient falls to either side.  Neighbours differ by one
+    such half step, so a wrong one shows in the order."""
+    g = gen(T)
+    V, rows = 64, 40
+    means = (1 << 24) + torch.randint(0, 1 << 10, (rows, V), generator=g)  # odd ones: half way
+    parts = torch.randint(-(1 << 20), 1 << 20, (T, rows, V), generator=g) * 2
+    parts[-1] = 0
+    parts[-1] = means * T - parts.sum(0)
+    x = parts.float()
+    # the last step in two, where fp32 does not hold it: what is left over goes to the first
+    x[0] = x[0] + (parts[-1] - x[-1].long()).float()
+    assert torch.equal(x.double().sum(0), (means * T).double())
+    tok = torch.zeros(rows, dtype=torch.int64)
+    want = torch.sort(x.double().mean(0).float(), dim=-1, descending=True, stable=True).indices[:, :32]
+    _, _, _, idx, _ = ops.token_logprobs(x.to(DEV), tok.to(DEV), top_k=32)
+    assert torch.equal(idx.cpu(), want)
+    negative = torch.sort((-x).double().mean(0).float(), dim=-1, descending=True, stable=True).indices[:, :32]
+    assert torch.equal(ops.token_logprobs(-x.to(DEV), tok.to(DEV), top_k=32)[3].cpu(), negative)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("T,V", [(1, 40), (4, 300), (1, 70000)])
 @pytest.mark.parametrize("dtype", FLOATS)
 def test_barred_symbols_and_rows_without_a_distribution(ops, T, V, dtype):
