@@ -431,7 +431,9 @@ __device__ __forceinline__ void range_of(int V, int head, int split, int splits,
 // memory, where the K best are ranked.  More keys than it holds (ties, or rows
 // without 32 numbers, where there is no floor): the K-th of those gathered is the
 // next floor, and the threads look again; every turn leaves out kGather - K keys
-// for good.  The K best do not depend on the order in which the keys came.
+// for good.  A floor among the keys of -inf and NaN is no bound on values (a NaN
+// compares with none), so every value is offered again and the keys are compared.
+// The K best do not depend on the order in which the keys came.
 template <int GT>
 struct Gather {
   static constexpr int kGather = GT == 32 ? 128 : 512;
@@ -484,8 +486,10 @@ struct Gather {
     for (;;) {
       if (tid == 0) count = 0;
       sync();
-      if (floor == 0 || mine >= (uint32_t)(floor >> 32))
-        offers(order_value((uint32_t)((floor + 1) >> 32)), floor == 0, [&](float v, int j) {
+      const uint32_t least = (uint32_t)((floor + 1) >> 32);
+      const bool all = least <= 0x007fffffu;  // -inf, NaN, or no floor
+      if (all || mine >= (uint32_t)(floor >> 32))
+        offers(order_value(least), all, [&](float v, int j) {
           const uint32_t bits = order_bits(v);
           const unsigned long long k = ((unsigned long long)bits << 32) | (uint32_t)~j;
           if (k > floor) {
@@ -859,8 +863,9 @@ __global__ void __launch_bounds__(256) bwd_kernel(Logits x, const int64_t* __res
   if constexpr (GT > 32) __syncthreads();
   else __syncwarp();
   if (GT > 32 && warp > 0) return;
-  auto mine = [&](int64_t j) {  // of this block's share of the row
-    return (j >= lo && j < hi) || (split == 0 && VEC > 1 && (j < head || j >= x.V - tail));
+  auto mine = [&](int64_t j) {  // of this block's share of the row, and a symbol at all
+    return (j >= lo && j < hi) ||
+           (split == 0 && VEC > 1 && ((j >= 0 && j < head) || (j >= x.V - tail && j < x.V)));
   };
   auto put = [&](int64_t j, float add) {
     const E d = Elem<DT>::make(fmaf(add, x.inv_t, at_one(mean_over_t<DT>(row + j, x.st, x.T, x.inv_t))));

@@ -677,6 +677,36 @@ def test_barred_symbols_and_rows_without_a_distribution(ops, T, V, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("T,rows,V", [(1, 9, 200), (2, 9, 1000), (1, 9, 1000), (1, 2400, 1000), (1, 9, 9000),
+                                      (1, 300, 20000), (1, 9, 70000), (3, 9, 70001)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("K", [5, 32])
+def test_alternatives_of_rows_with_more_nans_than_numbers(ops, T, rows, V, dtype, K):
+    """Fewer numbers than alternatives asked for, more NaNs than are gathered at once: the
+    numbers come first, then -inf, then NaNs, each by index, and nothing outside the row
+    is read or written."""
+    x = torch.full((rows, V), float("nan"))
+    places = torch.randperm(V, generator=gen(V))[:K - 1]
+    kinds = rows // 3  # a third all NaN, a third with K - 1 numbers, a third with -inf besides
+    x[kinds:, places] = torch.arange(K - 1).float()
+    x[2 * kinds:, places[:2]] = float("-inf")
+    want = []
+    for r in range(rows):
+        key = x[r].clone()
+        low = key == float("-inf")
+        key[low] = -1.0
+        key[key.isnan()] = -2.0
+        want.append(torch.sort(key, descending=True, stable=True).indices[:K])
+    xd = x.to(dtype).expand(T, rows, V).contiguous().to(DEV).requires_grad_(True)
+    tok = torch.zeros(rows, dtype=torch.int64, device=DEV)
+    logp, H, top, idx, bad = ops.token_logprobs(xd, tok, top_k=K)
+    assert torch.equal(idx.cpu(), torch.stack(want)) and int(bad) == 0
+    assert logp.isnan().all() and H.isnan().all() and top.isnan().all()
+    (gx,) = torch.autograd.grad(top, xd, torch.ones_like(top))
+    assert gx.isnan().all()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("V", [48, 300, 9000])
 @pytest.mark.parametrize("dtype", FLOATS)
 def test_lowest_values_are_above_minus_infinity(ops, V, dtype):
