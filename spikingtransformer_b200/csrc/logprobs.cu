@@ -12,6 +12,8 @@
 // whose only errors are its own rounding and that of the constant, and a change
 // of c scales sums by a power of two.  With S = sum 2^t_j and
 // A = sum t_j 2^t_j:  logp = ln 2 (t_y - log2 S),  H = ln 2 (log2 S - A / S).
+// t_y and log2 S of a likely symbol are small, so logp and H near 0 are right to a
+// few 2^-24 (not to so much of themselves); they are held at their side of 0.
 // Where the maximum is beyond 2^20 (a row barred with the type's lowest value),
 // c would be coarser than 1, so the maximum itself is taken off first:
 // t_j = (z_j - off) log2 e.  t is held at -200 or above, where 2^t is 0 already,
@@ -611,21 +613,27 @@ struct Out {
   float4* stats;
 };
 
-// the row's results from its state and list (one warp)
+// a log probability: the rounded difference of two numbers may come out above 0 (and an
+// entropy below it); a NaN passes
+__device__ __forceinline__ float at_most_0(float v) { return v > 0.0f ? 0.0f : v; }
+
+// the row's results from its state and list (one warp).  The gradient gets the
+// entropy as it came out: where one symbol has all of the probability its error and
+// that of log p cancel in log p + H.
 template <int DT>
 __device__ __forceinline__ void write_row(const Logits& x, const typename Elem<DT>::T* row, int64_t r, int64_t y,
                                           State s, unsigned long long key, int K, int lane, const Out& o) {
   const Ref f = s.f;
   const float l2s = log2f(s.S), H = kLn2 * (l2s - s.A / s.S);
   if (lane == 0) {
-    o.logp[r] = kLn2 * (log2_from(mean_over_t<DT>(row + y, x.st, x.T, x.inv_t), f) - l2s);
-    o.entropy[r] = H;
+    o.logp[r] = at_most_0(kLn2 * (log2_from(mean_over_t<DT>(row + y, x.st, x.T, x.inv_t), f) - l2s));
+    o.entropy[r] = H < 0.0f ? 0.0f : H;
     if (o.stats) o.stats[r] = make_float4(f.off, f.c, s.S, H);
   }
   if (lane < K) {
     o.top_idx[r * K + lane] = (int64_t)(~(uint32_t)key);
     // a row without a distribution has none for the alternatives either
-    o.top_logp[r * K + lane] = kLn2 * (log2_from(order_value((uint32_t)(key >> 32)), f) - l2s);
+    o.top_logp[r * K + lane] = at_most_0(kLn2 * (log2_from(order_value((uint32_t)(key >> 32)), f) - l2s));
   }
 }
 

@@ -737,6 +737,32 @@ def test_lowest_values_are_above_minus_infinity(ops, V, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("T,V", [(1, 1), (1, 40), (3, 300), (1, 5000), (1, 70000)])
+@pytest.mark.parametrize("dtype", FLOATS)
+def test_rows_of_one_symbol_have_no_positive_logp_and_no_negative_entropy(ops, T, V, dtype):
+    """One symbol with (nearly) all of the probability, at maxima of any size: logp <= 0
+    and entropy >= 0, both within their bounds of the exact values near 0."""
+    rows, K = 64, min(2, V)
+    g = gen(V)
+    x = torch.full((T, rows, V), float("-inf"))
+    tok = torch.randint(0, V, (rows,), generator=g)
+    if V > 1:
+        x[:, rows // 2:] = -20.0 + torch.rand(T, rows // 2, V, generator=g)  # half: others far below
+    x[:, torch.arange(rows), tok] = torch.randn(T, rows, generator=g) * 10 + 20
+    x = x.to(dtype)
+    o = lp_exact(x, tok, K)
+    xd = x.to(DEV).requires_grad_(True)
+    logp, H, top, idx, _ = ops.token_logprobs(xd, tok.to(DEV), top_k=K)
+    assert (logp <= 0).all() and (H >= 0).all() and (top <= 0).all()
+    assert torch.equal(idx[:, 0].cpu(), tok)
+    assert_within(logp, o["logp"], o["e_logp"], "logp")
+    assert_within(H, o["entropy"], o["e_H"], "entropy")
+    gl, gh = torch.randn(rows, generator=g), torch.randn(rows, generator=g)
+    (gx,) = torch.autograd.grad((logp, H), xd, (gl.to(DEV), gh.to(DEV)))
+    assert_within(gx[0], *lp_grad_exact(o, gl, gh, None, T, dtype), "grad")
+
+
+@pytest.mark.gpu
 def test_token_logprobs_near_one_keeps_its_digits(ops):
     """p_y = 1 - 1e-7 or so: logp comes from t_y - log2 S, not from the difference
     of two numbers near 20."""
