@@ -21,6 +21,7 @@ import math
 import torch
 import torch.nn as nn
 from torch import Tensor
+from torch.autograd import forward_ad
 
 from . import ops
 from ._fused import bf16_weight, fast_path_ok, lif_params, mark_spike_counts, spike_counts_bf16
@@ -47,11 +48,32 @@ class PositionalEncoding(nn.Module):
         return self.dropout(token_embedding + self.pos_embedding[:, : token_embedding.size(1)])
 
 
+def _only_looks_up(e, tokens):
+    """Whether calling the module ``e`` on ``tokens`` is the lookup of a plain
+    ``nn.Embedding`` and its first and second derivatives, with nothing to see it: no
+    subclass or wrapper, no hook, no option that changes the result or the
+    gradient, no tensor subclass, and no transform (forward mode, ``torch.func``,
+    tracing, compiling) that follows tensors through torch's own operations."""
+    if type(e) is not nn.Embedding or "forward" in e.__dict__ or e._compiled_call_impl is not None:
+        return False
+    if (e.max_norm is not None or e.scale_grad_by_freq or e.sparse or e._forward_hooks or e._forward_pre_hooks
+            or e._backward_hooks or e._backward_pre_hooks or nn.modules.module._has_any_global_hook()):
+        return False
+    if type(e.weight) not in (nn.Parameter, Tensor) or type(tokens) is not Tensor:
+        return False
+    if e.padding_idx is not None and not 0 <= e.padding_idx < e.weight.shape[0]:
+        return False
+    return not (forward_ad._current_level >= 0 or torch._C._are_functorch_transforms_active()
+                or torch.compiler.is_compiling() or torch.jit.is_tracing())
+
+
 class TokenEmbedding(nn.Module):
     """``Seq2Seq.py:29-36``: ``embedding(tokens) * sqrt(emb_size)``, on CUDA through
     ``ops.embedding`` (lookup and scaling in one kernel, the weight's gradient by
-    sorted tokens).  ``bad_tokens`` is then the device flag of the last call: 1 if
-    a token lay outside the vocabulary (its row is zeros)."""
+    sorted tokens) where that is all that calling ``embedding`` would do; any other
+    module, hook or transform is called as it is.  ``bad_tokens`` is the device flag
+    of the last call through ``ops.embedding``: 1 if a token lay outside the
+    vocabulary (its row is zeros)."""
 
     bad_tokens = None
 
@@ -62,9 +84,7 @@ class TokenEmbedding(nn.Module):
 
     def forward(self, tokens: Tensor):
         e = self.embedding
-        plain = e.max_norm is None and not (e.scale_grad_by_freq or e.sparse or e._forward_hooks
-                                            or e._forward_pre_hooks or e._backward_hooks)
-        if plain and e.weight.is_cuda and e.weight.dtype in ops.EMBEDDING_DTYPES:
+        if _only_looks_up(e, tokens) and e.weight.is_cuda and e.weight.dtype in ops.EMBEDDING_DTYPES:
             out, self.bad_tokens = ops.embedding(tokens.long(), e.weight, math.sqrt(self.emb_size),
                                                  padding_idx=e.padding_idx)
             return out

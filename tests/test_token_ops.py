@@ -879,6 +879,110 @@ def test_token_embedding_module_matches_the_lookup(ops):
     assert int(m.bad_tokens) == 1
 
 
+class CountedEmbedding(torch.nn.Embedding):
+    """A forward of its own: every row halved."""
+
+    def forward(self, tokens):
+        return super().forward(tokens) / 2
+
+
+class Adapter(torch.nn.Module):
+    """A wrapper with a ``weight`` and nothing else of ``nn.Embedding``."""
+
+    def __init__(self, inner):
+        super().__init__()
+        self.inner = inner
+
+    @property
+    def weight(self):
+        return self.inner.weight
+
+    def forward(self, tokens):
+        return self.inner(tokens) + 1
+
+
+def observers(m, seen):
+    """Ways to see or change a call of ``m.embedding``: (name, set up, undo)."""
+    note = lambda *a: seen.append(1)  # noqa: E731
+    glob = torch.nn.modules.module
+    e = m.embedding
+    yield "forward hook", e.register_forward_hook(note)
+    yield "forward pre-hook", e.register_forward_pre_hook(note)
+    yield "backward hook", e.register_full_backward_hook(note)
+    yield "backward pre-hook", e.register_full_backward_pre_hook(note)
+    yield "global forward hook", glob.register_module_forward_hook(note)
+    yield "global forward pre-hook", glob.register_module_forward_pre_hook(note)
+    yield "global backward hook", glob.register_module_full_backward_hook(note)
+    yield "global backward pre-hook", glob.register_module_full_backward_pre_hook(note)
+
+
+DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_token_embedding_calls_what_is_more_than_a_lookup(device):
+    """Subclasses, wrappers, replaced forwards and every kind of hook on the embedding
+    of a TokenEmbedding are run."""
+    from spikingtransformer_b200.Seq2Seq import TokenEmbedding, _only_looks_up
+    tok = torch.randint(0, 9, (3, 4), generator=gen(1)).to(device)
+    m = TokenEmbedding(9, 16).to(device)
+    weight, scale = m.embedding.weight, 4.0
+    plain = weight.detach()[tok] * scale
+    assert _only_looks_up(m.embedding, tok) and torch.equal(m(tok), plain)
+    seen = []
+    for name, hook in observers(m, seen):
+        del seen[:]
+        assert not _only_looks_up(m.embedding, tok), name
+        m(tok).sum().backward()
+        assert seen, name
+        hook.remove()
+    assert _only_looks_up(m.embedding, tok)
+    sub = CountedEmbedding(9, 16).to(device)
+    sub.weight = weight
+    m.embedding = sub
+    assert torch.equal(m(tok), weight.detach()[tok] / 2 * scale)
+    m.embedding = Adapter(sub)
+    assert torch.equal(m(tok), (weight.detach()[tok] / 2 + 1) * scale)
+    m.embedding = torch.nn.Embedding(9, 16).to(device)
+    m.embedding.forward = lambda t: weight[t] * 3
+    assert torch.equal(m(tok), weight.detach()[tok] * 3 * scale)
+    for change in (dict(max_norm=1.0), dict(sparse=True), dict(scale_grad_by_freq=True)):
+        assert not _only_looks_up(torch.nn.Embedding(9, 16, **change), tok)
+    e = torch.nn.Embedding(9, 16, padding_idx=2)
+    assert _only_looks_up(e, tok)
+    e.padding_idx = -1  # torch counts from the end
+    assert not _only_looks_up(e, tok)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_token_embedding_under_forward_mode_and_function_transforms(device):
+    """Tangents, ``torch.func`` and tracing pass through a TokenEmbedding (it is linear in
+    its weight: small integers, equality)."""
+    import torch.autograd.forward_ad as fwd
+    from torch.func import functional_call, grad, jvp, vmap
+    from spikingtransformer_b200.Seq2Seq import TokenEmbedding
+    m = TokenEmbedding(9, 16).to(device)
+    tok = torch.randint(0, 9, (3, 4), generator=gen(1)).to(device)
+    w, v = (torch.randint(-4, 5, (9, 16), generator=gen(i)).float().to(device) for i in (2, 3))
+    name = "embedding.weight"
+
+    def f(weight):
+        return functional_call(m, {name: weight}, (tok,))
+
+    out, tangent = jvp(f, (w,), (v,))
+    assert torch.equal(out, w[tok] * 4) and torch.equal(tangent, v[tok] * 4)
+    with fwd.dual_level():
+        for leaf in (w, w.clone().requires_grad_(True)):
+            assert torch.equal(fwd.unpack_dual(f(fwd.make_dual(leaf, v))).tangent, v[tok] * 4)
+    counts = torch.bincount(tok.flatten(), minlength=9).float().unsqueeze(1).expand(9, 16)
+    assert torch.equal(grad(lambda p: f(p).sum())(w), counts * 4)
+    both = vmap(f)(torch.stack([w, v]))
+    assert torch.equal(both, torch.stack([w[tok], v[tok]]) * 4)
+    traced = torch.jit.trace(m, (tok,), check_trace=False)
+    other = (tok + 1) % 9
+    assert torch.equal(traced(other), m(other))
+
+
 @pytest.mark.gpu
 def test_score_is_the_log_softmax_of_the_mean_logits(ops):
     model = small_model().eval()
