@@ -888,6 +888,15 @@ def _embedding_bwd(dev, g, tokens, plan, V, scale, padding_idx, dtype):
     return gw
 
 
+def _embedding_bwd_composed(g, tokens, V, scale, padding_idx, dtype):
+    """The same in torch's operations, for a ``g`` that is more than its data (a batch of
+    gradients at once)."""
+    used = (tokens >= 0) & (tokens < V)
+    rows = torch.where(used.unsqueeze(-1), g.float(), 0.0)
+    gw = torch.ops.aten.embedding_dense_backward(rows, torch.where(used, tokens, 0), V, padding_idx, False)
+    return (gw * scale).to(dtype)
+
+
 class _Embedding(torch.autograd.Function):
     @staticmethod
     def forward(ctx, weight, tokens, scale, padding_idx, dev, dt):
@@ -904,9 +913,11 @@ class _Embedding(torch.autograd.Function):
         if g is None:
             return None, None, None, None, None, None
         plan, tokens = ctx.saved_tensors
+        dev, V, scale, padding_idx, dtype = ctx.meta
+        if torch._C._functorch.is_legacy_batchedtensor(g):  # of autograd.grad(..., is_grads_batched=True)
+            return _embedding_bwd_composed(g, tokens, V, scale, padding_idx, dtype), None, None, None, None, None
         if torch.is_grad_enabled():
             return _EmbeddingGrad.apply(g, plan, tokens, ctx.meta), None, None, None, None, None
-        dev, V, scale, padding_idx, dtype = ctx.meta
         return _embedding_bwd(dev, g, None, plan, V, scale, padding_idx, dtype), None, None, None, None, None
 
 

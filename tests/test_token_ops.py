@@ -416,6 +416,21 @@ def test_embedding_second_derivatives(ops):
 
 
 @pytest.mark.gpu
+def test_embedding_gradients_in_a_batch(ops):
+    """``is_grads_batched``: each gradient of the batch is that of its own call (integers:
+    equality), tokens outside the vocabulary and the padding row without one."""
+    tok = torch.randint(0, 7, (5, 6), generator=gen(1))
+    tok[0, 0], tok[1, 1] = -1, 1 << 40
+    w = torch.randn(7, 12, generator=gen(2)).to(DEV).requires_grad_(True)
+    g = torch.randint(-9, 10, (3, 5, 6, 12), generator=gen(3)).float().to(DEV)
+    out, bad = ops.embedding(tok.to(DEV), w, 0.5, padding_idx=2)
+    (got,) = torch.autograd.grad(out, w, g, is_grads_batched=True)
+    for i in range(3):
+        want = scatter_exact(tok.flatten(), g[i].reshape(30, 12).cpu(), 7, 0.5, 2)
+        assert torch.equal(got[i].cpu().double(), want)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("n,V,D", [(50, 9, 24), (3000, 257, 40)])
 def test_embedding_padding_and_bad_tokens(ops, n, V, D):
     gr = gen(n)
