@@ -5,6 +5,7 @@ CPU implementation in this package.
 """
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -648,13 +649,22 @@ def _one_device(first, *ts):
     return dev
 
 
+def _dual(*ts):
+    """Whether a tensor carries a tangent of forward-mode differentiation, which a call by
+    pointers would drop."""
+    return forward_ad._current_level >= 0 and any(
+        t is not None and forward_ad.unpack_dual(t).tangent is not None for t in ts)
+
+
 def _backward(fn):
     """The backward of a Function with first derivatives only: as
     ``once_differentiable``, whose work is skipped where no graph of the
-    gradient is being built."""
+    gradient is being built.  Gradients with tangents are refused."""
     guarded = torch.autograd.function.once_differentiable(fn)
 
     def backward(ctx, *grads):
+        if _dual(*grads):
+            raise NotImplementedError("the gradient has no forward-mode derivative")
         return guarded(ctx, *grads) if torch.is_grad_enabled() else fn(ctx, *grads)
 
     return staticmethod(backward)
@@ -795,11 +805,12 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, out_dtype=None):
     """Differentiable LayerNorm over the last dimension (``torch.nn.LayerNorm``
     without a LIF behind it, for the shapes and uses ``ln_lif_fwd`` does not
     cover): ``layer_norm_fwd`` with gradients of ``x``, ``weight`` and ``bias``
-    (first derivatives only).  Autocast does not change the types: a bf16 ``x``
+    (first derivatives only; forward-mode tangents are refused, here and in the
+    other token-side operators).  Autocast does not change the types: a bf16 ``x``
     gives a bf16 result unless ``out_dtype`` says otherwise."""
     dev, dt = _check_layer_norm_fwd(x, weight, bias, out_dtype)
     if torch.is_grad_enabled() and (x.requires_grad or weight is not None and weight.requires_grad
-                                    or bias is not None and bias.requires_grad):
+                                    or bias is not None and bias.requires_grad) or _dual(x, weight, bias):
         return _LayerNorm.apply(x, weight, bias, eps, dev, dt)
     return _layer_norm_fwd(dev, x, weight, bias, eps, dt, False)[0]
 
@@ -890,7 +901,7 @@ def _embedding_bwd(dev, g, tokens, plan, V, scale, padding_idx, dtype):
 
 def _embedding_bwd_composed(g, tokens, V, scale, padding_idx, dtype):
     """The same in torch's operations, for a ``g`` that is more than its data (a batch of
-    gradients at once)."""
+    gradients at once, a tangent)."""
     used = (tokens >= 0) & (tokens < V)
     rows = torch.where(used.unsqueeze(-1), g.float(), 0.0)
     gw = torch.ops.aten.embedding_dense_backward(rows, torch.where(used, tokens, 0), V, padding_idx, False)
@@ -914,7 +925,7 @@ class _Embedding(torch.autograd.Function):
             return None, None, None, None, None, None
         plan, tokens = ctx.saved_tensors
         dev, V, scale, padding_idx, dtype = ctx.meta
-        if torch._C._functorch.is_legacy_batchedtensor(g):  # of autograd.grad(..., is_grads_batched=True)
+        if torch._C._functorch.is_legacy_batchedtensor(g) or _dual(g):  # the former with is_grads_batched=True
             return _embedding_bwd_composed(g, tokens, V, scale, padding_idx, dtype), None, None, None, None, None
         if torch.is_grad_enabled():
             return _EmbeddingGrad.apply(g, plan, tokens, ctx.meta), None, None, None, None, None
@@ -951,7 +962,7 @@ def embedding(tokens, weight, scale=1.0, padding_idx=None, out_dtype=None):
         padding_idx = -1
     elif not 0 <= padding_idx < weight.shape[0]:
         raise ValueError("padding_idx %d outside [0, %d)" % (padding_idx, weight.shape[0]))
-    if torch.is_grad_enabled() and weight.requires_grad:
+    if torch.is_grad_enabled() and weight.requires_grad or _dual(weight):
         return _Embedding.apply(weight, tokens, scale, padding_idx, dev, dt)
     return _embedding_fwd(dev, tokens, weight, scale, dt, None, -1)
 
@@ -1049,7 +1060,7 @@ def token_logprobs(logits, tokens, top_k=0, ignore_index=-100):
     if not 0 <= top_k <= min(MAX_TOP_K, logits.shape[-1]):
         raise ValueError("top_k must be between 0 and min(%d, V) (got %d)" % (MAX_TOP_K, top_k))
     tokens = _tokens_i64(tokens)
-    if torch.is_grad_enabled() and logits.requires_grad:
+    if torch.is_grad_enabled() and logits.requires_grad or _dual(logits):
         return _TokenLogprobs.apply(logits, tokens, int(top_k), int(ignore_index), dev)
     return _token_logprobs_fwd(dev, logits, tokens, int(top_k), int(ignore_index), False)[:5]
 

@@ -124,6 +124,38 @@ def test_second_derivatives_are_refused(ops):
             g.sum().backward()
 
 
+@pytest.mark.gpu
+def test_forward_mode_tangents_are_refused_and_not_lost(ops):
+    """A tangent on an input, with or without a gradient wanted, or on a gradient: an
+    error, as from every operator without a forward-mode derivative.  The embedding's
+    gradient is linear in g and takes g's tangent through."""
+    import torch.autograd.forward_ad as fwd
+    x, v = torch.randn(4, 8, device=DEV), torch.randn(4, 8, device=DEV)
+    w = torch.ones(8, device=DEV)
+    t = torch.tensor([0, 3, 1, 3], device=DEV)
+    calls = [lambda p: ops.layer_norm(p), lambda p: ops.layer_norm(x, p[0]), lambda p: ops.layer_norm(x, None, p[0]),
+             lambda p: ops.embedding(t, p), lambda p: ops.token_logprobs(p[None], t)]
+    with fwd.dual_level():
+        for call in calls:
+            for leaf in (x, x.clone().requires_grad_(True)):
+                with pytest.raises(NotImplementedError):
+                    call(fwd.make_dual(leaf, v))
+                with pytest.raises(NotImplementedError), torch.no_grad():
+                    call(fwd.make_dual(leaf, v))
+            call(x)  # no tangent: as ever
+        for call in (lambda p: ops.layer_norm(p), lambda p: ops.layer_norm(x, p[0]),
+                     lambda p: ops.token_logprobs(p[None], t)[0]):
+            leaf = x.clone().requires_grad_(True)
+            y = call(leaf)
+            with pytest.raises(NotImplementedError):
+                torch.autograd.grad(y, leaf, fwd.make_dual(torch.ones_like(y), torch.ones_like(y)))
+        leaf = x.clone().requires_grad_(True)
+        g = torch.randint(-9, 10, (4, 8), device=DEV).float()
+        (gw,) = torch.autograd.grad(ops.embedding(t, leaf, 2.0)[0], leaf, fwd.make_dual(g, g + 1))
+        for got, of in zip(fwd.unpack_dual(gw), (g, g + 1)):
+            assert torch.equal(got.cpu().double(), scatter_exact(t.cpu(), of.cpu(), 4, 2.0))
+
+
 # ------------------------------------------------------------------ LayerNorm
 
 
