@@ -52,7 +52,7 @@
  *   spk_layer_norm_fwd / _bwd
  *                          nn.LayerNorm on its own (SSA.py:218-249,
  *                          SpikingMLP.py:31-36) and its autograd
- *   spk_embedding_fwd / _bwd
+ *   spk_embedding_fwd / _fwd_watched / _bwd
  *                          TokenEmbedding, Seq2Seq.py:29-36, and the gradient
  *                          of its weight
  *   spk_token_logprobs_fwd / _bwd
@@ -519,7 +519,9 @@ int spk_layer_norm_bwd(const void* g, int g_dtype, const void* x, int x_dtype, i
  * Scaled token embedding (TokenEmbedding, Seq2Seq.py:29-36) and the gradient
  * of its weight.  out[i] = scale * weight[tokens[i]], [n][D] of out_dtype;
  * weight: [V][D] of w_dtype with row stride ldw.  A token outside [0, V) reads
- * as zeros and sets *bad_token (which the call clears first).
+ * as zeros and sets *bad_token (which the call clears first).  The watched form
+ * also sets *bad_ever, which no call clears: device memory, or page-locked host
+ * memory that the host may look at whenever it likes (NULL: none).
  * With `plan` (spk_embedding_plan_bytes(n) bytes, 16-byte aligned) the call also
  * sorts the positions by token into it, for the backward, beside the lookup;
  * NULL where no gradient will be wanted.
@@ -533,6 +535,9 @@ int64_t spk_embedding_plan_bytes(int64_t n);
 int spk_embedding_fwd(const int64_t* tokens, const void* weight, int w_dtype, int64_t ldw, float scale, int64_t n,
                       int64_t V, int64_t D, void* out, int out_dtype, int* bad_token, int64_t padding_idx, void* plan,
                       int64_t plan_bytes, void* stream);
+int spk_embedding_fwd_watched(const int64_t* tokens, const void* weight, int w_dtype, int64_t ldw, float scale,
+                              int64_t n, int64_t V, int64_t D, void* out, int out_dtype, int* bad_token, int* bad_ever,
+                              int64_t padding_idx, void* plan, int64_t plan_bytes, void* stream);
 int64_t spk_embedding_bwd_workspace_bytes(int64_t n, int64_t V, int64_t D);
 int spk_embedding_bwd(const int64_t* tokens, const void* g, int g_dtype, float scale, int64_t padding_idx, int64_t n,
                       int64_t V, int64_t D, void* gw, int w_dtype, void* plan, int64_t plan_bytes, void* workspace,

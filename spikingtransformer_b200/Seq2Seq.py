@@ -54,6 +54,9 @@ def _only_looks_up(e, tokens):
     subclass or wrapper, no hook, no option that changes the result or the
     gradient, no tensor subclass, and no transform (forward mode, ``torch.func``,
     tracing, compiling) that follows tensors through torch's own operations."""
+    if (torch.compiler.is_compiling() or torch.jit.is_tracing() or forward_ad._current_level >= 0
+            or torch._C._are_functorch_transforms_active()):
+        return False
     if type(e) is not nn.Embedding or "forward" in e.__dict__ or e._compiled_call_impl is not None:
         return False
     if (e.max_norm is not None or e.scale_grad_by_freq or e.sparse or e._forward_hooks or e._forward_pre_hooks
@@ -61,33 +64,44 @@ def _only_looks_up(e, tokens):
         return False
     if type(e.weight) not in (nn.Parameter, Tensor) or type(tokens) is not Tensor:
         return False
-    if e.padding_idx is not None and not 0 <= e.padding_idx < e.weight.shape[0]:
-        return False
-    return not (forward_ad._current_level >= 0 or torch._C._are_functorch_transforms_active()
-                or torch.compiler.is_compiling() or torch.jit.is_tracing())
+    return e.padding_idx is None or 0 <= e.padding_idx < e.weight.shape[0]
 
 
 class TokenEmbedding(nn.Module):
     """``Seq2Seq.py:29-36``: ``embedding(tokens) * sqrt(emb_size)``, on CUDA through
     ``ops.embedding`` (lookup and scaling in one kernel, the weight's gradient by
     sorted tokens) where that is all that calling ``embedding`` would do; any other
-    module, hook or transform is called as it is.  ``bad_tokens`` is the device flag
-    of the last call through ``ops.embedding``: 1 if a token lay outside the
-    vocabulary (its row is zeros)."""
-
-    bad_tokens = None
+    module, hook or transform is called as it is.  A token outside the vocabulary
+    (a row of zeros, no gradient) is an error, raised as an ``IndexError`` by the
+    first call after the one with the token has run, or read from ``bad_tokens``."""
 
     def __init__(self, vocab_size: int, emb_size: int):
         super().__init__()
         self.embedding = nn.Embedding(vocab_size, emb_size)
         self.emb_size = emb_size
+        self._watch = ops.BadTokens()
+
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        self.__dict__.pop("bad_tokens", None)  # of modules saved with a flag, or without one
+        self.__dict__.setdefault("_watch", ops.BadTokens())
+
+    @property
+    def bad_tokens(self) -> int:
+        """1 if a call had a token outside the vocabulary and no error has told of it yet,
+        else 0.  Waits for the weight's device."""
+        if self.embedding.weight.is_cuda:
+            torch.cuda.synchronize(self.embedding.weight.device)
+        return int(self._watch.seen())
 
     def forward(self, tokens: Tensor):
         e = self.embedding
         if _only_looks_up(e, tokens) and e.weight.is_cuda and e.weight.dtype in ops.EMBEDDING_DTYPES:
-            out, self.bad_tokens = ops.embedding(tokens.long(), e.weight, math.sqrt(self.emb_size),
-                                                 padding_idx=e.padding_idx)
-            return out
+            if self._watch.seen():
+                self._watch.clear()
+                raise IndexError("an earlier call of this TokenEmbedding had tokens outside [0, %d)" % e.weight.shape[0])
+            return ops.embedding(tokens.long(), e.weight, math.sqrt(self.emb_size), padding_idx=e.padding_idx,
+                                 watch=self._watch)[0]
         return e(tokens.long()) * math.sqrt(self.emb_size)
 
 

@@ -71,6 +71,7 @@ SIGNATURES = {
     "spk_layer_norm_bwd": ([_p, _i, _p, _i, _i64, _p, _p, _i, _i64, _i64, _p, _p, _p, _i, _p, _i64, _p], _i),
     "spk_embedding_plan_bytes": ([_i64], _i64),
     "spk_embedding_fwd": ([_p, _p, _i, _i64, _f, _i64, _i64, _i64, _p, _i, _p, _i64, _p, _i64, _p], _i),
+    "spk_embedding_fwd_watched": ([_p, _p, _i, _i64, _f, _i64, _i64, _i64, _p, _i, _p, _p, _i64, _p, _i64, _p], _i),
     "spk_embedding_bwd_workspace_bytes": ([_i64, _i64, _i64], _i64),
     "spk_embedding_bwd": ([_p, _p, _i, _f, _i64, _i64, _i64, _i64, _p, _i, _p, _i64, _p, _i64, _p], _i),
     "spk_token_logprobs_workspace_bytes": ([_i64, _i64, _i64, _i64], _i64),

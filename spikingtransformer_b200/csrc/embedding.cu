@@ -4,7 +4,8 @@
 //   g_W[v] = scale * sum over i with tok[i] = v, in ascending i, of g[i]
 //
 // Tokens outside [0, V) read as a row of zeros, take no gradient and raise the
-// caller's flag.
+// caller's flag, and a second one that no call clears (a word of the host's memory,
+// so that the host can look at it without waiting).
 //
 // The gradient needs the positions sorted by token (stable, radix).  One cluster
 // of blocks does that; a forward whose gradient will be wanted launches it just
@@ -87,10 +88,10 @@ template <int WDT, int ODT, int VEC>
 __global__ void __launch_bounds__(256, 4) gather_kernel(const int64_t* __restrict__ tokens,
                                                      const typename Elem<WDT>::T* __restrict__ w, int64_t ldw,
                                                      float scale, int64_t n, int64_t V, int D, int tiles,
-                                                     typename Elem<ODT>::T* __restrict__ out, int* bad, int extra,
-                                                     int scan_bad, int after_sort) {
+                                                     typename Elem<ODT>::T* __restrict__ out, int* bad, int* ever,
+                                                     int extra, int scan_bad, int after_sort) {
   if (extra && blockIdx.x == 0) {  // the first block, so that it is not the last to end
-    if (scan_bad) scan_tokens(tokens, n, V, 0, bad);
+    if (scan_bad && scan_tokens(tokens, n, V, 0, bad) && ever && threadIdx.x == 0) *ever = 1;
     // The sort before this kernel may still be running: this block does not end before it, so
     // whoever comes after this kernel finds the sort done.
     if (after_sort) pdl_wait();
@@ -107,7 +108,10 @@ __global__ void __launch_bounds__(256, 4) gather_kernel(const int64_t* __restric
     tok = __ldg(tokens + i0 + lane);
     if (tok < 0 || tok >= V) {
       tok = -1;
-      if (!scan_bad) atomicExch(bad, 1);
+      if (!scan_bad) {
+        atomicExch(bad, 1);
+        if (ever) *reinterpret_cast<volatile int*>(ever) = 1;
+      }
     }
   }
   Raw<WDT, VEC> x[kDeep];
@@ -596,7 +600,7 @@ inline const uint2* sorted_items(const Plan& pl, const void* plan) {
 
 template <int WDT, int ODT>
 int launch_gather(const int64_t* tokens, const void* w, int64_t ldw, float scale, int64_t n, int64_t V, int D,
-                  void* out, int* bad, bool after_sort, cudaStream_t st) {
+                  void* out, int* bad, int* ever, bool after_sort, cudaStream_t st) {
   constexpr int kWide = WDT == SPK_F32 || ODT == SPK_F32 ? 4 : 8;
   const bool wide = D % kWide == 0 && ldw % kWide == 0 && aligned(w, kWide * dtype_size(WDT)) &&
                     aligned(out, kWide * dtype_size(ODT));
@@ -611,7 +615,7 @@ int launch_gather(const int64_t* tokens, const void* w, int64_t ldw, float scale
   const cudaError_t e = cudaLaunchKernelEx(
       &cfg, wide ? gather_kernel<WDT, ODT, kWide> : gather_kernel<WDT, ODT, 1>, tokens,
       reinterpret_cast<const typename Elem<WDT>::T*>(w), ldw, scale, n, V, D, tiles,
-      reinterpret_cast<typename Elem<ODT>::T*>(out), bad, extra, scan, after_sort ? 1 : 0);
+      reinterpret_cast<typename Elem<ODT>::T*>(out), bad, ever, extra, scan, after_sort ? 1 : 0);
   return e == cudaSuccess ? check_launch("embedding_fwd") : fail(SPK_ERR_LAUNCH, "embedding_fwd: %s", cudaGetErrorString(e));
 }
 
@@ -638,6 +642,13 @@ int64_t spk_embedding_plan_bytes(int64_t n) { return n < 1 ? 16 : 2 * spk::embg:
 int spk_embedding_fwd(const int64_t* tokens, const void* weight, int w_dtype, int64_t ldw, float scale, int64_t n,
                       int64_t V, int64_t D, void* out, int out_dtype, int* bad_token, int64_t padding_idx, void* plan,
                       int64_t plan_bytes, void* stream) {
+  return spk_embedding_fwd_watched(tokens, weight, w_dtype, ldw, scale, n, V, D, out, out_dtype, bad_token, nullptr,
+                                   padding_idx, plan, plan_bytes, stream);
+}
+
+int spk_embedding_fwd_watched(const int64_t* tokens, const void* weight, int w_dtype, int64_t ldw, float scale,
+                              int64_t n, int64_t V, int64_t D, void* out, int out_dtype, int* bad_token, int* bad_ever,
+                              int64_t padding_idx, void* plan, int64_t plan_bytes, void* stream) {
   using namespace spk;
   using namespace spk::embg;
   SPK_REQUIRE(tokens && weight && out && bad_token, SPK_ERR_INVALID, "null pointer argument");
@@ -647,7 +658,8 @@ int spk_embedding_fwd(const int64_t* tokens, const void* weight, int w_dtype, in
               (long long)D, (long long)ldw);
   SPK_REQUIRE(!plan || plan_bytes >= spk_embedding_plan_bytes(n), SPK_ERR_INVALID,
               "plan smaller than spk_embedding_plan_bytes()");
-  SPK_REQUIRE(aligned(plan, 16), SPK_ERR_ALIGN, "plan must be 16-byte aligned");
+  SPK_REQUIRE(aligned(plan, 16) && aligned(bad_ever, 4), SPK_ERR_ALIGN,
+              "plan must be 16-byte aligned, bad_ever 4-byte aligned");
   int rc = check_stream_device(stream);
   if (rc != SPK_OK) return rc;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
@@ -656,7 +668,7 @@ int spk_embedding_fwd(const int64_t* tokens, const void* weight, int w_dtype, in
     rc = launch_sort(Plan(n, V, D, 8), tokens, n, V, padding_idx, plan, st);
     if (rc != SPK_OK) return rc;
   }
-#define CALL(W, O) return launch_gather<W, O>(tokens, weight, ldw, scale, n, V, (int)D, out, bad_token, plan != nullptr, st)
+#define CALL(W, O) return launch_gather<W, O>(tokens, weight, ldw, scale, n, V, (int)D, out, bad_token, bad_ever, plan != nullptr, st)
   SPK_EMB_TYPES(w_dtype, out_dtype, CALL);
 #undef CALL
 }

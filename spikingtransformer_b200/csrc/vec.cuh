@@ -55,9 +55,9 @@ __device__ __forceinline__ void st_any(void* p, int dt, int64_t i, float v) {
 // Whether a token lies outside [0, V) and is not `ignore`, by one block: the only
 // writer of *bad, so nothing has to clear it first.  For up to kScanTokens tokens
 // (a few microseconds beside the other blocks); more are marked by the blocks
-// that meet them, after a memset.
+// that meet them, after a memset.  Returns whether there is one.
 constexpr int64_t kScanTokens = 16384;
-__device__ __forceinline__ void scan_tokens(const int64_t* __restrict__ tokens, int64_t n, int64_t V, int64_t ignore,
+__device__ __forceinline__ bool scan_tokens(const int64_t* __restrict__ tokens, int64_t n, int64_t V, int64_t ignore,
                                             int* bad) {
   int any = 0;
 #pragma unroll 8
@@ -67,6 +67,7 @@ __device__ __forceinline__ void scan_tokens(const int64_t* __restrict__ tokens, 
   }
   any = __syncthreads_or(any);
   if (threadIdx.x == 0) *bad = any;
+  return any;
 }
 
 inline bool float_type(int dt) { return dt == SPK_F32 || dt == SPK_F16 || dt == SPK_BF16; }

@@ -4,6 +4,9 @@ Every function requires CUDA tensors and raises on CPU input: there is no
 CPU implementation in this package.
 """
 
+import ctypes
+import threading
+
 import torch
 from torch.autograd import forward_ad
 
@@ -829,6 +832,46 @@ def _tokens_i64(tokens):
 EMBEDDING_DTYPES = tuple(_FLOATS)  # weights that embedding takes
 
 
+class BadTokens:
+    """Whether any call given this as ``watch`` met a token outside its vocabulary: a word
+    of page-locked host memory that the kernels set and nothing but ``clear`` resets,
+    so that looking at it waits for no device (and sees calls that have run by
+    then).  The word stays allocated for good, since a kernel in flight may write it
+    when its owner is gone; a copy, or one from a pickle, has a word of its own."""
+
+    _lock = threading.Lock()
+    _page, _left = None, 0  # the words not yet handed out
+    _pages = []
+
+    def __init__(self):
+        self._word = None
+
+    def address(self):
+        if self._word is None:
+            with self._lock:
+                if self._word is None:
+                    cls = BadTokens
+                    if cls._left == 0:
+                        cls._page, cls._left = torch.zeros(1024, dtype=torch.int32, pin_memory=True), 1024
+                        cls._pages.append(cls._page)
+                    cls._left -= 1
+                    self._word = ctypes.c_int32.from_address(cls._page.data_ptr() + 4 * cls._left)
+        return ctypes.addressof(self._word)
+
+    def seen(self):
+        return self._word is not None and self._word.value != 0
+
+    def clear(self):
+        if self._word is not None:
+            self._word.value = 0
+
+    def __deepcopy__(self, memo):
+        return BadTokens()
+
+    def __reduce__(self):
+        return BadTokens, ()
+
+
 def _check_embedding(tokens, weight, out_dtype):
     """``(device, output type, int64 tokens)`` of a lookup with these arguments."""
     dev = _one_device(weight, tokens)
@@ -845,10 +888,10 @@ def embedding_fwd(tokens, weight, scale=1.0, out_dtype=None):
     [*tokens.shape, D] in out_dtype (the weight's by default), bad)``; ``bad`` is
     a device flag, 1 if a token lies outside ``[0, V)`` (its row is zeros)."""
     dev, dt, tokens = _check_embedding(tokens, weight, out_dtype)
-    return _embedding_fwd(dev, tokens, weight, scale, dt, None, -1)
+    return _embedding_fwd(dev, tokens, weight, scale, dt, None, -1, None)
 
 
-def _embedding_fwd(dev, tokens, weight, scale, dt, plan, padding_idx):
+def _embedding_fwd(dev, tokens, weight, scale, dt, plan, padding_idx, watch):
     V, D = weight.shape
     weight, ld = _rows_of(weight)
     n = tokens.numel()
@@ -856,9 +899,10 @@ def _embedding_fwd(dev, tokens, weight, scale, dt, plan, padding_idx):
     if n == 0:
         return out, torch.zeros(1, dtype=torch.int32, device=dev)
     bad = torch.empty(1, dtype=torch.int32, device=dev)
-    _lib.launch(dev, "spk_embedding_fwd", "embedding_fwd", 1 if plan is None else 2, n * (8 + D * (weight.itemsize + out.itemsize)),
-                tokens.data_ptr(), weight.data_ptr(), _FLOATS[weight.dtype], ld, float(scale), n, V, D, out.data_ptr(),
-                _FLOATS[dt], bad.data_ptr(), padding_idx, None if plan is None else plan.data_ptr(),
+    _lib.launch(dev, "spk_embedding_fwd_watched", "embedding_fwd", 1 if plan is None else 2,
+                n * (8 + D * (weight.itemsize + out.itemsize)), tokens.data_ptr(), weight.data_ptr(),
+                _FLOATS[weight.dtype], ld, float(scale), n, V, D, out.data_ptr(), _FLOATS[dt], bad.data_ptr(),
+                None if watch is None else watch.address(), padding_idx, None if plan is None else plan.data_ptr(),
                 0 if plan is None else plan.numel())
     return out, bad
 
@@ -910,9 +954,9 @@ def _embedding_bwd_composed(g, tokens, V, scale, padding_idx, dtype):
 
 class _Embedding(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, weight, tokens, scale, padding_idx, dev, dt):
+    def forward(ctx, weight, tokens, scale, padding_idx, dev, dt, watch):
         plan = _embedding_plan(dev, tokens)
-        out, bad = _embedding_fwd(dev, tokens, weight, scale, dt, plan, padding_idx)
+        out, bad = _embedding_fwd(dev, tokens, weight, scale, dt, plan, padding_idx, watch)
         ctx.save_for_backward(plan, tokens)
         ctx.meta = dev, weight.shape[0], scale, padding_idx, weight.dtype
         ctx.mark_non_differentiable(bad)
@@ -922,14 +966,16 @@ class _Embedding(torch.autograd.Function):
     @staticmethod
     def backward(ctx, g, _g_bad):
         if g is None:
-            return None, None, None, None, None, None
+            return (None,) * 7
         plan, tokens = ctx.saved_tensors
         dev, V, scale, padding_idx, dtype = ctx.meta
         if torch._C._functorch.is_legacy_batchedtensor(g) or _dual(g):  # the former with is_grads_batched=True
-            return _embedding_bwd_composed(g, tokens, V, scale, padding_idx, dtype), None, None, None, None, None
-        if torch.is_grad_enabled():
-            return _EmbeddingGrad.apply(g, plan, tokens, ctx.meta), None, None, None, None, None
-        return _embedding_bwd(dev, g, None, plan, V, scale, padding_idx, dtype), None, None, None, None, None
+            gw = _embedding_bwd_composed(g, tokens, V, scale, padding_idx, dtype)
+        elif torch.is_grad_enabled():
+            gw = _EmbeddingGrad.apply(g, plan, tokens, ctx.meta)
+        else:
+            gw = _embedding_bwd(dev, g, None, plan, V, scale, padding_idx, dtype)
+        return gw, None, None, None, None, None, None
 
 
 class _EmbeddingGrad(torch.autograd.Function):
@@ -952,19 +998,22 @@ class _EmbeddingGrad(torch.autograd.Function):
         return embedding(tokens, gg, scale, out_dtype=dtype)[0], None, None, None
 
 
-def embedding(tokens, weight, scale=1.0, padding_idx=None, out_dtype=None):
+def embedding(tokens, weight, scale=1.0, padding_idx=None, out_dtype=None, watch=None):
     """Differentiable scaled token embedding (``Seq2Seq.py:29-36``: ``embedding(tokens)
     * sqrt(D)``): ``embedding_fwd`` with the weight's gradient of
     ``embedding_bwd``.  ``padding_idx`` (0 <= padding_idx < V, or None): the row
-    that takes no gradient.  Returns ``(out, bad)``."""
+    that takes no gradient.  ``watch``: a ``BadTokens`` that the call sets beside
+    ``bad``, or None.  Returns ``(out, bad)``."""
     dev, dt, tokens = _check_embedding(tokens, weight, out_dtype)
     if padding_idx is None:
         padding_idx = -1
     elif not 0 <= padding_idx < weight.shape[0]:
         raise ValueError("padding_idx %d outside [0, %d)" % (padding_idx, weight.shape[0]))
+    if watch is not None and type(watch) is not BadTokens:
+        raise TypeError("watch must be a BadTokens (got %s)" % type(watch).__name__)
     if torch.is_grad_enabled() and weight.requires_grad or _dual(weight):
-        return _Embedding.apply(weight, tokens, scale, padding_idx, dev, dt)
-    return _embedding_fwd(dev, tokens, weight, scale, dt, None, -1)
+        return _Embedding.apply(weight, tokens, scale, padding_idx, dev, dt, watch)
+    return _embedding_fwd(dev, tokens, weight, scale, dt, None, -1, watch)
 
 
 MAX_TOP_K = 32  # alternatives that token_logprobs can return

@@ -1028,6 +1028,79 @@ def test_token_embedding_under_forward_mode_and_function_transforms(device):
     traced = torch.jit.trace(m, (tok,), check_trace=False)
     other = (tok + 1) % 9
     assert torch.equal(traced(other), m(other))
+    compiled = torch.compile(m, backend="eager", fullgraph=True)
+    assert torch.equal(compiled(other), m(other))
+
+
+def test_token_embedding_is_copied_and_saved_without_its_flag():
+    import copy
+    import io
+    from spikingtransformer_b200.Seq2Seq import TokenEmbedding
+    m = TokenEmbedding(9, 16)
+    tok = torch.arange(9)
+    file = io.BytesIO()
+    torch.save(m, file)
+    file.seek(0)
+    for other in (copy.deepcopy(m), copy.copy(m), torch.load(file, weights_only=False)):
+        assert torch.equal(other(tok), m(tok)) and other.bad_tokens == 0
+    assert copy.deepcopy(m)._watch is not m._watch
+    state = dict(m.__dict__, bad_tokens=torch.ones(1))  # saved when the flag was a tensor
+    del state["_watch"]
+    old = TokenEmbedding.__new__(TokenEmbedding)
+    old.__setstate__(state)
+    assert torch.equal(old(tok), m(tok)) and old.bad_tokens == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [3, 4096, 20000])  # tokens looked through by one block, or marked by those that meet them
+@pytest.mark.parametrize("train", [False, True])
+def test_token_embedding_raises_after_tokens_outside_the_vocabulary(ops, n, train):
+    import copy
+    from spikingtransformer_b200.Seq2Seq import TokenEmbedding
+    m, other = TokenEmbedding(50, 96).to(DEV).requires_grad_(train), TokenEmbedding(60, 96).to(DEV)
+    tok = torch.randint(0, 50, (n,), generator=gen(n)).to(DEV)
+    want = (m.embedding.weight[tok] * 96 ** 0.5).detach()
+    for wrong in (50, -1):
+        bad = tok.clone()
+        bad[n - 1] = wrong
+        m(tok)
+        m(bad)
+        if wrong == 50:
+            other(bad)  # inside this one's vocabulary
+        torch.cuda.synchronize()
+        twin = copy.deepcopy(m)
+        with pytest.raises(IndexError):
+            m(tok)
+        for e in (m, other, twin):  # told once, and to its owner alone
+            assert e.bad_tokens == 0
+            e(tok)
+        assert torch.equal(m(tok), want)
+    m(bad)
+    try:  # a later call that comes too early to see it does not clear it
+        m(tok)
+    except IndexError:
+        return
+    assert m.bad_tokens == 1
+
+
+@pytest.mark.gpu
+def test_token_embedding_tells_of_tokens_in_a_replayed_graph(ops):
+    from spikingtransformer_b200.Seq2Seq import TokenEmbedding
+    m = TokenEmbedding(50, 96).to(DEV)
+    tok = torch.zeros(64, dtype=torch.int64, device=DEV)
+    TokenEmbedding(2, 8).to(DEV)(tok)  # the library is loaded; m's first call is the captured one
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = m(tok)
+        (gw,) = torch.autograd.grad(out, m.embedding.weight, torch.ones_like(out))
+    graph.replay()
+    assert m.bad_tokens == 0 and torch.equal(gw[0], torch.full((96,), 64 * 96 ** 0.5, device=DEV))
+    tok[5] = 77
+    graph.replay()
+    assert m.bad_tokens == 1
+    with pytest.raises(IndexError):
+        m(tok)
 
 
 @pytest.mark.gpu
