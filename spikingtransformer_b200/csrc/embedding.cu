@@ -20,6 +20,9 @@
 //   join    adds the parts of the tokens that reach over chunks, in order.
 // A chunk costs the same whatever its tokens are, so a token that fills half the
 // batch (padding, a space) is spread over the machine like any other.
+#include <atomic>
+#include <cstdlib>
+
 #include "vec.cuh"
 
 namespace spk {
@@ -569,12 +572,46 @@ inline int bwd_vec(const void* g, int g_dtype, const void* gw, int w_dtype, int6
   return D % v == 0 && aligned(g, v * dtype_size(g_dtype)) && aligned(gw, v * dtype_size(w_dtype)) ? v : 1;
 }
 
+// The most blocks of a cluster of the sort that the current device can hold: 16 (not
+// portable) where a partition or another program's claim leaves room for them, else 8.
+// Asked once a device.  SPK_SORT_CLUSTER=8 leaves the 16 out (for tests).
+inline int largest_cluster() {
+  static std::atomic<int> known[64];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 8;
+  int most = known[dev].load(std::memory_order_relaxed);
+  if (most) return most;
+  const char* env = getenv("SPK_SORT_CLUSTER");
+  most = env && atoi(env) == 8 ? 8 : 16;
+  if (most == 16) {
+    constexpr int kSmem = ((kSortWarps + 2) << kMaxDigit) * 4;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(16);
+    cfg.blockDim = dim3(kSortThreads);
+    cfg.dynamicSmemBytes = kSmem;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim = {16, 1, 1};
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    int clusters = 0;
+    if (cudaFuncSetAttribute(sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) != cudaSuccess ||
+        cudaFuncSetAttribute(sort_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess ||
+        cudaOccupancyMaxActiveClusters(&clusters, (const void*)sort_kernel, &cfg) != cudaSuccess || clusters < 1) {
+      cudaGetLastError();  // the answer is no, and no error of the call's
+      most = 8;
+    }
+  }
+  known[dev].store(most, std::memory_order_relaxed);
+  return most;
+}
+
 // The items in order: in plan, or in plan + its second half.
 int launch_sort(const Plan& pl, const int64_t* tokens, int64_t n, int64_t V, int64_t padding_idx, void* plan,
                 cudaStream_t st) {
   uint2* item0 = reinterpret_cast<uint2*>(plan);
   uint2* item1 = reinterpret_cast<uint2*>(reinterpret_cast<char*>(plan) + pl.items);
-  const int csize = n <= 4096 ? 1 : n <= 32768 ? 8 : 16;
+  const int csize = n <= 4096 ? 1 : n <= 32768 ? 8 : largest_cluster();
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)csize);
   cfg.blockDim = dim3(kSortThreads);

@@ -508,6 +508,34 @@ def test_embedding_token_types_layouts_and_empty_input(ops):
     assert out.shape == (0, 3, D) and int(bad) == 0 and not g3.any()
 
 
+SORT_TWICE = """
+import torch
+from spikingtransformer_b200 import ops
+g = torch.Generator().manual_seed(1)
+n, V, D = 40000, 5000, 24
+tok = torch.randint(0, V, (n,), generator=g)
+gi = torch.randint(-9, 10, (n, D), generator=g).float()
+want = torch.zeros(V, D).index_add_(0, tok, gi)
+w = torch.zeros(V, D, device="cuda", requires_grad=True)
+out, _ = ops.embedding(tok.cuda(), w)
+got = [torch.autograd.grad(out, w, gi.cuda())[0], ops.embedding_bwd(gi.cuda(), tok.cuda(), V)]
+assert all(torch.equal(t.cpu(), want) for t in got)
+"""
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("largest", ["8", "16"])
+def test_embedding_sorts_without_the_largest_clusters(largest):
+    """A device that holds no cluster of 16 blocks sorts many tokens with 8."""
+    import os
+    import subprocess
+    import sys
+    env = dict(os.environ, SPK_SORT_CLUSTER=largest)
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", SORT_TWICE], cwd=root, env=env, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]
+
+
 # ------------------------------------------------------------------ token log probabilities
 
 
