@@ -547,7 +547,7 @@ int spk_embedding_bwd(const int64_t* tokens, const void* g, int g_dtype, float s
  * Log probabilities of given tokens under the mean over T of the logits, with
  * entropy and the top_k (<= 32) largest alternatives (falling, ties to the
  * lower index, NaN smallest).  logits: element (t, r, v) of dtype
- * (F32/F16/BF16) at t*step_stride + r*row_stride + v; tokens: [rows];
+ * (F32/F16/BF16) at t*step_stride + r*row_stride + v, T <= 64 as in the LIF; tokens: [rows];
  * logp, entropy: [rows]; top_logp, top_idx: [rows][top_k] (NULL with top_k 0);
  * stats: [rows][4] for the backward, 16-byte aligned (NULL: none).  Rows whose token is ignore_index give
  * zeros and top_idx -1; so do tokens outside [0, V), which set *bad_token

@@ -1017,6 +1017,7 @@ def embedding(tokens, weight, scale=1.0, padding_idx=None, out_dtype=None, watch
 
 
 MAX_TOP_K = 32  # alternatives that token_logprobs can return
+MAX_STEPS = 64  # steps that it takes the mean of: as many as a LIF can make
 
 
 def _logit_rows(logits):
@@ -1090,7 +1091,7 @@ def token_logprobs(logits, tokens, top_k=0, ignore_index=-100):
     """Log probabilities of given tokens under the T-averaged logits (the
     distribution whose argmax the metric and the greedy decoding take), with
     entropy and alternatives.  ``logits``: ``[T, ..., V]`` fp32, fp16 or bf16
-    (T = 1 for plain logits: ``x.unsqueeze(0)``; slices are read in place);
+    (1 <= T <= 64; T = 1 for plain logits: ``x.unsqueeze(0)``; slices are read in place);
     ``tokens``: ``[...]`` integers.  Returns ``(logp [...], entropy [...],
     top_logp [..., top_k], top_idx [..., top_k], bad)``, fp32 and int64,
     ``top_*`` None with ``top_k`` 0 (at most 32).  Alternatives come in falling
@@ -1106,6 +1107,8 @@ def token_logprobs(logits, tokens, top_k=0, ignore_index=-100):
     if logits.dim() < 2 or logits.shape[0] < 1 or logits.shape[-1] < 1 or logits.shape[1:-1] != tokens.shape:
         raise RuntimeError("tokens %s do not match logits %s ([T, ..., V])"
                            % (tuple(tokens.shape), tuple(logits.shape)))
+    if logits.shape[0] > MAX_STEPS:
+        raise ValueError("token_logprobs takes at most %d steps (got %d)" % (MAX_STEPS, logits.shape[0]))
     if not 0 <= top_k <= min(MAX_TOP_K, logits.shape[-1]):
         raise ValueError("top_k must be between 0 and min(%d, V) (got %d)" % (MAX_TOP_K, top_k))
     tokens = _tokens_i64(tokens)

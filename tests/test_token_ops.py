@@ -915,6 +915,22 @@ def test_token_logprobs_gradient_against_differences(ops):
     assert abs((gx.cpu().double() * v).sum() - diff) <= bound
 
 
+@pytest.mark.gpu
+def test_steps_up_to_those_of_a_lif(ops):
+    """64 steps give the mean's values; 65 are refused, as by the LIF."""
+    x = torch.randn(65, 3, 40, generator=gen(1))
+    tok = torch.tensor([0, 39, 7])
+    o = lp_exact(x[:64], tok, 0)
+    logp, H = ops.token_logprobs(x[:64].to(DEV), tok.to(DEV))[:2]
+    assert_within(logp, o["logp"], o["e_logp"], "logp")
+    assert_within(H, o["entropy"], o["e_H"], "entropy")
+    with pytest.raises(ValueError, match="64 steps"):
+        ops.token_logprobs(x.to(DEV), tok.to(DEV))
+    one = torch.ones(1, device=DEV)
+    with pytest.raises(RuntimeError, match="64"):
+        ops.lif_fwd(x.to(DEV), one, one, one)
+
+
 # ------------------------------------------------------------------ in the model
 
 
