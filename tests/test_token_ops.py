@@ -782,6 +782,46 @@ def test_alternatives_of_rows_with_more_nans_than_numbers(ops, T, rows, V, dtype
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("V", [40, 300, 5000, 5001])
+def test_infinities_among_the_steps(ops, V):
+    """The mean over the steps where some are not finite, or their partial sums are not:
+    -inf in the first, a later or every step bars the symbol, steps of +-3e38 whose
+    mean is finite do not, +inf, NaN or both infinities take the row."""
+    T, rows, K = 3, 10, 4
+    x = torch.randn(T, rows, V, generator=gen(V))
+    inf = float("inf")
+    for c, steps in enumerate([(-inf, 1.0, 2.0), (1.0, -inf, 2.0), (1.0, 2.0, -inf), (-inf,) * 3, (-inf, -3e38, -3e38),
+                               (-3e38, -3e38, -inf), (3e38, 3e38, -inf), (3e38, 3e38, -3e38 * 2 + 3.4e38),
+                               (3.25, -3e38, 3e38)]):
+        x[:, :, 5 + c] = torch.tensor(steps)[:, None]
+    x[:, 0:6, 12] = 0.0  # the rows whose symbols are all of ordinary size but the barred ones
+    x[1, 1, 30] = inf
+    x[:, 2, 30] = torch.tensor([inf, -inf, 0.0])
+    x[:, 3, 30] = torch.tensor([-inf, 0.0, inf])
+    x[2, 4, 30] = float("nan")
+    x[:, 5, 30] = torch.tensor([float("nan"), -inf, 0.0])
+    tok = torch.zeros(rows, dtype=torch.int64)
+    z = x.double().mean(0)
+    z[:, 13] = 3.25 / 3  # 64 bits lose the 3.25 beside 3e38
+    o = lp_exact(z.float()[None], tok, K)
+    xd = x.to(DEV).requires_grad_(True)
+    logp, H, top, idx, _ = ops.token_logprobs(xd, tok.to(DEV), top_k=K)
+    gl = torch.randn(rows, generator=gen(1))
+    (gx,) = torch.autograd.grad(logp, xd, gl.to(DEV))
+    d, e = lp_grad_exact(o, gl, None, None, T, torch.float32)
+    for r in range(1, 6):
+        assert logp[r].isnan() and H[r].isnan() and gx[:, r].isnan().all()
+    for r in (0, 6, 7, 8, 9):
+        assert torch.equal(idx[r].cpu(), o["top_idx"][r])
+        if r == 0:
+            assert_within(logp[r], o["logp"][r], o["e_logp"][r], "logp")
+            assert_within(H[r], o["entropy"][r], o["e_H"][r], "entropy")
+            assert_within(gx[0, r], d[r], e[r], "grad")
+        else:  # one symbol near 1e38 takes it all
+            assert float(top[r, 0]) == 0 and int(idx[r, 0]) == 12 and float(H[r]) == 0
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("V", [48, 300, 9000])
 @pytest.mark.parametrize("dtype", FLOATS)
 def test_lowest_values_are_above_minus_infinity(ops, V, dtype):
