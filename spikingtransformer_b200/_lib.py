@@ -131,11 +131,13 @@ class LaunchRecorder:
         global _recorder
         self._prev = _recorder
         _recorder = self
+        _tell_watchers()
         return self
 
     def __exit__(self, *exc):
         global _recorder
         _recorder = self._prev
+        _tell_watchers()
         return False
 
     def summary(self):
@@ -162,11 +164,13 @@ class LaunchCounter:
         global _counter
         self._prev = _counter
         _counter = self
+        _tell_watchers()
         return self
 
     def __exit__(self, *exc):
         global _counter
         _counter = self._prev
+        _tell_watchers()
         return False
 
     def total(self):
@@ -175,6 +179,24 @@ class LaunchCounter:
 
 _recorder = None
 _counter = None
+_watchers = []
+
+
+def watching():
+    """Whether launches are being recorded or counted."""
+    return _recorder is not None or _counter is not None
+
+
+def on_watch(fn):
+    """``fn(watching())`` now and whenever a recorder or counter begins or ends: for code that
+    launches without ``call``."""
+    _watchers.append(fn)
+    fn(watching())
+
+
+def _tell_watchers():
+    for fn in _watchers:
+        fn(watching())
 
 
 def call(name, *args, tag=None, work=None):

@@ -4,6 +4,8 @@ Each ``csrc/*.cu`` file is compiled to an object with nvcc in parallel, then
 linked into ``spikingtransformer_b200/libspk.so``.  The CUDA runtime is linked
 statically; the driver API entry point used for TMA descriptors is resolved at
 run time (``cudaGetDriverEntryPoint``), so the library needs no ``-lcuda``.
+``csrc/embedding_autograd.cpp`` becomes the Python module ``_autograd.so`` beside
+it, against the running torch's headers and libraries and ``libspk.so``.
 
     python -m spikingtransformer_b200.build [--force] [-j N]
 """
@@ -14,12 +16,15 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 PKG = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(PKG, "csrc")
 INCLUDE = os.path.join(os.path.dirname(PKG), "include")
 BUILD = os.path.join(PKG, "_build")
 LIB = os.path.join(PKG, "libspk.so")
+NODES = os.path.join(CSRC, "embedding_autograd.cpp")
+NODES_LIB = os.path.join(PKG, "_autograd.so")
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC,-O2", "--expt-relaxed-constexpr",
@@ -59,10 +64,44 @@ def needs_build():
     return any(os.path.getmtime(f) > t for f in _sources() + _headers() + [__file__])
 
 
+def nodes_need_build():
+    if not os.path.exists(NODES_LIB):
+        return True
+    t = os.path.getmtime(NODES_LIB)
+    return any(os.path.getmtime(f) > t for f in [NODES, os.path.join(INCLUDE, "spk.h"), __file__])
+
+
+def build_nodes(force=False):
+    """Compile the autograd nodes (after libspk.so, which they are linked to)."""
+    if not force and not nodes_need_build():
+        return NODES_LIB
+    import torch
+    at = os.path.dirname(torch.__file__)
+    cuda = os.path.dirname(os.path.dirname(os.path.realpath(nvcc())))
+    tmp = NODES_LIB + ".tmp"
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-D_GLIBCXX_USE_CXX11_ABI=%d" % torch._C._GLIBCXX_USE_CXX11_ABI,
+           "-I" + INCLUDE, "-I" + os.path.join(at, "include"),
+           "-I" + os.path.join(at, "include", "torch", "csrc", "api", "include"),
+           "-I" + sysconfig.get_paths()["include"], "-I" + os.path.join(cuda, "include"), NODES, "-o", tmp,
+           "-L" + os.path.join(at, "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python", "-L" + PKG, "-lspk",
+           "-Wl,-rpath,$ORIGIN"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError("g++ failed for %s:\n%s\n%s" % (NODES, " ".join(cmd), r.stderr[-8000:]))
+    os.replace(tmp, NODES_LIB)
+    return NODES_LIB
+
+
 def build(force=False, jobs=None, verbose=False, ptxas_info=False):
-    """Compile every CUDA source for sm_100a and link libspk.so (no-op if fresh)."""
-    if not force and not needs_build():
-        return LIB
+    """Compile every CUDA source for sm_100a, link libspk.so, then the autograd nodes (no-op
+    where they are fresh)."""
+    if force or needs_build():
+        build_library(jobs, verbose, ptxas_info)
+    build_nodes(force)
+    return LIB
+
+
+def build_library(jobs=None, verbose=False, ptxas_info=False):
     os.makedirs(BUILD, exist_ok=True)
     extra = ["-Xptxas", "-v"] if ptxas_info else []
     srcs = _sources()

@@ -943,59 +943,27 @@ def _embedding_bwd(dev, g, tokens, plan, V, scale, padding_idx, dtype):
     return gw
 
 
-def _embedding_bwd_composed(g, tokens, V, scale, padding_idx, dtype):
-    """The same in torch's operations, for a ``g`` that is more than its data (a batch of
-    gradients at once, a tangent)."""
-    used = (tokens >= 0) & (tokens < V)
-    rows = torch.where(used.unsqueeze(-1), g.float(), 0.0)
-    gw = torch.ops.aten.embedding_dense_backward(rows, torch.where(used, tokens, 0), V, padding_idx, False)
-    return (gw * scale).to(dtype)
+_nodes = None
 
 
-class _Embedding(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, weight, tokens, scale, padding_idx, dev, dt, watch):
-        plan = _embedding_plan(dev, tokens)
-        out, bad = _embedding_fwd(dev, tokens, weight, scale, dt, plan, padding_idx, watch)
-        ctx.save_for_backward(plan, tokens)
-        ctx.meta = dev, weight.shape[0], scale, padding_idx, weight.dtype
-        ctx.mark_non_differentiable(bad)
-        ctx.set_materialize_grads(False)
-        return out, bad
-
-    @staticmethod
-    def backward(ctx, g, _g_bad):
-        if g is None:
-            return (None,) * 7
-        plan, tokens = ctx.saved_tensors
-        dev, V, scale, padding_idx, dtype = ctx.meta
-        if torch._C._functorch.is_legacy_batchedtensor(g) or _dual(g):  # the former with is_grads_batched=True
-            gw = _embedding_bwd_composed(g, tokens, V, scale, padding_idx, dtype)
-        elif torch.is_grad_enabled():
-            gw = _EmbeddingGrad.apply(g, plan, tokens, ctx.meta)
-        else:
-            gw = _embedding_bwd(dev, g, None, plan, V, scale, padding_idx, dtype)
-        return gw, None, None, None, None, None, None
+def _embedding_nodes():
+    """The compiled autograd nodes of the embedding (csrc/embedding_autograd.cpp)."""
+    global _nodes
+    if _nodes is None:
+        _lib.load()
+        try:
+            from . import _autograd
+        except ImportError as e:
+            raise RuntimeError("cannot load the autograd nodes (%s); build them with "
+                               "`python -m spikingtransformer_b200.build`" % e) from e
+        _lib.on_watch(lambda on: _autograd.set_watched(_embedding_bwd_watched if on else None))
+        _nodes = _autograd
+    return _nodes
 
 
-class _EmbeddingGrad(torch.autograd.Function):
-    """The weight's gradient as a function of ``g``; it is linear, and its own gradient
-    is the lookup (zeros for padding_idx)."""
-
-    @staticmethod
-    def forward(ctx, g, plan, tokens, meta):
-        dev, V, scale, padding_idx, dtype = meta
-        ctx.save_for_backward(tokens)
-        ctx.meta = scale, padding_idx, g.dtype
-        return _embedding_bwd(dev, g, None, plan, V, scale, padding_idx, dtype)
-
-    @staticmethod
-    def backward(ctx, gg):
-        scale, padding_idx, dtype = ctx.meta
-        tokens = ctx.saved_tensors[0]
-        if padding_idx >= 0:
-            tokens = torch.where(tokens == padding_idx, -1, tokens)
-        return embedding(tokens, gg, scale, out_dtype=dtype)[0], None, None, None
+def _embedding_bwd_watched(g, plan, V, scale, padding_idx, dtype):
+    """The nodes' backward where launches are being counted or timed."""
+    return _embedding_bwd(plan.device, g, None, plan, V, scale, padding_idx, dtype)
 
 
 def embedding(tokens, weight, scale=1.0, padding_idx=None, out_dtype=None, watch=None):
@@ -1011,9 +979,17 @@ def embedding(tokens, weight, scale=1.0, padding_idx=None, out_dtype=None, watch
         raise ValueError("padding_idx %d outside [0, %d)" % (padding_idx, weight.shape[0]))
     if watch is not None and type(watch) is not BadTokens:
         raise TypeError("watch must be a BadTokens (got %s)" % type(watch).__name__)
-    if torch.is_grad_enabled() and weight.requires_grad or _dual(weight):
-        return _Embedding.apply(weight, tokens, scale, padding_idx, dev, dt, watch)
-    return _embedding_fwd(dev, tokens, weight, scale, dt, None, -1, watch)
+    if _dual(weight):
+        raise NotImplementedError("embedding has no forward-mode derivative")
+    if not (torch.is_grad_enabled() and weight.requires_grad):
+        return _embedding_fwd(dev, tokens, weight, scale, dt, None, -1, watch)
+    nodes = _embedding_nodes()
+    if not _lib.watching():
+        return nodes.embedding(weight, tokens, scale, padding_idx, dt, 0 if watch is None else watch.address())
+    plan = _embedding_plan(dev, tokens)
+    with torch.no_grad():
+        out, bad = _embedding_fwd(dev, tokens, weight, scale, dt, plan, padding_idx, watch)
+    return nodes.attach(out, weight, tokens, plan, scale, padding_idx), bad
 
 
 MAX_TOP_K = 32  # alternatives that token_logprobs can return

@@ -87,6 +87,15 @@ def test_ops_refuse_cpu_tensors(ops):
             call()
 
 
+def test_autograd_nodes_load_and_report_their_errors(ops):
+    """The compiled nodes load without a device, and refuse what has no data."""
+    nodes = ops._embedding_nodes()
+    assert nodes is ops._embedding_nodes()
+    with pytest.raises(RuntimeError, match="data"):
+        nodes.embedding(torch.empty(4, 8, device="meta"), torch.zeros(2, dtype=torch.int64, device="meta"), 1.0, -1,
+                        torch.float32, 0)
+
+
 @pytest.mark.gpu
 def test_ops_refuse_what_they_do_not_take(ops):
     x = torch.randn(4, 8, device=DEV)
@@ -460,6 +469,68 @@ def test_embedding_gradients_in_a_batch(ops):
     for i in range(3):
         want = scatter_exact(tok.flatten(), g[i].reshape(30, 12).cpu(), 7, 0.5, 2)
         assert torch.equal(got[i].cpu().double(), want)
+
+
+@pytest.mark.gpu
+def test_embedding_launches_are_counted_and_recorded(ops):
+    """A counter or recorder around both directions, one of them, or neither sees the
+    launches inside it (lookup and sort, sums and join), with equal results."""
+    tok = torch.randint(0, 50, (6, 40), generator=gen(1)).to(DEV)
+    w = torch.randn(50, 24, generator=gen(2)).to(DEV).requires_grad_(True)
+    g = torch.randn(6, 40, 24, generator=gen(3)).to(DEV)
+    out, bad = ops.embedding(tok, w, 2.0)
+    want = out, torch.autograd.grad(out, w, g)[0]
+    for kind in (_lib.LaunchCounter, _lib.LaunchRecorder):
+        def seen(c):
+            return c.counts if kind is _lib.LaunchCounter else {k: v["launches"] for k, v in c.summary().items()}
+        with kind() as both:
+            out, bad = ops.embedding(tok, w, 2.0)
+            (gw,) = torch.autograd.grad(out, w, g, retain_graph=True)
+        with kind() as backward:
+            (again,) = torch.autograd.grad(out, w, g)
+        with kind() as forward:
+            out2, _ = ops.embedding(tok, w, 2.0)
+        (gw2,) = torch.autograd.grad(out2, w, g)
+        assert seen(both) == {"embedding_fwd": 2, "embedding_bwd": 2}
+        assert seen(backward) == {"embedding_bwd": 2} and seen(forward) == {"embedding_fwd": 2}
+        for t, v in ((out, want[0]), (out2, want[0]), (gw, want[1]), (again, want[1]), (gw2, want[1])):
+            assert torch.equal(t, v)
+        assert int(bad) == 0
+
+
+@pytest.mark.gpu
+def test_embedding_node_keeps_to_torchs_rules(ops):
+    """A second backward needs retain_graph, tokens changed in place after the lookup are
+    an error, an unused result has no gradient, and a row-strided, transposed or empty
+    weight or token tensor is read as it is."""
+    tok = torch.randint(0, 9, (20,), generator=gen(1)).to(DEV)
+    w = torch.randn(9, 16, generator=gen(2)).to(DEV).requires_grad_(True)
+    out, _ = ops.embedding(tok, w)
+    out.sum().backward()
+    with pytest.raises(RuntimeError, match="second time"):
+        out.sum().backward()
+    counts = torch.bincount(tok, minlength=9).float().unsqueeze(1).expand(9, 16)
+    assert torch.equal(w.grad, counts)
+    out, _ = ops.embedding(tok, w)
+    tok2 = tok.clone()
+    out2, _ = ops.embedding(tok2, w)
+    tok2 += 1
+    with pytest.raises(RuntimeError, match="inplace|in-place"):
+        out2.sum().backward()
+    assert torch.autograd.grad((out * 0 + w.sum()).sum(), w)[0].eq(320).all()
+    for leaf in (torch.randn(9, 40, generator=gen(3))[:, 3:19], torch.randn(16, 9, generator=gen(4)).t()):
+        leaf = leaf.to(DEV).detach()
+        base = leaf.clone(memory_format=torch.contiguous_format)
+        leaf.requires_grad_(True)
+        out, _ = ops.embedding(tok, leaf, 0.5)
+        (gw,) = torch.autograd.grad(out.sum(), leaf)
+        assert torch.equal(out, base[tok] * 0.5) and torch.equal(gw, counts * 0.5)
+    for dt in FLOATS:
+        out, _ = ops.embedding(tok, w, 3.0, out_dtype=dt)
+        (gw,) = torch.autograd.grad(out, w, torch.ones_like(out))
+        assert out.dtype == dt and gw.dtype == torch.float32 and torch.equal(gw, counts * 3)
+    with pytest.raises(TypeError):
+        ops.embedding(tok, w, watch=1)
 
 
 @pytest.mark.gpu
