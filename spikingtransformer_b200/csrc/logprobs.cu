@@ -662,7 +662,8 @@ constexpr int kWarpRow = 1024, kManyRow = 8192;
 // Without alternatives bound by instructions more than by HBM: 8192 x 65536 bf16
 // (1.07 GB) take 213 us, 0.78 of a plain copy's rate, at 80 % of the issue slots;
 // with 5 alternatives 389 us, with 32 537 us.  16384 x 256 fp32 of 4 steps: 27 us,
-// with 5 alternatives 37 us, where a row's reductions cost more than its values.
+// with 5 alternatives 37 us, bound by latency (half of the issue slots, 43 and 33 %
+// of the warps: a warp waits for its one row's copies and reductions).
 // GT = 32: a warp a row.  GT = 256: a block a (row, split); with several splits
 // the state and list go to part / keys.
 template <int DT, int VEC, int U, int GT, bool TOP>
@@ -949,7 +950,10 @@ int dispatch_fwd(bool wide, const Logits& x, const int64_t* tokens, int64_t igno
   constexpr int kWide = 16 / (int)sizeof(typename Elem<DT>::T);
 #define GO(VEC, U, GT) launch_fwd<DT, VEC, U, GT>(x, tokens, ignore, K, splits, o, part, keys, bad, st)
   if (warp_rows(x.rows, x.V)) return wide ? GO(kWide, 8 / kWide, 32) : GO(1, 8, 32);
-  if (x.V <= 4096) return wide ? GO(kWide, 1, 256) : GO(1, 4, 256);  // shorter tiles: fewer threads without a value
+  // Shorter tiles: fewer threads without a value.  Shorter / longer, us: 10 x 1003 x 1000 fp32
+  // 21 / 35 (with 5 alternatives 37 / 55), 4096 x 2048 bf16 25 / 29 (51 / 53), 4096 x 4096 31 / 29
+  // (59 / 55), 2048 x 8192 23 / 21 (41 / 37).
+  if (x.V <= 4096) return wide ? GO(kWide, 1, 256) : GO(1, 4, 256);
   return wide ? GO(kWide, 16 / kWide, 256) : GO(1, 8, 256);
 #undef GO
 }
@@ -971,7 +975,9 @@ int dispatch_bwd(bool wide, const Logits& x, const int64_t* tokens, int64_t igno
   constexpr int kWide = 16 / (int)sizeof(typename Elem<DT>::T);
 #define GO(VEC, U, GT) launch_bwd<DT, VEC, U, GT>(x, tokens, ignore, K, splits, g, grad, st)
   if (warp_rows(x.rows, x.V)) return wide ? GO(kWide, 8 / kWide, 32) : GO(1, 8, 32);
-  if (x.V <= 4096) return wide ? GO(kWide, 1, 256) : GO(1, 4, 256);  // shorter tiles: fewer threads without a value
+  // forward and backward with shorter / longer tiles, us: 10 x 1003 x 1000 fp32 37 / 64, 4096 x
+  // 4096 bf16 53 / 62, 2048 x 8192 41 / 43
+  if (x.V <= 4096) return wide ? GO(kWide, 1, 256) : GO(1, 4, 256);
   return wide ? GO(kWide, 16 / kWide, 256) : GO(1, 8, 256);
 #undef GO
 }

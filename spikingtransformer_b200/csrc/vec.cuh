@@ -55,7 +55,8 @@ __device__ __forceinline__ void st_any(void* p, int dt, int64_t i, float v) {
 // Whether a token lies outside [0, V) and is not `ignore`, by one block: the only
 // writer of *bad, so nothing has to clear it first.  For up to kScanTokens tokens
 // (a few microseconds beside the other blocks); more are marked by the blocks
-// that meet them, after a memset.  Returns whether there is one.
+// that meet them, after a memset: 64 to 4096 tokens looked up 8 us against 10, 16384 12
+// against 14, 131072 43 against 41.  Returns whether there is one.
 constexpr int64_t kScanTokens = 16384;
 __device__ __forceinline__ bool scan_tokens(const int64_t* __restrict__ tokens, int64_t n, int64_t V, int64_t ignore,
                                             int* bad) {
